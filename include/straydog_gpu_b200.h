@@ -338,6 +338,57 @@ int sdx_qsa_attention_gathered(void* handle, const void* state, uint64_t context
 int sdx_attention_batch(void* handle, void* const* states, const uint64_t* contexts, const uint64_t* bases, uint64_t sequences,
                         uint64_t heads, uint64_t kv_heads, float scale, const void* q, const float* k, const float* v, float* out);
 
+/* ---- K/V rows in 8 bits with one scale for each block of 32 positions and head, and the attention, masks and eviction around them ----
+   (no reference counterpart: the reference's K/V formats are sd_kv_format's two). Where the Q8_0 rows above carry eight FP16 scales a row
+   for 256 columns, these carry one F32 scale for 32 rows of 64, 128 or 256 columns. A state is one allocation of sdx_kv8_bytes bytes,
+   16-byte aligned: 2 * kv_heads planes (keys of head 0 .., then values) of `context` rows (a multiple of 32, at most 2^24) of `dim` one-byte
+   codes, then the planes' scales, context / 32 F32 a plane. code 0: int8, value = code * scale, scale = max |x| / 127; code 1: E4M3, scale =
+   max |x| / 448. An infinity is held as its block's largest magnitude, a NaN as 0. Element types are 0 F32, 1 F16, 30 BF16. All arrays of
+   per-sequence numbers and pointers are host arrays, read before the call returns; what they point to is device memory. The calls queue work
+   on the handle's stream and read nothing back; they may be captured into a graph once a call of the same sizes has run (a call that would
+   have to grow a workspace inside a capture is refused). Graphs of one handle share its workspaces: replays and other calls of the handle
+   are to be ordered one behind the other, as on one stream. */
+uint64_t sdx_kv8_bytes(uint64_t context, uint64_t kv_heads, uint64_t dim);
+/* Rows bases[s] .. bases[s] + steps[s] - 1 of every state written from packed rows: keys and values hold the sequences' rows one behind the
+   other, [kv_heads][dim] elements of `type` each, `stride` elements apart (0: kv_heads * dim; rows on 16-byte boundaries). Scales: a block whose
+   first position is written takes max |x| / top of the call's rows in it; a begun block keeps its scale unless the new rows need a larger
+   one, and then its older codes are rounded again in it (code * old / new, to nearest even). What lies behind the last row is not touched. No
+   state may be listed twice. */
+int sdx_kv8_write(void* handle, void* const* states, const uint64_t* contexts, const uint64_t* bases, const uint64_t* steps,
+                  uint64_t sequences, uint64_t kv_heads, uint64_t dim, int code, const void* keys, const void* values, uint64_t stride, int type);
+/* Attention of rows[s] query rows of every sequence over its first lengths[s] positions (the rows' own keys written before). Row i of
+   sequence s sits at position p = lengths[s] - rows[s] + i (below 0 when there are more rows than positions) and sees position j when j <= p
+   and, with a window, j > p - window, or when j < prefixes[s] (prefixes null: none). Score: x = scale * q . k, then cap * tanh(x / cap) when
+   cap > 0, then x - slopes[head] * |p - j| (slopes: [heads] F32 in device memory, or null). out = softmax over the seen positions times the
+   values; a row that sees none is 0. q and out: [heads][dim] F16 or BF16 rows, packed in sequence order, q_stride and out_stride elements
+   apart (0: heads * dim), on 16-byte boundaries; out apart from q. heads / kv_heads <= 128. weights (or null): per sequence [kv_heads]
+   [contexts[s]] F32, to which every seen position's softmax weight is added, summed over the rows and the heads of its K/V head, for at
+   most 64 query rows (rows * heads / kv_heads) a K/V head. Up to 64 such query rows a K/V head run on the decode kernel, more on the prompt
+   kernel. A position's codes and scale must have been written. */
+int sdx_kv8_attention(void* handle, const void* const* states, const uint64_t* contexts, const uint64_t* lengths, const uint64_t* rows,
+                      uint64_t sequences, uint64_t heads, uint64_t kv_heads, uint64_t dim, int code, float scale, float cap,
+                      const float* slopes, uint64_t window, const uint64_t* prefixes, const void* q, uint64_t q_stride,
+                      float* const* weights, void* out, uint64_t out_stride, int type);
+/* The same attention over 16-bit keys and values of packed documents: document d has rows[d] queries and lengths[d] keys, one behind the
+   other in q, out ([heads][dim] rows) and k, v ([kv_heads][dim] rows), each with its own row stride in elements (0: packed), so that the parts
+   of one projection's rows can be given as they are; rows on 16-byte boundaries. A row sees keys of its own document only, by the rule
+   above (a prefix of lengths[d]: every key). What a row does not see does not reach its output, infinities and NaN included. dim 64, 128
+   or 256, type 1 (F16) or 30 (BF16), heads / kv_heads <= 128. */
+int sdx_masked_attention(void* handle, const void* q, uint64_t q_stride, const void* k, uint64_t k_stride, const void* v, uint64_t v_stride,
+                         const uint64_t* rows, const uint64_t* lengths, uint64_t documents, uint64_t heads, uint64_t kv_heads, uint64_t dim,
+                         int type, float scale, float cap, const float* slopes, uint64_t window, const uint64_t* prefixes, void* out,
+                         uint64_t out_stride);
+/* Eviction: of a sequence of more than `keep` positions every K/V head keeps the first `sinks`, the last `recent` and, between them, the
+   keep - sinks - recent positions of greatest weight (weights[s]: [kv_heads][contexts[s]], as sdx_kv8_attention adds them up; equal weights:
+   the lower position; NaN below every number); a sequence of keep positions or fewer is kept whole. The kept rows move, in their order, to
+   positions 0 .. of targets[s] (another state, of target_contexts[s] positions), their weights to target_weights[s] ([kv_heads]
+   [target_contexts[s]]), their positions to kept ([sequences][kv_heads][keep] int32, or null). A target block's scale is the largest among the blocks its
+   rows come from; codes from a block with a smaller one are rounded again in it. Nothing written may overlap what is read or written
+   beside it. Positions behind the kept ones are not touched. The rows keep the rotation they were written with. */
+int sdx_kv8_evict(void* handle, const void* const* states, const uint64_t* contexts, const uint64_t* lengths, const float* const* weights,
+                  uint64_t sequences, uint64_t keep, uint64_t sinks, uint64_t recent, uint64_t kv_heads, uint64_t dim, int code,
+                  void* const* targets, const uint64_t* target_contexts, float* const* target_weights, int32_t* kept);
+
 #ifdef __cplusplus
 }
 #endif

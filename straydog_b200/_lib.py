@@ -81,6 +81,11 @@ SIGNATURES = {
     "sdx_trace_read": ([p, C.POINTER(C.c_int64), u64], i32),
     "sdx_qsa_prompt": ([p, p, u64, u64, u64, u64, u64, f32, p, p], i32),
     "sdx_qsa_attention_rows": ([p, p, u64, u64, p, u64, u64, u64, u64, f32, p, p, u64, p, u64, p], i32),
+    "sdx_kv8_bytes": ([u64, u64, u64], u64),
+    "sdx_kv8_write": ([p, p, p, p, p, u64, u64, u64, i32, p, p, u64, i32], i32),
+    "sdx_kv8_attention": ([p, p, p, p, p, u64, u64, u64, u64, i32, f32, f32, p, u64, p, p, u64, p, p, u64, i32], i32),
+    "sdx_masked_attention": ([p, p, u64, p, u64, p, u64, p, p, u64, u64, u64, u64, i32, f32, f32, p, u64, p, p, u64], i32),
+    "sdx_kv8_evict": ([p, p, p, p, p, u64, u64, u64, u64, u64, u64, i32, p, p, p, p], i32),
     "sdx_attention_batch": ([p, pp, pu64, pu64, u64, u64, u64, f32, p, p, p, p], i32),
 }
 

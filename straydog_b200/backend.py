@@ -40,6 +40,27 @@ def _host(a):
     return a.ctypes.data_as(C.c_void_p)
 
 
+F32, F16, BF16 = 0, 1, 30   # element types (their GGML numbers)
+INT8, E4M3 = 0, 1           # codes of 8-bit K/V rows
+
+
+def _u64(values, count=None):
+    """A host array of 64-bit numbers or device addresses (Buffers too); a uint64 array passes as it is."""
+    if not (isinstance(values, np.ndarray) and values.dtype == np.uint64 and values.flags.c_contiguous):
+        values = np.asarray([v.pointer if isinstance(v, Buffer) else v for v in values], np.uint64)
+    if count is not None and values.size != count:
+        raise StraydogError(f"an array of {values.size} entries for {count} sequences")
+    return values
+
+
+def _at(array):
+    return None if array is None else array.ctypes.data
+
+
+def _pointer(x):
+    return x.pointer if isinstance(x, Buffer) else x
+
+
 class Buffer:
     """A device allocation of the backend (zeroed at creation). base() is its device address."""
 
@@ -66,6 +87,17 @@ class Backend:
         if not self.handle:
             _fail(self.lib)
         self.ordinal = ordinal
+
+    @classmethod
+    def adopt(cls, ordinal, stream):
+        """sdx_adopt: a handle over another library's device and stream (a cudaStream_t's address, 0 for the default stream). Its device
+        pointers are taken as they come: no allocation tracking, no range checks."""
+        self = cls.__new__(cls)
+        self.lib, self.handle, self.ordinal = lib(), None, ordinal
+        self.handle = self.lib.sdx_adopt(ordinal, stream or None)
+        if not self.handle:
+            _fail(self.lib)
+        return self
 
     def _c(self, result):
         return _check(result, self.lib)
@@ -312,6 +344,57 @@ class Backend:
         self._c(self.lib.sdx_attention_batch(self.handle, ptrs, ctx, bs, n, heads, kv_heads, scale, _host(q_host), _host(k_host),
                                          _host(v_host), _host(out_host)))
         return out_host
+
+    # ---- 8-bit K/V rows with block scales; per-sequence arguments are lists or uint64 arrays, pointers are device addresses or Buffers ----
+    def kv8_bytes(self, context, kv_heads, dim):
+        """sdx_kv8_bytes: the size of a state of `context` positions."""
+        size = self.lib.sdx_kv8_bytes(context, kv_heads, dim)
+        if not size:
+            _fail(self.lib)
+        return size
+
+    def kv8_write(self, states, contexts, bases, steps, kv_heads, dim, code, keys, values, type, stride=0):
+        """sdx_kv8_write: steps[s] new rows from position bases[s] of every state."""
+        states = _u64(states)
+        n = states.size
+        contexts, bases, steps = _u64(contexts, n), _u64(bases, n), _u64(steps, n)
+        self._c(self.lib.sdx_kv8_write(self.handle, _at(states), _at(contexts), _at(bases), _at(steps), n, kv_heads, dim, code, _pointer(keys),
+                                       _pointer(values), stride, type))
+
+    def kv8_attention(self, states, contexts, lengths, rows, heads, kv_heads, dim, code, scale, q, out, type, cap=0.0, slopes=None, window=0,
+                      prefixes=None, weights=None, q_stride=0, out_stride=0):
+        """sdx_kv8_attention: rows[s] queries of every sequence over its first lengths[s] positions; weights: per sequence the running sums the
+        attention weights are added to, or None."""
+        states = _u64(states)
+        n = states.size
+        contexts, lengths, rows = _u64(contexts, n), _u64(lengths, n), _u64(rows, n)
+        prefixes = None if prefixes is None else _u64(prefixes, n)
+        weights = None if weights is None else _u64(weights, n)
+        self._c(self.lib.sdx_kv8_attention(self.handle, _at(states), _at(contexts), _at(lengths), _at(rows), n, heads, kv_heads, dim, code, scale,
+                                           cap, _pointer(slopes), window, _at(prefixes), _pointer(q), q_stride, _at(weights), _pointer(out),
+                                           out_stride, type))
+
+    def masked_attention(self, q, k, v, out, rows, lengths, heads, kv_heads, dim, type, scale, cap=0.0, slopes=None, window=0, prefixes=None,
+                         q_stride=0, k_stride=0, v_stride=0, out_stride=0):
+        """sdx_masked_attention: packed documents of rows[d] queries and lengths[d] keys over 16-bit keys and values."""
+        rows = _u64(rows)
+        n = rows.size
+        lengths = _u64(lengths, n)
+        prefixes = None if prefixes is None else _u64(prefixes, n)
+        self._c(self.lib.sdx_masked_attention(self.handle, _pointer(q), q_stride, _pointer(k), k_stride, _pointer(v), v_stride, _at(rows),
+                                              _at(lengths), n, heads, kv_heads, dim, type, scale, cap, _pointer(slopes), window, _at(prefixes),
+                                              _pointer(out), out_stride))
+
+    def kv8_evict(self, states, contexts, lengths, weights, keep, sinks, recent, kv_heads, dim, code, targets, target_contexts, target_weights,
+                  kept=None):
+        """sdx_kv8_evict: `keep` rows a K/V head of every longer sequence moved to the target states: the first `sinks`, the last `recent`
+        and those of greatest weight between them; kept: their positions, or None."""
+        states = _u64(states)
+        n = states.size
+        contexts, lengths, weights = _u64(contexts, n), _u64(lengths, n), _u64(weights, n)
+        targets, target_contexts, target_weights = _u64(targets, n), _u64(target_contexts, n), _u64(target_weights, n)
+        self._c(self.lib.sdx_kv8_evict(self.handle, _at(states), _at(contexts), _at(lengths), _at(weights), n, keep, sinks, recent, kv_heads, dim,
+                                       code, _at(targets), _at(target_contexts), _at(target_weights), _pointer(kept)))
 
     # ---- DeepSeek-style latent attention ----
     def attention_turns_reserve(self, rows, rope_dims):

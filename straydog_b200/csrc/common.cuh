@@ -43,6 +43,13 @@ struct Segment {
     uint32_t first_piece, pieces, length;
 };
 
+// A library-owned device buffer that a captured graph may hold: a buffer a capture has used is never freed before the handle is.
+struct Workspace {
+    void* pointer = nullptr;
+    size_t bytes = 0;
+    bool captured = false;
+};
+
 struct Device {
     int ordinal = 0;
     int sms = 0;
@@ -68,6 +75,8 @@ struct Device {
     void* kv_stage = nullptr; uint64_t kv_stage_rows = 0;
     uint32_t* rope_rows = nullptr; size_t rope_first = 0, rope_count = 0;   // a sequence with images: three rotation positions a row (sd_rope_rows)
     uint64_t launches = 0;   // kernels launched through this handle (the benchmark's gpu_launches)
+    Workspace kv8_partial, kv8_scores, kv8_rows, kv8_kept;   // 8-bit rows: split partials, scores behind the weights, unpacked rows, an eviction's positions
+    std::vector<void*> retired;                               // outgrown workspaces that a captured graph may still use (freed with the handle)
     bool adopted = false;    // made by sdx_adopt over another library's stream and allocations: no range checks, nothing owned but workspaces
     explicit Device(int o) : ordinal(o) {}
 };
@@ -79,6 +88,7 @@ void span(Device& d, const void* pointer, size_t bytes, const char* what);
 void span_or_peer(Device& d, const void* pointer, size_t bytes, const char* what);   // also accepts a mapped peer allocation
 size_t allocation_bytes(Device& d, const void* base);   // requested bytes of the allocation that starts at `base`, 0 if none (takes the lock)
 void* ensure(Device& d, void*& slot, size_t& have, size_t bytes, bool pinned_host = false);
+void* workspace(Device& d, Workspace& slot, size_t bytes);   // at least `bytes`; refuses to grow while the handle's stream is being captured
 int* status_word(Device& d);
 // top_k_kernel's other output (csrc/topk.cu): a row's chosen 4-position blocks written into its packed attention row as positions
 struct TopKExpand {

@@ -102,6 +102,27 @@ void* ensure(Device& d, void*& slot, size_t& have, size_t bytes, bool pinned_hos
     return slot;
 }
 
+void* workspace(Device& d, Workspace& slot, size_t bytes) {
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    SDB_CHECK(cudaStreamIsCapturing(d.stream, &capture));
+    if (!slot.pointer || slot.bytes < bytes) {
+        if (capture != cudaStreamCaptureStatusNone)
+            throw std::runtime_error("a Straydog workspace would have to grow inside a stream capture: run one call of this size before the capture");
+        if (slot.pointer && !slot.captured) {
+            SDB_CHECK(cudaStreamSynchronize(d.stream));
+            SDB_CHECK(cudaFree(slot.pointer));
+        } else if (slot.pointer) {
+            d.retired.push_back(slot.pointer);
+        }
+        slot = Workspace{};
+        const size_t grown = bytes + bytes / 4 + 4096;
+        SDB_CHECK(cudaMalloc(&slot.pointer, grown));
+        slot.bytes = grown;
+    }
+    if (capture != cudaStreamCaptureStatusNone) slot.captured = true;
+    return slot.pointer;
+}
+
 cudaStream_t side_stream_begin(Device& d) {
     if (!d.side) {
         SDB_CHECK(cudaStreamCreateWithFlags(&d.side, cudaStreamNonBlocking));
@@ -193,6 +214,8 @@ void sd_destroy(void* handle) {
         }
         if (value->pinned) cudaFreeHost(value->pinned);
         for (void* p : {value->work, value->partial, value->tables, value->unions, static_cast<void*>(value->turns), static_cast<void*>(value->rope_rows)}) if (p) cudaFree(p);
+        for (const Workspace& slot : {value->kv8_partial, value->kv8_scores, value->kv8_rows, value->kv8_kept}) if (slot.pointer) cudaFree(slot.pointer);
+        for (void* p : value->retired) cudaFree(p);
         if (value->side) { cudaStreamDestroy(value->side); cudaEventDestroy(value->side_fork); cudaEventDestroy(value->side_join); }
         if (!value->adopted) cudaStreamDestroy(value->stream);
         cudaGetLastError();

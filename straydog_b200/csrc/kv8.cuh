@@ -1,0 +1,104 @@
+// K/V rows in 8 bits whose scale is shared by a block of 32 positions of one head: layout, codecs and the host checks that the
+// write, the attention and the eviction over such states have in common.
+//
+// A state holds 2 * kv_heads planes (keys of head 0 .., then values of head 0 ..). Plane p is `context` rows (a multiple of 32) of `dim`
+// one-byte codes at state + p * context * dim; behind the planes lie their block scales, F32, context / 32 a plane. A code c stands for
+// c * scale of its block. int8: scale = max |x| / 127, c = x / scale rounded to nearest even; e4m3: scale = max |x| / 448, c = x / scale in
+// E4M3 (nearest even). A zero scale means zero rows. Codes are never NaN: an infinity is held as the block's largest magnitude, a NaN as 0
+// (one such value must not take its 31 neighbours' scale with it).
+#pragma once
+#include "common.cuh"
+
+#include <algorithm>
+#include <cfloat>
+#include <cuda_fp8.h>
+
+namespace sdb {
+namespace kv8 {
+
+constexpr unsigned kBlock = 32;        // positions that share a scale
+constexpr unsigned kSequences = 64;    // sequences a launch: their descriptors travel as kernel parameters (no table to upload, nothing to keep alive)
+constexpr int kInt8 = 0, kE4m3 = 1;
+constexpr int kF32 = 0, kF16 = 1, kBf16 = 30;   // element types by their GGML numbers, as sd_op_index_select_proj takes them
+
+inline size_t state_bytes(uint64_t context, uint64_t kv_heads, uint64_t dim) {
+    const size_t raw = checked_product({2 * kv_heads, context, dim}) + checked_product({2 * kv_heads, context / kBlock, 4});
+    return (raw + 15) / 16 * 16;
+}
+
+inline void check_shape(uint64_t sequences, uint64_t kv_heads, uint64_t dim, int code) {
+    if (!sequences || sequences > 65535 || !kv_heads || kv_heads > 1024 || (dim != 64 && dim != 128 && dim != 256))
+        throw std::runtime_error("invalid Straydog 8-bit K/V dimensions");
+    if (code != kInt8 && code != kE4m3) throw std::runtime_error("an 8-bit K/V code is 0 (int8) or 1 (e4m3)");
+}
+
+inline void check_state(Device& d, const void* state, uint64_t context, uint64_t kv_heads, uint64_t dim) {
+    if (!context || context % kBlock || context > (uint64_t(1) << 24))
+        throw std::runtime_error("an 8-bit K/V state's context is a multiple of 32, at most 2^24");
+    span(d, state, state_bytes(context, kv_heads, dim), "an 8-bit K/V state");
+    if (reinterpret_cast<uintptr_t>(state) % 16) throw std::runtime_error("an 8-bit K/V state must be 16-byte aligned");
+}
+
+// A state listed twice would be written by two blocks of one launch.
+inline void check_distinct(const void* const* states, uint64_t sequences) {
+    std::vector<const void*> sorted(states, states + sequences);
+    std::sort(sorted.begin(), sorted.end());
+    if (std::adjacent_find(sorted.begin(), sorted.end()) != sorted.end())
+        throw std::runtime_error("an 8-bit K/V state is listed twice in one batch: its rows would be written twice");
+}
+
+inline bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return x < y + b_bytes && y < x + a_bytes;
+}
+
+#if defined(__CUDACC__)
+template<int CODE> constexpr float top_code() { return CODE == kInt8 ? 127.0f : 448.0f; }
+
+// x over scale in the block's code. The divide is the IEEE one: the codes are the definition's, bit for bit.
+template<int CODE> __device__ __forceinline__ uint32_t encode(float x, float scale) {
+    if (!(scale > 0.0f) || x != x) return 0;
+    const float y = __fdiv_rn(x, scale);
+    if (CODE == kInt8) {
+        int q = __float2int_rn(y);
+        q = q > 127 ? 127 : q < -127 ? -127 : q;
+        return uint32_t(q) & 0xffu;
+    }
+    return __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
+}
+// Sixteen codes of a row whose block takes a larger scale: their values in the old scale, rounded again in the new one (ratio = old / new
+// <= 1). Code times ratio in F32, then one rounding to the code: what encode(decode(c) * ratio, 1) gives, without the conversion unit where
+// it can be done without (its 16 results a clock an SM would bound an eviction). int8: a byte becomes 2^23 + 128 + c by a byte permute, and a
+// sum with 1.5 * 2^23 rounds to nearest even and leaves the code in the low byte. E4M3: the code's bits placed in an F32 are its value times 2^-120.
+template<int CODE> __device__ __forceinline__ uint4 recode16(uint4 v, float ratio) {
+    if (ratio == 1.0f) return v;
+    uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    #pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (CODE == kInt8) {
+            const uint32_t u = w[i] ^ 0x80808080u;
+            uint32_t q[4];
+            #pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const float c = __fsub_rn(__uint_as_float(prmt(u, 0x4b000000u, 0x7440u | b)), 8388736.0f);
+                q[b] = __float_as_uint(__fadd_rn(__fmul_rn(c, ratio), 12582912.0f));
+            }
+            w[i] = prmt(prmt(q[0], q[1], 0x0040u), prmt(q[2], q[3], 0x0040u), 0x5410u);
+        } else {
+            const float up = ratio * 1.329227995784916e36f;   // 2^120
+            float f[4];
+            #pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const uint32_t byte = w[i] >> (8 * b);
+                f[b] = __fmul_rn(__uint_as_float((byte & 0x80u) << 24 | (byte & 0x7fu) << 20), up);
+            }
+            w[i] = uint32_t(__nv_cvt_float2_to_fp8x2(make_float2(f[0], f[1]), __NV_SATFINITE, __NV_E4M3)) |
+                   uint32_t(__nv_cvt_float2_to_fp8x2(make_float2(f[2], f[3]), __NV_SATFINITE, __NV_E4M3)) << 16;
+        }
+    }
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+#endif
+
+}  // namespace kv8
+}  // namespace sdb

@@ -1,0 +1,675 @@
+// Attention of a few query rows a sequence (decode, verification) over states of 8-bit rows with block scales, and the entry that sends
+// longer chunks to the prompt kernel (csrc/masked_attention.cu). csrc/kv8.cuh has the layout.
+//
+//   s(r, j) = scale * q_r . (code_j * key scale of j's block), capped, biased by distance, masked;   out_r = sum_j softmax(s)_j * v_j
+//
+// The query rows of one K/V head (rows x heads a K/V head: up to 16 at a time, 8 of 256 columns) read its K and V once: 2 * dim bytes a position, 8 to 32 flops a byte,
+// so memory binds this. The work of a batch is every sequence's (K/V head, tile of keys) laid end to end and cut into equal runs, one a block
+// (one block of eight warps an SM): ragged lengths balance to within a tile. A block's run is one piece a (sequence, K/V head) it crosses.
+// The warps take a piece's tiles in turn; each has a ring of tiles in shared memory filled by 16-byte asynchronous copies, two or more
+// tiles ahead, pieces' borders not minded. The arithmetic is on mma.sync (16 keys x 8 queries x 16 columns): int8 and E4M3 codes become FP16
+// exactly by byte permutes; the blocks' scales multiply scores and weighted sums in FP32. Softmax is online, in the exp2 domain. Queries
+// enter as FP16: BF16 rows are multiplied by a power of two that brings their largest value to 2^14 (exact), undone on the scores.
+// Weights enter the value product as FP16 at 2^10 times their size (the running maximum has 2^10): 11 bits down to 2^-24 of the largest.
+// A piece's eight partial results meet in shared memory; a piece that is all of its (sequence, K/V head) writes the output, the others
+// leave FP32 partials that a second kernel joins. Where a piece is cut depends on the batch, the order of the sums inside it does not.
+#include "kv8.cuh"
+#include "masked_attention.cuh"
+#include "../../include/straydog_gpu_b200.h"
+
+namespace sdb {
+namespace kv8 {
+
+constexpr int kWarps = 8, kThreads = 32 * kWarps;
+constexpr float kLift = 10.0f;   // log2 of what weights are multiplied by on their way to FP16
+
+struct AttentionSequence {
+    const uint8_t* state;
+    float* weights;          // [kv_heads][context] or null
+    uint32_t context, length, rows, first_row, prefix;
+    uint32_t tiles;          // tiles a (K/V head, part)
+    uint32_t head_tiles, jump;   // tiles below head_tiles are at their place, the others `jump` tiles further on (keys no row sees are passed over)
+    uint32_t first_unit;
+    uint32_t parts;          // how often a K/V head's rows are read: query rows over queries a unit
+    uint64_t first_tile;     // of all sequences' tiles
+};
+struct AttentionArgs {
+    AttentionSequence sequence[kSequences];
+    uint32_t sequences, heads, kv_heads, group, units;
+    uint64_t tiles, tiles_a_block;
+    const void* q;
+    void* out;
+    const float* slopes;
+    size_t q_stride, out_stride;
+    float scale_log2, cap, scale_over_cap;
+    uint32_t window;
+    int bf16;
+    float* partial;          // [block + unit][queries][D], then [block + unit][queries][2]
+    float* sums;             // [block + unit][queries][2]: maximum (exp2 domain, lifted), denominator
+    float* scores;           // [tile][keys][queries] or null
+    float* stats;            // [unit][queries][2]: final maximum and denominator, for the weights
+};
+
+__device__ __forceinline__ void copy16(uint32_t to, const void* from) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t to, const void* from) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
+}
+
+// Two codes of a word as an FP16 pair: low bytes 0 and 1 or 2 and 3 (keys: neighbouring columns), bytes 0 and 2 or 1 and 3 (values:
+// one column of two keys). int8 exactly (x is the word xor 0x80808080: 1024 + 128 + c, less 1152); E4M3 at 2^-8 of its value, exactly
+// (its exponent and mantissa bits moved to FP16's places), which the caller's scale makes good.
+template<int CODE> __device__ __forceinline__ uint32_t pair_of(uint32_t x, uint32_t int8_selector, uint32_t e4m3_selector) {
+    if (CODE == kInt8) {
+        const uint32_t h = prmt(x, 0x64646464u, int8_selector);
+        const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&h), __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
+        return *reinterpret_cast<const uint32_t*>(&r);
+    }
+    const uint32_t y = prmt(x, 0u, e4m3_selector);   // each code in the high byte of its half
+    return (y & 0x80008000u) | ((y >> 1) & 0x3f803f80u);
+}
+template<int CODE> __device__ __forceinline__ uint32_t pair01(uint32_t x) { return pair_of<CODE>(x, 0x4140u, 0x1404u); }
+template<int CODE> __device__ __forceinline__ uint32_t pair23(uint32_t x) { return pair_of<CODE>(x, 0x4342u, 0x3424u); }
+template<int CODE> __device__ __forceinline__ uint32_t pair02(uint32_t x) { return pair_of<CODE>(x, 0x4240u, 0x2404u); }
+template<int CODE> __device__ __forceinline__ uint32_t pair13(uint32_t x) { return pair_of<CODE>(x, 0x4341u, 0x3414u); }
+template<int CODE> __device__ __forceinline__ uint32_t flipped(uint32_t x) { return CODE == kInt8 ? x ^ 0x80808080u : x; }
+
+template<int D, int NT> struct Shape {
+    static constexpr int kTile = D == 256 ? 16 : 32;                  // keys a tile: 8 KB of keys and values for D 128 and 256, 4 KB for 64
+    static constexpr int kQueries = 8 * NT;
+    static constexpr int kPlane = kTile * D, kSlot = 2 * kPlane;      // bytes
+    static constexpr int kStages = D == 64 ? 6 : 3;
+    static constexpr int kChunk = 16384 / (kWarps * kQueries * 4) < D ? 16384 / (kWarps * kQueries * 4) : D;   // columns that meet at a time
+    static constexpr int kRing = kWarps * kStages * kSlot, kScales = kWarps * kStages * 8;
+    static constexpr int kJoin = kWarps * kQueries * (kChunk + 4) * 4;
+    static constexpr int kStats = kWarps * kQueries * 8;
+    static constexpr int kSmem = kRing + kScales + kJoin + kStats;
+};
+
+// A walk over the tiles of a block's run: the (sequence, unit) a tile belongs to, without divisions after the first.
+struct Place {
+    uint32_t s, unit;        // unit: counted over all sequences
+    uint64_t begin, end;     // tiles of the unit
+    __device__ __forceinline__ void find(const AttentionArgs& a, uint64_t tile) {
+        s = 0;
+        uint32_t high = a.sequences;
+        while (high - s > 1) { const uint32_t mid = (s + high) / 2; if (a.sequence[mid].first_tile <= tile) s = mid; else high = mid; }
+        const AttentionSequence& q = a.sequence[s];
+        const uint32_t inside = uint32_t((tile - q.first_tile) / q.tiles);
+        unit = q.first_unit + inside;
+        begin = q.first_tile + uint64_t(inside) * q.tiles;
+        end = begin + q.tiles;
+    }
+    __device__ __forceinline__ void next(const AttentionArgs& a) {
+        ++unit;
+        while (s + 1 < a.sequences && a.sequence[s + 1].first_tile <= end) unit = a.sequence[++s].first_unit;   // (one without tiles shares the next one's first tile)
+        begin = end;
+        end = begin + a.sequence[s].tiles;
+    }
+};
+
+template<int D, int NT, int CODE>
+__global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_constant__ AttentionArgs a) {
+    using S = Shape<D, NT>;
+    extern __shared__ __align__(128) uint8_t smem[];
+    const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
+    uint8_t* ring = smem + warp * (S::kStages * S::kSlot);
+    float* ring_scales = reinterpret_cast<float*>(smem + S::kRing) + warp * (S::kStages * 2);
+    float* join = reinterpret_cast<float*>(smem + S::kRing + S::kScales);
+    float* stat = reinterpret_cast<float*>(smem + S::kRing + S::kScales + S::kJoin);   // [warp][query][maximum, denominator]
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+
+    const uint64_t run_begin = blockIdx.x * a.tiles_a_block, run_end = min(run_begin + a.tiles_a_block, a.tiles);
+    if (run_begin >= run_end) return;
+
+    // ---- the copies: this warp's tiles run_begin + warp, + 8, ... ----
+    Place at;
+    at.find(a, run_begin);
+    Place ahead = at;
+    uint64_t ahead_tile = run_begin + warp;
+    // Rows are laid in a slot as they lie in memory, their 16-byte pieces exchanged so that the reads below meet in no bank: keys by the
+    // row's parity (a read takes 64 bytes of each of two neighbouring rows), values by the row's low bits (a transposing read takes one
+    // piece of each of eight rows).
+    constexpr int kPieces = D / 16, kStepRows = 32 / kPieces;   // pieces a row, rows a copy instruction of the warp
+    const int row0 = lane / kPieces, piece0 = lane % kPieces;
+    const uint32_t ring_address = smem_u32(ring), scales_address = smem_u32(ring_scales);
+    auto fetch = [&](int slot) {
+        if (ahead_tile < run_end) {
+            while (ahead_tile >= ahead.end) ahead.next(a);
+            const AttentionSequence& q = a.sequence[ahead.s];
+            uint32_t tile = uint32_t(ahead_tile - ahead.begin);
+            if (tile >= q.head_tiles) tile += q.jump;
+            const uint32_t kv = (ahead.unit - q.first_unit) / q.parts, key = tile * S::kTile;
+            const size_t k_row = size_t(kv) * q.context + key, v_row = size_t(a.kv_heads + kv) * q.context + key;
+            const uint8_t* k_from = q.state + k_row * D + lane * 16;
+            const uint8_t* v_from = q.state + v_row * D + lane * 16;
+            const uint32_t k_to = ring_address + slot * S::kSlot, v_to = k_to + S::kPlane;
+            #pragma unroll
+            for (int i = 0; i < S::kTile / kStepRows; ++i) {
+                const int row = row0 + i * kStepRows;
+                const int k_piece = D == 64 ? piece0 : piece0 ^ (4 * (row & 1));
+                copy16(k_to + row * D + k_piece * 16, k_from + i * 512);
+            }
+            #pragma unroll
+            for (int i = 0; i < S::kTile / kStepRows; ++i) {
+                const int row = row0 + i * kStepRows;
+                const int v_piece = D == 64 ? piece0 ^ ((row >> 1) & 3) : piece0 ^ (row & 7);
+                copy16(v_to + row * D + v_piece * 16, v_from + i * 512);
+            }
+            if (lane < 2) {
+                const float* scales = reinterpret_cast<const float*>(q.state + size_t(2 * a.kv_heads) * q.context * D);
+                copy4(scales_address + slot * 8 + lane * 4, scales + (lane ? v_row : k_row) / kBlock);
+            }
+            ahead_tile += kWarps;
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    #pragma unroll
+    for (int i = 0; i < S::kStages - 1; ++i) fetch(i);
+
+    const uint32_t v_lane = uint32_t(lane % 8 + 8 * ((lane / 8) & 1));   // the key row this lane's address names in a transposing read
+    int slot = 0, fill = S::kStages - 1;
+    uint64_t tile_id = run_begin + warp;
+
+    for (;;) {
+        // ---- a piece: the part of the run that lies in one (sequence, K/V head, part) ----
+        const AttentionSequence& sequence = a.sequence[at.s];
+        const uint64_t piece_end = min(at.end, run_end);
+        const uint32_t inside = at.unit - sequence.first_unit, kv = inside / sequence.parts, part = inside % sequence.parts;
+        const uint32_t first_query = part * S::kQueries, queries = sequence.rows * a.group;
+
+        // the queries as B fragments: lane (g, t) holds query 8n + g, of each 64 columns the sixteen from 16 t
+        uint32_t qf[NT][D / 8];
+        float unscale[NT][2], slope[NT][2];
+        int position[NT][2], low[NT][2];
+        uint32_t prefix[NT][2];
+        #pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            const uint32_t query = first_query + 8 * n + g, row = query / a.group, head = kv * a.group + query % a.group;
+            const bool real = query < queries;
+            const uint8_t* from = static_cast<const uint8_t*>(a.q) +
+                                  (real ? (size_t(sequence.first_row + row) * a.q_stride + size_t(head) * D + 16 * t) * 2 : 0);
+            #pragma unroll
+            for (int c = 0; c < D / 64; ++c)
+                #pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint4 v = real ? *reinterpret_cast<const uint4*>(from + c * 128 + i * 16) : make_uint4(0, 0, 0, 0);
+                    qf[n][c * 8 + i * 4] = v.x; qf[n][c * 8 + i * 4 + 1] = v.y; qf[n][c * 8 + i * 4 + 2] = v.z; qf[n][c * 8 + i * 4 + 3] = v.w;
+                }
+            float down = CODE == kE4m3 ? 256.0f : 1.0f;
+            if (a.bf16) {
+                uint32_t top = 0;   // magnitudes of BF16 values compare as their bits do
+                #pragma unroll
+                for (int i = 0; i < D / 8; ++i) { top = max(top, qf[n][i] & 0x7fffu); top = max(top, (qf[n][i] >> 16) & 0x7fffu); }
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+                top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+                const int exponent = int(top >> 7);   // biased; 255: an infinity or a NaN among them, left as they are
+                const int lift = exponent == 255 || exponent == 0 ? 0 : max(-100, min(100, 127 + 14 - exponent));
+                const float up = __uint_as_float(uint32_t(127 + lift) << 23);
+                down *= __uint_as_float(uint32_t(127 - lift) << 23);
+                #pragma unroll
+                for (int i = 0; i < D / 8; ++i)
+                    qf[n][i] = pack_half2(__uint_as_float(qf[n][i] << 16) * up, __uint_as_float(qf[n][i] & 0xffff0000u) * up);
+            }
+            #pragma unroll
+            for (int i = 0; i < 2; ++i) {   // the queries whose scores this lane will hold
+                const uint32_t other = first_query + 8 * n + 2 * t + i, other_row = other / a.group;
+                const bool there = other < queries;
+                unscale[n][i] = __shfl_sync(0xffffffffu, down, (2 * t + i) * 4);
+                position[n][i] = there ? int(sequence.length) - int(sequence.rows) + int(other_row) : -1;
+                low[n][i] = a.window ? position[n][i] - int(a.window) : -1;   // keys above this one
+                prefix[n][i] = there ? sequence.prefix : 0;
+                slope[n][i] = there && a.slopes ? a.slopes[kv * a.group + other % a.group] * 1.4426950408889634f : 0.0f;
+            }
+        }
+        float o[D / 16][NT][4], m[NT][2], l[NT][2];
+        #pragma unroll
+        for (int n = 0; n < NT; ++n) {
+            m[n][0] = m[n][1] = -INFINITY; l[n][0] = l[n][1] = 0.0f;
+            #pragma unroll
+            for (int i = 0; i < D / 16; ++i)
+                #pragma unroll
+                for (int c = 0; c < 4; ++c) o[i][n][c] = 0.0f;
+        }
+
+        for (; tile_id < piece_end; tile_id += kWarps) {
+            __syncwarp();   // (all lanes are past their reads of the slot to fill)
+            fetch(fill);
+            fill = fill + 1 == S::kStages ? 0 : fill + 1;
+            asm volatile("cp.async.wait_group %0;" ::"n"(S::kStages - 1) : "memory");
+            __syncwarp();
+            uint32_t tile = uint32_t(tile_id - at.begin);
+            if (tile >= sequence.head_tiles) tile += sequence.jump;
+            const int key0 = int(tile * S::kTile);
+            const uint8_t* kt = ring + slot * S::kSlot;
+            const uint32_t vt = ring_address + slot * S::kSlot + S::kPlane;
+            const float k_scale = ring_scales[slot * 2], v_scale = ring_scales[slot * 2 + 1] * (CODE == kE4m3 ? 256.0f : 1.0f);
+
+            // ---- scores ----
+            float x[S::kTile / 16][NT][4];
+            #pragma unroll
+            for (int h = 0; h < S::kTile / 16; ++h) {
+                float acc[NT][4];
+                #pragma unroll
+                for (int n = 0; n < NT; ++n) acc[n][0] = acc[n][1] = acc[n][2] = acc[n][3] = 0.0f;
+                #pragma unroll
+                for (int c = 0; c < D / 64; ++c) {
+                    const int piece = D == 64 ? t : (4 * c + t) ^ (4 * (g & 1));
+                    const uint4 r0 = *reinterpret_cast<const uint4*>(kt + (16 * h + g) * D + piece * 16);
+                    const uint4 r1 = *reinterpret_cast<const uint4*>(kt + (16 * h + g + 8) * D + piece * 16);
+                    const uint32_t w0[4] = {flipped<CODE>(r0.x), flipped<CODE>(r0.y), flipped<CODE>(r0.z), flipped<CODE>(r0.w)};
+                    const uint32_t w1[4] = {flipped<CODE>(r1.x), flipped<CODE>(r1.y), flipped<CODE>(r1.z), flipped<CODE>(r1.w)};
+                    #pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const uint32_t af[4] = {pair01<CODE>(w0[i]), pair01<CODE>(w1[i]), pair23<CODE>(w0[i]), pair23<CODE>(w1[i])};
+                        #pragma unroll
+                        for (int n = 0; n < NT; ++n) mma_f16(acc[n], af, qf[n][c * 8 + 2 * i], qf[n][c * 8 + 2 * i + 1]);
+                    }
+                }
+                #pragma unroll
+                for (int n = 0; n < NT; ++n)
+                    #pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        const int i = c & 1, key = key0 + 16 * h + g + 8 * (c >> 1);
+                        float s = acc[n][c] * (k_scale * unscale[n][i]);
+                        s = a.cap > 0.0f ? a.cap * tanhf(s * a.scale_over_cap) : s * a.scale_log2;   // (the cap is in the exp2 domain too)
+                        s = fmaf(-slope[n][i], fabsf(float(position[n][i] - key)), s);
+                        const bool seen = ((key <= position[n][i] && key > low[n][i]) || uint32_t(key) < prefix[n][i]) && key < int(sequence.length);
+                        x[h][n][c] = seen ? s : -INFINITY;
+                    }
+            }
+            if (a.scores) {
+                float* to = a.scores + size_t(tile_id) * (S::kTile * S::kQueries);
+                #pragma unroll
+                for (int h = 0; h < S::kTile / 16; ++h)
+                    #pragma unroll
+                    for (int n = 0; n < NT; ++n)
+                        #pragma unroll
+                        for (int i = 0; i < 2; ++i)
+                            *reinterpret_cast<float2*>(to + (16 * h + g + 8 * i) * S::kQueries + 8 * n + 2 * t) = make_float2(x[h][n][2 * i], x[h][n][2 * i + 1]);
+            }
+            // ---- the running maximum (lifted) and the weights ----
+            bool grew = false;
+            float now[NT][2];
+            #pragma unroll
+            for (int n = 0; n < NT; ++n)
+                #pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    float top = fmaxf(x[0][n][i], x[0][n][i + 2]);
+                    #pragma unroll
+                    for (int h = 1; h < S::kTile / 16; ++h) top = fmaxf(top, fmaxf(x[h][n][i], x[h][n][i + 2]));
+                    #pragma unroll
+                    for (int offset = 4; offset < 32; offset *= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, offset));
+                    now[n][i] = fmaxf(m[n][i], top - kLift);
+                    grew |= now[n][i] > m[n][i];
+                }
+            if (__any_sync(0xffffffffu, grew)) {
+                #pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const float f0 = m[n][0] == -INFINITY ? 0.0f : fast_exp2(m[n][0] - now[n][0]), f1 = m[n][1] == -INFINITY ? 0.0f : fast_exp2(m[n][1] - now[n][1]);
+                    l[n][0] *= f0; l[n][1] *= f1; m[n][0] = now[n][0]; m[n][1] = now[n][1];
+                    #pragma unroll
+                    for (int i = 0; i < D / 16; ++i) { o[i][n][0] *= f0; o[i][n][1] *= f1; o[i][n][2] *= f0; o[i][n][3] *= f1; }
+                }
+            }
+            uint32_t pf[S::kTile / 16][NT][2];
+            #pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const float u0 = m[n][0] == -INFINITY ? 0.0f : m[n][0], u1 = m[n][1] == -INFINITY ? 0.0f : m[n][1];   // (nothing seen so far: every weight 0)
+                #pragma unroll
+                for (int h = 0; h < S::kTile / 16; ++h) {
+                    const float p0 = fast_exp2(x[h][n][0] - u0), p1 = fast_exp2(x[h][n][1] - u1), p2 = fast_exp2(x[h][n][2] - u0), p3 = fast_exp2(x[h][n][3] - u1);
+                    l[n][0] += p0 + p2; l[n][1] += p1 + p3;
+                    pf[h][n][0] = movmatrix_trans(pack_half2(p0, p1));
+                    pf[h][n][1] = movmatrix_trans(pack_half2(p2, p3));
+                }
+            }
+            // ---- O^T += value scale * V^T P^T: per 32 columns the tile's keys into fresh accumulators, then the scale in FP32 ----
+            #pragma unroll
+            for (int b = 0; b < D / 32; ++b) {
+                float acc[2][NT][4];
+                #pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    #pragma unroll
+                    for (int n = 0; n < NT; ++n) acc[i][n][0] = acc[i][n][1] = acc[i][n][2] = acc[i][n][3] = 0.0f;
+                #pragma unroll
+                for (int h = 0; h < S::kTile / 16; ++h) {
+                    const uint32_t row = v_lane + 16 * h, piece = (2 * b + lane / 16) ^ (D == 64 ? (row >> 1) & 3 : row & 7);
+                    uint32_t w[4];   // w[0], w[1]: columns 32b + 2g, + 1 of keys (2t, 2t + 1) and (2t + 8, 2t + 9); w[2], w[3]: columns 32b + 16 + 2g, + 1
+                    ldmatrix_x4_trans(w, vt + row * D + piece * 16);
+                    #pragma unroll
+                    for (int i = 0; i < 4; ++i) w[i] = flipped<CODE>(w[i]);
+                    const uint32_t af[4] = {pair02<CODE>(w[0]), pair13<CODE>(w[0]), pair02<CODE>(w[1]), pair13<CODE>(w[1])};
+                    const uint32_t ag[4] = {pair02<CODE>(w[2]), pair13<CODE>(w[2]), pair02<CODE>(w[3]), pair13<CODE>(w[3])};
+                    #pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        mma_f16(acc[0][n], af, pf[h][n][0], pf[h][n][1]);
+                        mma_f16(acc[1][n], ag, pf[h][n][0], pf[h][n][1]);
+                    }
+                }
+                #pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    #pragma unroll
+                    for (int n = 0; n < NT; ++n)
+                        #pragma unroll
+                        for (int c = 0; c < 4; ++c) o[2 * b + i][n][c] = fmaf(v_scale, acc[i][n][c], o[2 * b + i][n][c]);
+            }
+            if (++slot == S::kStages) slot = 0;
+        }
+
+        // ---- the warps' partial results of the piece meet ----
+        #pragma unroll
+        for (int n = 0; n < NT; ++n)
+            #pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                #pragma unroll
+                for (int offset = 4; offset < 32; offset *= 2) l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], offset);
+                if (g == 0) *reinterpret_cast<float2*>(stat + (warp * S::kQueries + 8 * n + 2 * t + i) * 2) = make_float2(m[n][i], l[n][i]);
+            }
+        __syncthreads();
+        float factor[NT][2];
+        #pragma unroll
+        for (int n = 0; n < NT; ++n)
+            #pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                float top = -INFINITY;
+                #pragma unroll
+                for (int w = 0; w < kWarps; ++w) top = fmaxf(top, stat[(w * S::kQueries + 8 * n + 2 * t + i) * 2]);
+                factor[n][i] = m[n][i] == -INFINITY ? 0.0f : fast_exp2(m[n][i] - top);   // (sums without a maximum are 0, or NaN: either stays)
+            }
+        const bool whole = piece_end - max(at.begin, run_begin) == sequence.tiles;   // the piece is all of its unit
+        const size_t mine = size_t(blockIdx.x) + at.unit;
+        constexpr int kPitch = S::kChunk + 4;
+        #pragma unroll
+        for (int chunk = 0; chunk < D / S::kChunk; ++chunk) {
+            #pragma unroll
+            for (int i = 0; i < S::kChunk / 16; ++i)
+                #pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const float (&v)[4] = o[chunk * (S::kChunk / 16) + i][n];
+                    float* to = join + (warp * S::kQueries + 8 * n + 2 * t) * kPitch + 16 * i + 2 * g;
+                    *reinterpret_cast<float2*>(to) = make_float2(v[0] * factor[n][0], v[2] * factor[n][0]);
+                    *reinterpret_cast<float2*>(to + kPitch) = make_float2(v[1] * factor[n][1], v[3] * factor[n][1]);
+                }
+            __syncthreads();
+            for (int e = threadIdx.x; e < S::kQueries * S::kChunk / 2; e += kThreads) {
+                const int query = e / (S::kChunk / 2), column = e % (S::kChunk / 2) * 2;
+                float2 total = make_float2(0.0f, 0.0f);
+                float top = -INFINITY, weight = 0.0f;
+                #pragma unroll
+                for (int w = 0; w < kWarps; ++w) {
+                    const float2 v = *reinterpret_cast<const float2*>(join + (w * S::kQueries + query) * kPitch + column);
+                    total.x += v.x; total.y += v.y;
+                    top = fmaxf(top, stat[(w * S::kQueries + query) * 2]);
+                }
+                #pragma unroll
+                for (int w = 0; w < kWarps; ++w) {
+                    const float2 v = *reinterpret_cast<const float2*>(stat + (w * S::kQueries + query) * 2);
+                    weight += v.y == 0.0f ? 0.0f : (v.x == -INFINITY ? 1.0f : fast_exp2(v.x - top)) * v.y;   // (scores that are all NaN leave a NaN sum)
+                }
+                const uint32_t global = first_query + query, all = chunk * S::kChunk + column;
+                if (!whole) {
+                    *reinterpret_cast<float2*>(a.partial + (mine * S::kQueries + query) * D + all) = total;
+                    if (all == 0) *reinterpret_cast<float2*>(a.sums + (mine * S::kQueries + query) * 2) = make_float2(top, weight);
+                } else if (global < queries) {
+                    const float inverse = weight > 0.0f ? 1.0f / weight : weight == 0.0f ? 0.0f : weight;
+                    const size_t to = size_t(sequence.first_row + global / a.group) * a.out_stride + size_t(kv * a.group + global % a.group) * D + all;
+                    const uint32_t packed = a.bf16 ? pack_bf16x2(total.x * inverse, total.y * inverse) : pack_half2(total.x * inverse, total.y * inverse);
+                    *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + to) = packed;
+                }
+                if (whole && a.scores && all == 0) *reinterpret_cast<float2*>(a.stats + (size_t(at.unit) * S::kQueries + query) * 2) = make_float2(top, weight);
+            }
+            __syncthreads();
+        }
+        if (piece_end == run_end) break;
+        at.next(a);
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+// Block = (unit, query): joins the partials of a unit that several blocks worked on, and zeroes the rows of a sequence without keys.
+template<int D>
+__global__ void __launch_bounds__(D) kv8_decode_join_kernel(const __grid_constant__ AttentionArgs a, uint32_t queries_a_unit) {
+    const uint32_t unit = blockIdx.x, query = blockIdx.y;
+    uint32_t s = 0;
+    {
+        uint32_t high = a.sequences;
+        while (high - s > 1) { const uint32_t mid = (s + high) / 2; if (a.sequence[mid].first_unit <= unit) s = mid; else high = mid; }
+    }
+    const AttentionSequence& sequence = a.sequence[s];
+    const uint32_t inside = unit - sequence.first_unit, kv = inside / sequence.parts, global = inside % sequence.parts * queries_a_unit + query;
+    const bool real = global < sequence.rows * a.group;
+    uint16_t* out = static_cast<uint16_t*>(a.out) + (real ? size_t(sequence.first_row + global / a.group) * a.out_stride + size_t(kv * a.group + global % a.group) * D : 0) + threadIdx.x;
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // (in every block: what is launched behind this one counts on the decode's end too)
+    if (!sequence.tiles) {
+        if (real) *out = 0;
+        return;
+    }
+    const uint64_t begin = sequence.first_tile + uint64_t(inside) * sequence.tiles, end = begin + sequence.tiles;
+    const uint32_t first = uint32_t(begin / a.tiles_a_block), last = uint32_t((end - 1) / a.tiles_a_block);
+    if (first == last) return;
+    const float2* sums = reinterpret_cast<const float2*>(a.sums) + (size_t(first) + unit) * queries_a_unit + query;
+    const float* partial = a.partial + ((size_t(first) + unit) * queries_a_unit + query) * D + threadIdx.x;
+    const uint32_t pieces = last - first + 1;
+    float top = -INFINITY;
+    for (uint32_t p = 0; p < pieces; ++p) top = fmaxf(top, sums[size_t(p) * queries_a_unit].x);
+    float total = 0.0f, weight = 0.0f;
+    #pragma unroll 4
+    for (uint32_t p = 0; p < pieces; ++p) {
+        const float2 v = sums[size_t(p) * queries_a_unit];
+        const float factor = v.x == -INFINITY ? 0.0f : fast_exp2(v.x - top);
+        weight += v.y == 0.0f ? 0.0f : (v.x == -INFINITY ? 1.0f : factor) * v.y;
+        total = fmaf(factor, partial[size_t(p) * queries_a_unit * D], total);
+    }
+    if (a.scores && threadIdx.x == 0) *reinterpret_cast<float2*>(a.stats + (size_t(unit) * queries_a_unit + query) * 2) = make_float2(top, weight);
+    if (!real) return;
+    const float result = weight > 0.0f ? total / weight : weight == 0.0f ? 0.0f : weight;
+    if (a.bf16) *reinterpret_cast<__nv_bfloat16*>(out) = __float2bfloat16_rn(result);
+    else *reinterpret_cast<__half*>(out) = __float2half_rn(result);
+}
+
+// Thread = (K/V head, seen key): the key's weights over a K/V head's query rows, from the scores the attention left, added to the running sums.
+template<int TILE, int QUERIES>
+__global__ void __launch_bounds__(256) kv8_weights_kernel(const __grid_constant__ AttentionArgs a) {
+    const uint32_t s = blockIdx.y;
+    const AttentionSequence& sequence = a.sequence[s];
+    const uint32_t keys = sequence.tiles * TILE;
+    const uint64_t index = uint64_t(blockIdx.x) * 256 + threadIdx.x;
+    if (index >= uint64_t(keys) * a.kv_heads) return;
+    const uint32_t kv = uint32_t(index / keys), at = uint32_t(index % keys);
+    uint32_t tile = at / TILE;
+    if (tile >= sequence.head_tiles) tile += sequence.jump;
+    const uint32_t key = tile * TILE + at % TILE;
+    if (key >= sequence.length) return;
+    float total = 0.0f;
+    for (uint32_t part = 0; part < sequence.parts; ++part) {
+        const uint32_t inside = kv * sequence.parts + part;
+        const uint32_t queries = min(uint32_t(QUERIES), sequence.rows * a.group - part * QUERIES);
+        const float4* scores = reinterpret_cast<const float4*>(a.scores + (sequence.first_tile + uint64_t(inside) * sequence.tiles) * (TILE * QUERIES) + size_t(at) * QUERIES);
+        const float2* stats = reinterpret_cast<const float2*>(a.stats) + size_t(sequence.first_unit + inside) * QUERIES;
+        #pragma unroll
+        for (int i = 0; i < QUERIES / 4; ++i) {
+            const float4 v = scores[i];
+            const float x[4] = {v.x, v.y, v.z, v.w};
+            #pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                if (uint32_t(4 * i + c) >= queries) continue;
+                const float2 stat = stats[4 * i + c];
+                if (x[c] != -INFINITY) total += fast_exp2(x[c] - stat.x) / stat.y;
+            }
+        }
+    }
+    float* to = sequence.weights + size_t(kv) * sequence.context + key;
+    *to += total;
+}
+
+template<int D, int NT, int CODE> static void launch_decode(Device& d, AttentionArgs& args, bool weights) {
+    using S = Shape<D, NT>;
+    args.units = 0; args.tiles = 0;
+    uint64_t most_keys = 0;
+    bool empty = false;
+    for (uint32_t s = 0; s < args.sequences; ++s) {
+        AttentionSequence& q = args.sequence[s];
+        const uint64_t low = args.window && q.length + 1 > uint64_t(q.rows) + args.window ? q.length + 1 - q.rows - args.window : 0;   // the first row's first key
+        const uint32_t all = uint32_t((q.length + S::kTile - 1) / S::kTile);
+        q.head_tiles = uint32_t((q.prefix + S::kTile - 1) / S::kTile);
+        const uint32_t body = std::min(all, std::max(q.head_tiles, uint32_t(low / S::kTile)));
+        q.jump = body - std::min(body, q.head_tiles);
+        q.tiles = all - q.jump;
+        q.parts = (q.rows * args.group + S::kQueries - 1) / S::kQueries;
+        q.first_unit = args.units;
+        q.first_tile = args.tiles;
+        args.units += args.kv_heads * q.parts;
+        args.tiles += uint64_t(args.kv_heads) * q.parts * q.tiles;
+        most_keys = std::max(most_keys, uint64_t(q.tiles) * S::kTile * args.kv_heads);
+        empty |= !q.tiles;
+    }
+    // One block an SM; a warp takes a tile at least
+    const uint64_t blocks = std::max<uint64_t>(1, std::min<uint64_t>(d.sms, (args.tiles + kWarps - 1) / kWarps));
+    args.tiles_a_block = std::max<uint64_t>(1, (args.tiles + blocks - 1) / blocks);
+    const size_t slots = blocks + args.units;
+    bool cut = false;   // a unit that several blocks work on
+    for (uint32_t s = 0; s < args.sequences && !cut; ++s) {
+        const AttentionSequence& q = args.sequence[s];
+        for (uint32_t u = 0; u < args.kv_heads * q.parts && q.tiles && !cut; ++u) {
+            const uint64_t begin = q.first_tile + uint64_t(u) * q.tiles;
+            cut = begin / args.tiles_a_block != (begin + q.tiles - 1) / args.tiles_a_block;
+        }
+    }
+    const size_t partial_floats = cut ? slots * S::kQueries * D : 0, sums_floats = cut ? slots * S::kQueries * 2 : 0;
+    float* partial = cut ? static_cast<float*>(workspace(d, d.kv8_partial, (partial_floats + sums_floats) * 4)) : nullptr;
+    args.partial = partial;
+    args.sums = partial + partial_floats;
+    args.scores = args.stats = nullptr;
+    if (weights && args.tiles) {
+        const size_t score_floats = checked_product({args.tiles, uint64_t(S::kTile), uint64_t(S::kQueries)});
+        args.scores = static_cast<float*>(workspace(d, d.kv8_scores, (score_floats + size_t(args.units) * S::kQueries * 2) * 4));
+        args.stats = args.scores + score_floats;
+    }
+    static bool configured[64] = {};
+    if (!configured[d.ordinal & 63]) {
+        SDB_CHECK(cudaFuncSetAttribute(kv8_decode_kernel<D, NT, CODE>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::kSmem));
+        configured[d.ordinal & 63] = true;
+    }
+    cudaLaunchAttribute attribute{};
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute.val.programmaticStreamSerializationAllowed = 1;
+    bool behind = false;   // a kernel of this call is ahead in the stream: the next is its programmatic dependent
+    if (args.tiles) {
+        kv8_decode_kernel<D, NT, CODE><<<unsigned(blocks), kThreads, S::kSmem, d.stream>>>(args);
+        ++d.launches;
+        behind = true;
+    }
+    if (cut || empty) {
+        cudaLaunchConfig_t config{};
+        config.gridDim = dim3(args.units, S::kQueries);
+        config.blockDim = dim3(D);
+        config.stream = d.stream;
+        config.attrs = &attribute;
+        config.numAttrs = behind ? 1 : 0;
+        SDB_CHECK(cudaLaunchKernelEx(&config, kv8_decode_join_kernel<D>, args, uint32_t(S::kQueries)));
+        ++d.launches;
+    }
+    if (args.scores) {
+        kv8_weights_kernel<S::kTile, S::kQueries><<<dim3(unsigned((most_keys + 255) / 256), args.sequences), 256, 0, d.stream>>>(args);
+        ++d.launches;
+    }
+}
+
+template<int D> static void launch_queries(Device& d, AttentionArgs& args, int code, bool weights, bool two) {
+    constexpr int kTwo = D == 256 ? 1 : 2;   // (256 columns: queries and sums of sixteen rows would not fit the registers; they are read in two parts)
+    if (two && code == kInt8) launch_decode<D, kTwo, kInt8>(d, args, weights);
+    else if (two) launch_decode<D, kTwo, kE4m3>(d, args, weights);
+    else if (code == kInt8) launch_decode<D, 1, kInt8>(d, args, weights);
+    else launch_decode<D, 1, kE4m3>(d, args, weights);
+}
+
+constexpr uint64_t kFewQueries = 64;   // query rows a K/V head up to which the decode kernel takes a sequence
+
+static void attention(Device& d, const void* const* states, const uint64_t* contexts, const uint64_t* lengths, const uint64_t* rows,
+                      uint64_t sequences, uint64_t heads, uint64_t kv_heads, uint64_t dim, int code, float scale, float cap, const float* slopes,
+                      uint64_t window, const uint64_t* prefixes, const void* q, uint64_t q_stride, float* const* weights, void* out,
+                      uint64_t out_stride, int type) {
+    check_shape(sequences, kv_heads, dim, code);
+    attn::check_rule(heads, kv_heads, dim, scale, cap, type);
+    if (!states || !contexts || !lengths || !rows) throw std::runtime_error("invalid Straydog attention dimensions");
+    const uint64_t group = heads / kv_heads;
+    if (!q_stride) q_stride = heads * dim;
+    if (!out_stride) out_stride = heads * dim;
+    uint64_t total = 0;
+    for (uint64_t s = 0; s < sequences; ++s) {
+        check_state(d, states[s], contexts[s], kv_heads, dim);
+        if (lengths[s] > contexts[s] || rows[s] > (uint64_t(1) << 24)) throw std::runtime_error("invalid Straydog attention dimensions");
+        if (weights) {
+            if (rows[s] * group > kFewQueries) throw std::runtime_error("attention weights are added up for at most 64 query rows a K/V head");
+            span(d, weights[s], checked_product({kv_heads, contexts[s], 4}), "attention weights");
+            if (reinterpret_cast<uintptr_t>(weights[s]) % 4) throw std::runtime_error("attention weights must be 4-byte aligned");
+        }
+        total += rows[s];
+    }
+    if (weights) check_distinct(reinterpret_cast<const void* const*>(weights), sequences);
+    if (!total) return;
+    attn::check_rows(d, q, total, q_stride, heads * dim, "attention queries");
+    attn::check_rows(d, out, total, out_stride, heads * dim, "an attention output");
+    if (slopes) span(d, slopes, checked_product({heads, 4}), "attention slopes");
+    if (overlap(q, ((total - 1) * q_stride + heads * dim) * 2, out, ((total - 1) * out_stride + heads * dim) * 2))
+        throw std::runtime_error("an attention output lies over its queries");
+
+    AttentionArgs args{};
+    args.heads = uint32_t(heads); args.kv_heads = uint32_t(kv_heads); args.group = uint32_t(group);
+    args.q = q; args.out = out; args.slopes = slopes;
+    args.q_stride = q_stride; args.out_stride = out_stride;
+    args.scale_log2 = scale * 1.4426950408889634f;
+    args.cap = cap * 1.4426950408889634f;
+    args.scale_over_cap = cap > 0.0f ? scale / cap : 0.0f;
+    args.window = uint32_t(std::min<uint64_t>(window, uint64_t(1) << 25));
+    args.bf16 = type == kBf16;
+    std::vector<attn::Sequence> chunks;   // what goes to the prompt kernel
+    uint64_t row = 0, most = 0;
+    auto flush = [&] {
+        if (!args.sequences) return;
+        const bool two = most > 8;
+        if (dim == 64) launch_queries<64>(d, args, code, weights != nullptr, two);
+        else if (dim == 128) launch_queries<128>(d, args, code, weights != nullptr, two);
+        else launch_queries<256>(d, args, code, weights != nullptr, two);
+        args.sequences = 0;
+        most = 0;
+    };
+    for (uint64_t s = 0; s < sequences; ++s) {
+        const uint64_t prefix = prefixes ? std::min(prefixes[s], lengths[s]) : 0;
+        if (rows[s] && rows[s] * group <= kFewQueries) {
+            AttentionSequence& to = args.sequence[args.sequences++];
+            to = AttentionSequence{};
+            to.state = static_cast<const uint8_t*>(states[s]);
+            to.weights = weights ? weights[s] : nullptr;
+            to.context = uint32_t(contexts[s]); to.length = uint32_t(lengths[s]); to.rows = uint32_t(rows[s]);
+            to.first_row = uint32_t(row); to.prefix = uint32_t(prefix);
+            most = std::max(most, rows[s] * group);
+            if (args.sequences == kSequences) flush();
+        } else if (rows[s]) {
+            attn::Sequence to{};
+            to.state = static_cast<const uint8_t*>(states[s]);
+            to.context = contexts[s]; to.length = lengths[s]; to.rows = rows[s]; to.first_row = row; to.prefix = prefix;
+            chunks.push_back(to);
+        }
+        row += rows[s];
+    }
+    flush();
+    if (!chunks.empty()) attn::attend_kv8(d, chunks, heads, kv_heads, dim, code, scale, cap, slopes, window, q, q_stride, out, out_stride, type);
+}
+
+}  // namespace kv8
+}  // namespace sdb
+
+using namespace sdb;
+
+extern "C" int sdx_kv8_attention(void* handle, const void* const* states, const uint64_t* contexts, const uint64_t* lengths,
+                                 const uint64_t* rows, uint64_t sequences, uint64_t heads, uint64_t kv_heads, uint64_t dim, int code, float scale,
+                                 float cap, const float* slopes, uint64_t window, const uint64_t* prefixes, const void* q, uint64_t q_stride,
+                                 float* const* weights, void* out, uint64_t out_stride, int type) {
+    SDB_OP_BEGIN
+    kv8::attention(value, states, contexts, lengths, rows, sequences, heads, kv_heads, dim, code, scale, cap, slopes, window, prefixes, q, q_stride,
+                   weights, out, out_stride, type);
+    SDB_OP_END
+}

@@ -1,0 +1,312 @@
+// Eviction from states of 8-bit rows by accumulated attention weight (csrc/kv8.cuh has the layout).
+//
+// Of a sequence of n > keep positions each K/V head keeps the first `sinks`, the last `recent` and, of those between, the
+// keep - sinks - recent with the greatest weights (equal weights: the lower position; a NaN below every number). The kept rows move, in
+// their order, to positions 0 .. keep - 1 of another state. A target block takes the largest scale among the blocks its rows come from,
+// and rows from a block with a smaller scale have their codes rounded again in it: the rule of an append to a begun block.
+//
+// kv8_evict_select_kernel: a cluster of 1 to 8 blocks a (sequence, head) finds the weight of the last place by sixteen steps of two bits each
+// (how many weights are at or above three candidate values), with the weights in registers: a step is a few compares a weight and one
+// exchange. Counting by compares costs no atomics, whatever the weights look like (a histogram's atomics meet in one bin when most weights are
+// equal, as the weights of never-attended rows are). Then ballots give every kept position its place in order.
+// kv8_evict_move_kernel: a block of 128 threads a (sequence, plane, target block of 32 rows): bound by memory, rows of `dim` bytes gathered.
+#include "kv8.cuh"
+#include "../../include/straydog_gpu_b200.h"
+
+#include <cooperative_groups.h>
+
+namespace sdb {
+namespace kv8 {
+
+struct EvictSequence {
+    const uint8_t* state;
+    uint8_t* target;
+    const float* weights;
+    float* target_weights;
+    uint32_t context, length, target_context, first_unit;
+};
+struct EvictArgs {
+    EvictSequence sequence[kSequences];
+    int32_t* kept;      // [sequences of this launch][kv_heads][keep]
+    uint32_t sequences, kv_heads, keep, sinks, recent;
+};
+
+constexpr int kSelectThreads = 1024, kSelectWarps = 32, kHeld = 32, kMostCluster = 8;   // weights a thread holds; blocks a head
+
+// weights in an order of unsigned integers: NaN 0, then -inf .. +inf; the two zeros are equal
+__device__ __forceinline__ uint32_t order_of(float w) {
+    if (w != w) return 0;
+    const uint32_t b = __float_as_uint(w + 0.0f);
+    return b & 0x80000000u ? ~b : b | 0x80000000u;
+}
+
+template<bool HELD>
+__global__ void __launch_bounds__(kSelectThreads, 1) kv8_evict_select_kernel(const __grid_constant__ EvictArgs a, uint32_t ctas) {
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    __shared__ uint32_t warp_counts[kSelectWarps][3];
+    __shared__ uint32_t shares[2][kMostCluster][3];   // every block's counts, written by that block into each block's copy; by parity of the step
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    if (ctas > 1) cluster.sync();   // (no block stores into another's shared memory before that one runs)
+    const uint32_t unit = blockIdx.x / ctas, rank = blockIdx.x % ctas, s = unit / a.kv_heads, head = unit % a.kv_heads;
+    const EvictSequence& sequence = a.sequence[s];
+    const uint32_t length = sequence.length, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
+    const bool all = length <= a.keep;
+    const uint32_t sinks = all ? length : a.sinks, recent = all ? 0 : a.recent, want = all ? 0 : a.keep - a.sinks - a.recent;
+    const uint32_t between = length - sinks - recent;
+    const float* weights = sequence.weights + size_t(head) * sequence.context;
+    float* target_weights = sequence.target_weights + size_t(head) * sequence.target_context;
+    int32_t* kept = a.kept + (size_t(s) * a.kv_heads + head) * a.keep;
+    for (uint32_t i = rank * kSelectThreads + threadIdx.x; i < sinks + recent; i += ctas * kSelectThreads) {
+        const uint32_t place = i < sinks ? i : want + i, from = i < sinks ? i : length - recent + (i - sinks);
+        kept[place] = int32_t(from);
+        target_weights[place] = weights[from];
+    }
+    // a warp's weights are consecutive: `each` steps of 32
+    const uint32_t each = (between + ctas * kSelectThreads - 1) / (ctas * kSelectThreads);
+    const uint32_t first = (rank * kSelectWarps + warp) * each * 32;
+    const float* mine = weights + sinks;
+    uint32_t key[HELD ? kHeld : 1];
+    auto load = [&](uint32_t j) -> uint32_t { const uint32_t i = first + j * 32 + lane; return i < between ? order_of(mine[i]) : 0u; };
+    if (HELD) {
+        #pragma unroll
+        for (int j = 0; j < kHeld; ++j) key[j] = uint32_t(j) < each ? load(j) : 0u;
+    }
+    auto count_at = [&](const uint32_t (&bound)[3], uint32_t (&counts)[3]) {
+        counts[0] = counts[1] = counts[2] = 0;
+        auto add = [&](uint32_t k) {
+            #pragma unroll
+            for (int c = 0; c < 3; ++c) counts[c] += k >= bound[c];
+        };
+        if (HELD) {
+            #pragma unroll
+            for (int j = 0; j < kHeld; ++j) if (uint32_t(j) < each) add(key[j]);
+        } else {
+            for (uint32_t j = 0; j < each; ++j) add(load(j));
+        }
+    };
+    int step = 0;
+    // sums of three counts over the head's weights; every block of the cluster gets them, and its own blocks' shares stay in shares[]
+    auto sum = [&](uint32_t (&counts)[3], uint32_t (&total)[3], uint32_t (&before)[3]) {
+        #pragma unroll
+        for (int c = 0; c < 3; ++c) counts[c] = __reduce_add_sync(0xffffffffu, counts[c]);
+        if (lane == 0) { warp_counts[warp][0] = counts[0]; warp_counts[warp][1] = counts[1]; warp_counts[warp][2] = counts[2]; }
+        __syncthreads();
+        const int parity = step++ & 1;
+        if (warp == 0) {
+            #pragma unroll
+            for (int c = 0; c < 3; ++c) {
+                const uint32_t block_total = __reduce_add_sync(0xffffffffu, warp_counts[lane][c]);
+                if (lane < ctas) cluster.map_shared_rank(&shares[0][0][0], lane)[(parity * kMostCluster + rank) * 3 + c] = block_total;
+            }
+        }
+        if (ctas > 1) cluster.sync(); else __syncthreads();
+        #pragma unroll
+        for (int c = 0; c < 3; ++c) {
+            total[c] = before[c] = 0;
+            for (uint32_t r = 0; r < ctas; ++r) { const uint32_t v = shares[parity][r][c]; total[c] += v; if (r < rank) before[c] += v; }
+        }
+    };
+    uint32_t last = 0xffffffffu;   // the key of the last place: the greatest value that `want` keys or more reach
+    uint32_t counts[3], total[3], before[3];
+    if (want) {
+        last = 0;
+        #pragma unroll 1
+        for (int shift = 30; shift >= 0; shift -= 2) {
+            const uint32_t bound[3] = {last | 1u << shift, last | 2u << shift, last | 3u << shift};
+            count_at(bound, counts);
+            sum(counts, total, before);
+            last = total[2] >= want ? bound[2] : total[1] >= want ? bound[1] : total[0] >= want ? bound[0] : last;
+        }
+    }
+    // places: keys above `last` all stay, of those equal to it the first want - above
+    {
+        const uint32_t bound[3] = {last, last == 0xffffffffu ? last : last + 1, 0xffffffffu};   // (no key is 2^32 - 1)
+        count_at(bound, counts);
+        // weights past the end count as key 0, behind every weight: they only matter when `last` is 0, and then lie behind the places wanted
+        sum(counts, total, before);
+        uint32_t reach = before[0], above = before[1];
+        for (uint32_t w = 0; w < warp; ++w) { reach += warp_counts[w][0]; above += warp_counts[w][1]; }
+        const uint32_t ties = want - min(want, total[1]);
+        uint32_t equal = reach - above;
+        uint32_t place = sinks + above + min(equal, ties);
+        const uint32_t below = (1u << lane) - 1u;
+        auto put = [&](uint32_t j, uint32_t k) {
+            const bool greater = want && k > last, tie = want && k == last;
+            const uint32_t ties_here = __ballot_sync(0xffffffffu, tie);
+            const bool stays = greater || (tie && equal + __popc(ties_here & below) < ties);
+            const uint32_t staying = __ballot_sync(0xffffffffu, stays);
+            if (stays) {
+                const uint32_t i = first + j * 32 + lane, at = place + __popc(staying & below);
+                kept[at] = int32_t(sinks + i);
+                target_weights[at] = mine[i];
+            }
+            equal += __popc(ties_here);
+            place += __popc(staying);
+        };
+        if (HELD) {
+            #pragma unroll
+            for (int j = 0; j < kHeld; ++j) if (uint32_t(j) < each) put(j, key[j]);
+        } else {
+            for (uint32_t j = 0; j < each; ++j) put(j, load(j));
+        }
+    }
+    if (ctas > 1) cluster.sync();   // (no block leaves while another may still store into its shares)
+}
+
+template<int D, int CODE>
+__global__ void __launch_bounds__(128) kv8_evict_move_kernel(const __grid_constant__ EvictArgs a) {
+    constexpr int kPieces = D / 16, kRows = 128 / kPieces, kPasses = int(kBlock) / kRows;   // threads a row, rows a pass
+    uint32_t s = 0;
+    {
+        uint32_t high = a.sequences;
+        while (high - s > 1) { const uint32_t mid = (s + high) / 2; if (a.sequence[mid].first_unit <= blockIdx.x) s = mid; else high = mid; }
+    }
+    const EvictSequence& sequence = a.sequence[s];
+    const uint32_t planes = 2 * a.kv_heads, unit = blockIdx.x - sequence.first_unit, plane = unit % planes, block = unit / planes;
+    const uint32_t rows = min(min(sequence.length, a.keep) - block * kBlock, kBlock);
+    const uint32_t row = threadIdx.x / kPieces, piece = threadIdx.x % kPieces;
+    const int32_t* kept = a.kept + (size_t(s) * a.kv_heads + plane % a.kv_heads) * a.keep + block * kBlock;
+    const uint8_t* codes = sequence.state + size_t(plane) * sequence.context * D;
+    const float* scales = reinterpret_cast<const float*>(sequence.state + size_t(planes) * sequence.context * D) + size_t(plane) * (sequence.context / kBlock);
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // the positions are the kernel's before
+    uint4 v[kPasses];
+    float old[kPasses];
+    #pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+        const uint32_t r = p * kRows + row;
+        const uint32_t from = r < rows ? uint32_t(kept[r]) : 0u;
+        old[p] = r < rows ? scales[from / kBlock] : 0.0f;
+        v[p] = r < rows ? *reinterpret_cast<const uint4*>(codes + size_t(from) * D + piece * 16) : make_uint4(0, 0, 0, 0);
+    }
+    float top = 0.0f;
+    #pragma unroll
+    for (int p = 0; p < kPasses; ++p) top = fmaxf(top, old[p]);
+    #pragma unroll
+    for (int offset = 16; offset; offset /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, offset));
+    __shared__ float tops[4];
+    if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = top;
+    __syncthreads();
+    const float scale = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    uint8_t* to = sequence.target + (size_t(plane) * sequence.target_context + block * kBlock) * D + piece * 16;
+    #pragma unroll
+    for (int p = 0; p < kPasses; ++p) {
+        const uint32_t r = p * kRows + row;
+        if (r >= rows) continue;
+        const float ratio = scale > 0.0f ? __fdiv_rn(old[p], scale) : 0.0f;
+        *reinterpret_cast<uint4*>(to + size_t(r) * D) = recode16<CODE>(v[p], ratio);
+    }
+    if (threadIdx.x == 0)
+        reinterpret_cast<float*>(sequence.target + size_t(planes) * sequence.target_context * D)[size_t(plane) * (sequence.target_context / kBlock) + block] = scale;
+}
+
+static void launch_move(Device& d, uint64_t dim, int code, const EvictArgs& args, uint32_t units) {
+    cudaLaunchConfig_t config{};
+    config.gridDim = dim3(units);
+    config.blockDim = dim3(128);
+    config.stream = d.stream;
+    cudaLaunchAttribute attribute{};
+    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attribute.val.programmaticStreamSerializationAllowed = 1;
+    config.attrs = &attribute;
+    config.numAttrs = 1;
+    const auto kernel = dim == 64    ? (code == kInt8 ? kv8_evict_move_kernel<64, kInt8> : kv8_evict_move_kernel<64, kE4m3>)
+                        : dim == 128 ? (code == kInt8 ? kv8_evict_move_kernel<128, kInt8> : kv8_evict_move_kernel<128, kE4m3>)
+                                     : (code == kInt8 ? kv8_evict_move_kernel<256, kInt8> : kv8_evict_move_kernel<256, kE4m3>);
+    SDB_CHECK(cudaLaunchKernelEx(&config, kernel, args));
+    ++d.launches;
+}
+
+static void evict(Device& d, const void* const* states, const uint64_t* contexts, const uint64_t* lengths, const float* const* weights,
+                  uint64_t sequences, uint64_t keep, uint64_t sinks, uint64_t recent, uint64_t kv_heads, uint64_t dim, int code,
+                  void* const* targets, const uint64_t* target_contexts, float* const* target_weights, int32_t* kept) {
+    check_shape(sequences, kv_heads, dim, code);
+    if (!states || !contexts || !lengths || !weights || !targets || !target_contexts || !target_weights)
+        throw std::runtime_error("invalid Straydog eviction");
+    if (!keep || keep > (uint64_t(1) << 24) || sinks > keep || recent > keep - sinks)
+        throw std::runtime_error("an eviction keeps at least its sinks and its recent positions, at most 2^24");
+    std::vector<std::pair<uintptr_t, uintptr_t>> written, read;
+    auto range = [](std::vector<std::pair<uintptr_t, uintptr_t>>& list, const void* p, size_t bytes) {
+        list.emplace_back(reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + bytes);
+    };
+    for (uint64_t s = 0; s < sequences; ++s) {
+        check_state(d, states[s], contexts[s], kv_heads, dim);
+        check_state(d, targets[s], target_contexts[s], kv_heads, dim);
+        if (lengths[s] > contexts[s] || std::min(lengths[s], keep) > target_contexts[s])
+            throw std::runtime_error("an eviction's lengths do not fit its states");
+        const size_t from = checked_product({kv_heads, contexts[s], 4}), to = checked_product({kv_heads, target_contexts[s], 4});
+        span(d, weights[s], from, "attention weights");
+        span(d, target_weights[s], to, "an eviction's target weights");
+        if (reinterpret_cast<uintptr_t>(weights[s]) % 4 || reinterpret_cast<uintptr_t>(target_weights[s]) % 4)
+            throw std::runtime_error("attention weights must be 4-byte aligned");
+        range(read, states[s], state_bytes(contexts[s], kv_heads, dim));
+        range(read, weights[s], from);
+        range(written, targets[s], state_bytes(target_contexts[s], kv_heads, dim));
+        range(written, target_weights[s], to);
+    }
+    if (kept) {
+        const size_t bytes = checked_product({sequences, kv_heads, keep, 4});
+        span(d, kept, bytes, "an eviction's positions");
+        if (reinterpret_cast<uintptr_t>(kept) % 4) throw std::runtime_error("an eviction's positions must be 4-byte aligned");
+        range(written, kept, bytes);
+    }
+    // what is written lies apart from everything else: rows move between blocks that run in any order
+    std::sort(written.begin(), written.end());
+    std::sort(read.begin(), read.end());
+    for (size_t i = 1; i < written.size(); ++i)
+        if (written[i].first < written[i - 1].second) throw std::runtime_error("an eviction's targets overlap");
+    for (size_t i = 0, j = 0; i < read.size(); ++i) {
+        while (j < written.size() && written[j].second <= read[i].first) ++j;
+        if (j < written.size() && written[j].first < read[i].second) throw std::runtime_error("an eviction's target overlaps what it reads");
+    }
+    if (!kept) kept = static_cast<int32_t*>(workspace(d, d.kv8_kept, checked_product({sequences, kv_heads, keep, 4})));
+    for (uint64_t at = 0; at < sequences;) {
+        EvictArgs args{};
+        args.kv_heads = uint32_t(kv_heads); args.keep = uint32_t(keep); args.sinks = uint32_t(sinks); args.recent = uint32_t(recent);
+        args.kept = kept + at * kv_heads * keep;
+        uint64_t units = 0, longest = 0;
+        for (; at < sequences && args.sequences < kSequences; ++at) {
+            const uint64_t more = (std::min(lengths[at], keep) + kBlock - 1) / kBlock * 2 * kv_heads;
+            if (units + more >= uint64_t(1) << 31) break;
+            args.sequence[args.sequences++] = EvictSequence{static_cast<const uint8_t*>(states[at]), static_cast<uint8_t*>(targets[at]), weights[at],
+                                                            target_weights[at], uint32_t(contexts[at]), uint32_t(lengths[at]),
+                                                            uint32_t(target_contexts[at]), uint32_t(units)};
+            units += more;
+            longest = std::max(longest, lengths[at]);
+        }
+        if (!units) continue;   // (every sequence of the group is empty)
+        // Blocks a head: enough for the weights to fit the registers, and twice as many again while the heads leave SMs idle
+        uint32_t ctas = 1;
+        const uint64_t heads = args.sequences * kv_heads;
+        while (ctas < kMostCluster && longest > uint64_t(ctas) * kSelectThreads * kHeld) ctas *= 2;
+        while (ctas < kMostCluster && heads * ctas * 2 <= uint64_t(d.sms) && longest > uint64_t(ctas) * kSelectThreads * 4) ctas *= 2;
+        const bool held = longest <= uint64_t(ctas) * kSelectThreads * kHeld;
+        cudaLaunchConfig_t config{};
+        config.gridDim = dim3(unsigned(heads * ctas));
+        config.blockDim = dim3(kSelectThreads);
+        config.stream = d.stream;
+        cudaLaunchAttribute attribute{};
+        attribute.id = cudaLaunchAttributeClusterDimension;
+        attribute.val.clusterDim.x = ctas; attribute.val.clusterDim.y = 1; attribute.val.clusterDim.z = 1;
+        config.attrs = &attribute;
+        config.numAttrs = 1;
+        SDB_CHECK(cudaLaunchKernelEx(&config, held ? kv8_evict_select_kernel<true> : kv8_evict_select_kernel<false>, args, ctas));
+        ++d.launches;
+        launch_move(d, dim, code, args, uint32_t(units));
+    }
+}
+
+}  // namespace kv8
+}  // namespace sdb
+
+using namespace sdb;
+
+extern "C" int sdx_kv8_evict(void* handle, const void* const* states, const uint64_t* contexts, const uint64_t* lengths,
+                             const float* const* weights, uint64_t sequences, uint64_t keep, uint64_t sinks, uint64_t recent, uint64_t kv_heads,
+                             uint64_t dim, int code, void* const* targets, const uint64_t* target_contexts, float* const* target_weights,
+                             int32_t* kept) {
+    SDB_OP_BEGIN
+    kv8::evict(value, states, contexts, lengths, weights, sequences, keep, sinks, recent, kv_heads, dim, code, targets, target_contexts,
+               target_weights, kept);
+    SDB_OP_END
+}
