@@ -3,22 +3,27 @@
 //
 //   s(r, j) = scale * q_r . (code_j * key scale of j's block), capped, biased by distance, masked;   out_r = sum_j softmax(s)_j * v_j
 //
-// The query rows of one K/V head (rows x heads a K/V head: up to 16 at a time, 8 of 256 columns) read its K and V once: 2 * dim bytes a position, 8 to 32 flops a byte,
-// so memory binds this. The work of a batch is every sequence's (K/V head, tile of keys) laid end to end and cut into equal runs, one a block
-// (one block of eight warps an SM): ragged lengths balance to within a tile. A block's run is one piece a (sequence, K/V head) it crosses.
-// The warps take a piece's tiles in turn; each has a ring of tiles in shared memory filled by 16-byte asynchronous copies, two or more
-// tiles ahead, pieces' borders not minded. The arithmetic is on mma.sync (16 keys x 8 queries x 16 columns): int8 and E4M3 codes become FP16
-// exactly by byte permutes; the blocks' scales multiply scores and weighted sums in FP32. Softmax is online, in the exp2 domain. Queries
-// enter as FP16: BF16 rows are multiplied by a power of two that brings their largest value to 2^14 (exact), undone on the scores.
-// Weights enter the value product as FP16 at 2^10 times their size (the running maximum has 2^10): 11 bits down to 2^-24 of the largest.
-// A piece's eight partial results meet in shared memory; a piece that is all of its (sequence, K/V head) writes the output, the others
-// leave FP32 partials that a second kernel joins. Where a piece is cut depends on the batch, the order of the sums inside it does not.
+// The query rows of one K/V head (rows x heads a K/V head: up to 16 at a time, 8 of 256 columns) read its K and V once: 2 * dim bytes a position,
+// 8 to 32 flops a byte, so memory binds this. The work of a batch is every sequence's (K/V head, tile of keys) laid end to end and cut into equal
+// runs, one a warp (a block of eight warps an SM): ragged lengths balance to within a tile. A warp's run is one piece a (sequence, K/V head) it
+// crosses. No warp waits for another: each has a ring of tiles in shared memory filled by its own 16-byte asynchronous copies, two or more tiles
+// ahead, pieces' borders not minded. (With the pieces cut a block and the eight warps' sums joined in shared memory, every piece cost its block
+// about 5 us of barriers and first loads: 78 us for 16 sequences of 4 rows and 167 MB.) The arithmetic is on mma.sync (16 keys x 8 queries x
+// 16 columns): int8 and E4M3 codes become FP16 exactly by byte permutes; the blocks' scales multiply scores and weighted sums in FP32. Softmax is
+// online, in the exp2 domain. Queries enter as FP16: BF16 rows are multiplied by a power of two that brings their largest value to 2^14 (exact),
+// undone on the scores. Weights enter the value product as FP16 at 2^10 times their size (the running maximum has 2^10): 11 bits down to 2^-24 of
+// the largest. A piece that is all of its (sequence, K/V head) writes the output, the others leave FP32 partials that a second kernel joins in
+// order. Where a piece is cut depends on the batch, the order of the sums inside it does not.
 #include "kv8.cuh"
 #include "masked_attention.cuh"
 #include "../../include/straydog_gpu_b200.h"
 
 namespace sdb {
 namespace kv8 {
+
+using attn::any_tanh;
+using attn::kSmallTanh;
+using attn::small_tanh;
 
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
 constexpr float kLift = 10.0f;   // log2 of what weights are multiplied by on their way to FP16
@@ -31,12 +36,14 @@ struct AttentionSequence {
     uint32_t head_tiles, jump;   // tiles below head_tiles are at their place, the others `jump` tiles further on (keys no row sees are passed over)
     uint32_t first_unit;
     uint32_t parts;          // how often a K/V head's rows are read: query rows over queries a unit
+    uint32_t score_queries;  // queries of a tile's scores (a multiple of four)
     uint64_t first_tile;     // of all sequences' tiles
+    uint64_t first_score;    // of all sequences' scores
 };
 struct AttentionArgs {
     AttentionSequence sequence[kSequences];
     uint32_t sequences, heads, kv_heads, group, units;
-    uint64_t tiles, tiles_a_block;
+    uint64_t tiles, tiles_a_warp;
     const void* q;
     void* out;
     const float* slopes;
@@ -44,15 +51,17 @@ struct AttentionArgs {
     float scale_log2, cap, scale_over_cap;
     uint32_t window;
     int bf16;
-    float* partial;          // [block + unit][queries][D], then [block + unit][queries][2]
-    float* sums;             // [block + unit][queries][2]: maximum (exp2 domain, lifted), denominator
-    float* scores;           // [tile][keys][queries] or null
+    float* partial;          // [warp + unit][queries][D]: a run's next piece has the next unit, a unit's next piece the next warp
+    float* sums;             // [warp + unit][queries][2]: maximum (exp2 domain, lifted), denominator
+    float* scores;           // [tile][keys][score_queries] or null
     float* stats;            // [unit][queries][2]: final maximum and denominator, for the weights
 };
 
 __device__ __forceinline__ void copy16(uint32_t to, const void* from) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
+// 1 / a row's sum of weights; 0 for a row that has seen nothing, NaN for one of NaN scores
+__device__ __forceinline__ float inverse_of(float sum) { return sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum; }
 __device__ __forceinline__ void copy4(uint32_t to, const void* from) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
 }
@@ -80,14 +89,10 @@ template<int D, int NT> struct Shape {
     static constexpr int kQueries = 8 * NT;
     static constexpr int kPlane = kTile * D, kSlot = 2 * kPlane;      // bytes
     static constexpr int kStages = D == 64 ? 6 : 3;
-    static constexpr int kChunk = 16384 / (kWarps * kQueries * 4) < D ? 16384 / (kWarps * kQueries * 4) : D;   // columns that meet at a time
-    static constexpr int kRing = kWarps * kStages * kSlot, kScales = kWarps * kStages * 8;
-    static constexpr int kJoin = kWarps * kQueries * (kChunk + 4) * 4;
-    static constexpr int kStats = kWarps * kQueries * 8;
-    static constexpr int kSmem = kRing + kScales + kJoin + kStats;
+    static constexpr int kRing = kWarps * kStages * kSlot, kSmem = kRing + kWarps * kStages * 8;
 };
 
-// A walk over the tiles of a block's run: the (sequence, unit) a tile belongs to, without divisions after the first.
+// A walk over the tiles of a warp's run: the (sequence, unit) a tile belongs to, without divisions after the first.
 struct Place {
     uint32_t s, unit;        // unit: counted over all sequences
     uint64_t begin, end;     // tiles of the unit
@@ -116,18 +121,17 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
     const int warp = threadIdx.x / 32, lane = threadIdx.x % 32, g = lane / 4, t = lane % 4;
     uint8_t* ring = smem + warp * (S::kStages * S::kSlot);
     float* ring_scales = reinterpret_cast<float*>(smem + S::kRing) + warp * (S::kStages * 2);
-    float* join = reinterpret_cast<float*>(smem + S::kRing + S::kScales);
-    float* stat = reinterpret_cast<float*>(smem + S::kRing + S::kScales + S::kJoin);   // [warp][query][maximum, denominator]
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 
-    const uint64_t run_begin = blockIdx.x * a.tiles_a_block, run_end = min(run_begin + a.tiles_a_block, a.tiles);
+    const uint64_t run = uint64_t(warp) * gridDim.x + blockIdx.x;   // (few warps are spread over many SMs rather than filling one)
+    const uint64_t run_begin = run * a.tiles_a_warp, run_end = min(run_begin + a.tiles_a_warp, a.tiles);
     if (run_begin >= run_end) return;
 
-    // ---- the copies: this warp's tiles run_begin + warp, + 8, ... ----
+    // ---- the copies ----
     Place at;
     at.find(a, run_begin);
     Place ahead = at;
-    uint64_t ahead_tile = run_begin + warp;
+    uint64_t ahead_tile = run_begin;
     // Rows are laid in a slot as they lie in memory, their 16-byte pieces exchanged so that the reads below meet in no bank: keys by the
     // row's parity (a read takes 64 bytes of each of two neighbouring rows), values by the row's low bits (a transposing read takes one
     // piece of each of eight rows).
@@ -136,7 +140,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
     const uint32_t ring_address = smem_u32(ring), scales_address = smem_u32(ring_scales);
     auto fetch = [&](int slot) {
         if (ahead_tile < run_end) {
-            while (ahead_tile >= ahead.end) ahead.next(a);
+            if (ahead_tile >= ahead.end) ahead.next(a);
             const AttentionSequence& q = a.sequence[ahead.s];
             uint32_t tile = uint32_t(ahead_tile - ahead.begin);
             if (tile >= q.head_tiles) tile += q.jump;
@@ -161,7 +165,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
                 const float* scales = reinterpret_cast<const float*>(q.state + size_t(2 * a.kv_heads) * q.context * D);
                 copy4(scales_address + slot * 8 + lane * 4, scales + (lane ? v_row : k_row) / kBlock);
             }
-            ahead_tile += kWarps;
+            ++ahead_tile;
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
     };
@@ -170,7 +174,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
 
     const uint32_t v_lane = uint32_t(lane % 8 + 8 * ((lane / 8) & 1));   // the key row this lane's address names in a transposing read
     int slot = 0, fill = S::kStages - 1;
-    uint64_t tile_id = run_begin + warp;
+    uint64_t tile_id = run_begin;
 
     for (;;) {
         // ---- a piece: the part of the run that lies in one (sequence, K/V head, part) ----
@@ -223,6 +227,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
                 slope[n][i] = there && a.slopes ? a.slopes[kv * a.group + other % a.group] * 1.4426950408889634f : 0.0f;
             }
         }
+        // tiles that every row sees whole need no mask: keys up to `open_to`, above `open_from`, or below `open_prefix`
+        const int first_position = int(sequence.length) - int(sequence.rows);
+        const int open_to = min(first_position, int(sequence.length) - 1), open_from = a.window ? int(sequence.length) - 1 - int(a.window) : -1;
+        const int open_prefix = int(sequence.prefix);
         float o[D / 16][NT][4], m[NT][2], l[NT][2];
         #pragma unroll
         for (int n = 0; n < NT; ++n) {
@@ -233,7 +241,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
                 for (int c = 0; c < 4; ++c) o[i][n][c] = 0.0f;
         }
 
-        for (; tile_id < piece_end; tile_id += kWarps) {
+        for (; tile_id < piece_end; ++tile_id) {
             __syncwarp();   // (all lanes are past their reads of the slot to fill)
             fetch(fill);
             fill = fill + 1 == S::kStages ? 0 : fill + 1;
@@ -270,24 +278,65 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
                 #pragma unroll
                 for (int n = 0; n < NT; ++n)
                     #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        const int i = c & 1, key = key0 + 16 * h + g + 8 * (c >> 1);
-                        float s = acc[n][c] * (k_scale * unscale[n][i]);
-                        s = a.cap > 0.0f ? a.cap * tanhf(s * a.scale_over_cap) : s * a.scale_log2;   // (the cap is in the exp2 domain too)
-                        s = fmaf(-slope[n][i], fabsf(float(position[n][i] - key)), s);
-                        const bool seen = ((key <= position[n][i] && key > low[n][i]) || uint32_t(key) < prefix[n][i]) && key < int(sequence.length);
-                        x[h][n][c] = seen ? s : -INFINITY;
-                    }
+                    for (int c = 0; c < 4; ++c) x[h][n][c] = acc[n][c];
+            }
+            const float to_score = k_scale * (a.cap > 0.0f ? a.scale_over_cap : a.scale_log2);
+            #pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const float factor[2] = {to_score * unscale[n][0], to_score * unscale[n][1]};
+                #pragma unroll
+                for (int h = 0; h < S::kTile / 16; ++h)
+                    #pragma unroll
+                    for (int c = 0; c < 4; ++c) x[h][n][c] *= factor[c & 1];
+            }
+            if (a.cap > 0.0f) {   // (the cap is in the exp2 domain too)
+                bool small = true;
+                #pragma unroll
+                for (int h = 0; h < S::kTile / 16; ++h)
+                    #pragma unroll
+                    for (int n = 0; n < NT; ++n)
+                        #pragma unroll
+                        for (int c = 0; c < 4; ++c) small &= fabsf(x[h][n][c]) <= kSmallTanh;
+                const bool all_small = __all_sync(0xffffffffu, small);   // (the usual case: scores well below the cap)
+                #pragma unroll
+                for (int h = 0; h < S::kTile / 16; ++h)
+                    #pragma unroll
+                    for (int n = 0; n < NT; ++n)
+                        #pragma unroll
+                        for (int c = 0; c < 4; ++c) x[h][n][c] = a.cap * (all_small ? small_tanh(x[h][n][c]) : any_tanh(x[h][n][c]));
+            }
+            if (a.slopes) {
+                #pragma unroll
+                for (int h = 0; h < S::kTile / 16; ++h)
+                    #pragma unroll
+                    for (int n = 0; n < NT; ++n)
+                        #pragma unroll
+                        for (int c = 0; c < 4; ++c)
+                            x[h][n][c] = fmaf(-slope[n][c & 1], fabsf(float(position[n][c & 1] - (key0 + 16 * h + g + 8 * (c >> 1)))), x[h][n][c]);
+            }
+            if (!((key0 + S::kTile - 1 <= open_to && key0 > open_from) || key0 + S::kTile <= open_prefix)) {
+                #pragma unroll
+                for (int h = 0; h < S::kTile / 16; ++h)
+                    #pragma unroll
+                    for (int n = 0; n < NT; ++n)
+                        #pragma unroll
+                        for (int c = 0; c < 4; ++c) {
+                            const int i = c & 1, key = key0 + 16 * h + g + 8 * (c >> 1);
+                            const bool seen = ((key <= position[n][i] && key > low[n][i]) || uint32_t(key) < prefix[n][i]) && key < int(sequence.length);
+                            if (!seen) x[h][n][c] = -INFINITY;
+                        }
             }
             if (a.scores) {
-                float* to = a.scores + size_t(tile_id) * (S::kTile * S::kQueries);
+                const uint32_t queries_kept = sequence.score_queries;
+                float* to = a.scores + sequence.first_score + (tile_id - sequence.first_tile) * (S::kTile * queries_kept);
                 #pragma unroll
                 for (int h = 0; h < S::kTile / 16; ++h)
                     #pragma unroll
                     for (int n = 0; n < NT; ++n)
                         #pragma unroll
                         for (int i = 0; i < 2; ++i)
-                            *reinterpret_cast<float2*>(to + (16 * h + g + 8 * i) * S::kQueries + 8 * n + 2 * t) = make_float2(x[h][n][2 * i], x[h][n][2 * i + 1]);
+                            if (8 * n + 2 * t < int(queries_kept))
+                                *reinterpret_cast<float2*>(to + (16 * h + g + 8 * i) * queries_kept + 8 * n + 2 * t) = make_float2(x[h][n][2 * i], x[h][n][2 * i + 1]);
             }
             // ---- the running maximum (lifted) and the weights ----
             bool grew = false;
@@ -358,79 +407,52 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
             if (++slot == S::kStages) slot = 0;
         }
 
-        // ---- the warps' partial results of the piece meet ----
+        // ---- the piece's sums: o[i][n][c] is query 8n + 2t + (c & 1), column 16i + 2g + (c >> 1) ----
         #pragma unroll
         for (int n = 0; n < NT; ++n)
             #pragma unroll
-            for (int i = 0; i < 2; ++i) {
+            for (int i = 0; i < 2; ++i)
                 #pragma unroll
                 for (int offset = 4; offset < 32; offset *= 2) l[n][i] += __shfl_xor_sync(0xffffffffu, l[n][i], offset);
-                if (g == 0) *reinterpret_cast<float2*>(stat + (warp * S::kQueries + 8 * n + 2 * t + i) * 2) = make_float2(m[n][i], l[n][i]);
-            }
-        __syncthreads();
-        float factor[NT][2];
+        const bool whole = piece_end - max(at.begin, run_begin) == sequence.tiles;   // the piece is all of its unit
+        const size_t mine = size_t(run) + at.unit;
         #pragma unroll
         for (int n = 0; n < NT; ++n)
             #pragma unroll
             for (int i = 0; i < 2; ++i) {
-                float top = -INFINITY;
-                #pragma unroll
-                for (int w = 0; w < kWarps; ++w) top = fmaxf(top, stat[(w * S::kQueries + 8 * n + 2 * t + i) * 2]);
-                factor[n][i] = m[n][i] == -INFINITY ? 0.0f : fast_exp2(m[n][i] - top);   // (sums without a maximum are 0, or NaN: either stays)
+                const int query = 8 * n + 2 * t + i;
+                const uint32_t global = first_query + query;
+                if (global >= queries) continue;
+                if (whole) {
+                    const float inverse = inverse_of(l[n][i]);
+                    uint16_t* to = static_cast<uint16_t*>(a.out) + size_t(sequence.first_row + global / a.group) * a.out_stride + size_t(kv * a.group + global % a.group) * D + 2 * g;
+                    #pragma unroll
+                    for (int b = 0; b < D / 16; ++b) {
+                        const float v0 = o[b][n][i] * inverse, v1 = o[b][n][i + 2] * inverse;
+                        *reinterpret_cast<uint32_t*>(to + 16 * b) = a.bf16 ? pack_bf16x2(v0, v1) : pack_half2(v0, v1);
+                    }
+                    if (a.scores && g == 0) *reinterpret_cast<float2*>(a.stats + (size_t(at.unit) * S::kQueries + query) * 2) = make_float2(m[n][i], l[n][i]);
+                } else {
+                    float* to = a.partial + (mine * S::kQueries + query) * D + 2 * g;
+                    #pragma unroll
+                    for (int b = 0; b < D / 16; ++b) *reinterpret_cast<float2*>(to + 16 * b) = make_float2(o[b][n][i], o[b][n][i + 2]);
+                    if (g == 0) *reinterpret_cast<float2*>(a.sums + (mine * S::kQueries + query) * 2) = make_float2(m[n][i], l[n][i]);
+                }
             }
-        const bool whole = piece_end - max(at.begin, run_begin) == sequence.tiles;   // the piece is all of its unit
-        const size_t mine = size_t(blockIdx.x) + at.unit;
-        constexpr int kPitch = S::kChunk + 4;
-        #pragma unroll
-        for (int chunk = 0; chunk < D / S::kChunk; ++chunk) {
-            #pragma unroll
-            for (int i = 0; i < S::kChunk / 16; ++i)
-                #pragma unroll
-                for (int n = 0; n < NT; ++n) {
-                    const float (&v)[4] = o[chunk * (S::kChunk / 16) + i][n];
-                    float* to = join + (warp * S::kQueries + 8 * n + 2 * t) * kPitch + 16 * i + 2 * g;
-                    *reinterpret_cast<float2*>(to) = make_float2(v[0] * factor[n][0], v[2] * factor[n][0]);
-                    *reinterpret_cast<float2*>(to + kPitch) = make_float2(v[1] * factor[n][1], v[3] * factor[n][1]);
-                }
-            __syncthreads();
-            for (int e = threadIdx.x; e < S::kQueries * S::kChunk / 2; e += kThreads) {
-                const int query = e / (S::kChunk / 2), column = e % (S::kChunk / 2) * 2;
-                float2 total = make_float2(0.0f, 0.0f);
-                float top = -INFINITY, weight = 0.0f;
-                #pragma unroll
-                for (int w = 0; w < kWarps; ++w) {
-                    const float2 v = *reinterpret_cast<const float2*>(join + (w * S::kQueries + query) * kPitch + column);
-                    total.x += v.x; total.y += v.y;
-                    top = fmaxf(top, stat[(w * S::kQueries + query) * 2]);
-                }
-                #pragma unroll
-                for (int w = 0; w < kWarps; ++w) {
-                    const float2 v = *reinterpret_cast<const float2*>(stat + (w * S::kQueries + query) * 2);
-                    weight += v.y == 0.0f ? 0.0f : (v.x == -INFINITY ? 1.0f : fast_exp2(v.x - top)) * v.y;   // (scores that are all NaN leave a NaN sum)
-                }
-                const uint32_t global = first_query + query, all = chunk * S::kChunk + column;
-                if (!whole) {
-                    *reinterpret_cast<float2*>(a.partial + (mine * S::kQueries + query) * D + all) = total;
-                    if (all == 0) *reinterpret_cast<float2*>(a.sums + (mine * S::kQueries + query) * 2) = make_float2(top, weight);
-                } else if (global < queries) {
-                    const float inverse = weight > 0.0f ? 1.0f / weight : weight == 0.0f ? 0.0f : weight;
-                    const size_t to = size_t(sequence.first_row + global / a.group) * a.out_stride + size_t(kv * a.group + global % a.group) * D + all;
-                    const uint32_t packed = a.bf16 ? pack_bf16x2(total.x * inverse, total.y * inverse) : pack_half2(total.x * inverse, total.y * inverse);
-                    *reinterpret_cast<uint32_t*>(static_cast<uint16_t*>(a.out) + to) = packed;
-                }
-                if (whole && a.scores && all == 0) *reinterpret_cast<float2*>(a.stats + (size_t(at.unit) * S::kQueries + query) * 2) = make_float2(top, weight);
-            }
-            __syncthreads();
-        }
         if (piece_end == run_end) break;
         at.next(a);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
 }
 
-// Block = (unit, query): joins the partials of a unit that several blocks worked on, and zeroes the rows of a sequence without keys.
+// Block = (unit, query): joins the partials of a unit that several warps worked on, and zeroes the rows of a sequence without keys.
+constexpr int kJoinThreads = 512, kMostWarps = 2048;   // (warps of a launch: eight an SM)
 template<int D>
-__global__ void __launch_bounds__(D) kv8_decode_join_kernel(const __grid_constant__ AttentionArgs a, uint32_t queries_a_unit) {
+__global__ void __launch_bounds__(kJoinThreads) kv8_decode_join_kernel(const __grid_constant__ AttentionArgs a, uint32_t queries_a_unit) {
+    constexpr int kColumns = D / 4, kGroups = kJoinThreads / kColumns;   // threads a partial row, partials at a time
+    __shared__ float factors[kMostWarps];
+    __shared__ float tops[kJoinThreads / 32], weights[kJoinThreads / 32];
+    __shared__ float4 totals[kGroups][kColumns];
     const uint32_t unit = blockIdx.x, query = blockIdx.y;
     uint32_t s = 0;
     {
@@ -439,34 +461,87 @@ __global__ void __launch_bounds__(D) kv8_decode_join_kernel(const __grid_constan
     }
     const AttentionSequence& sequence = a.sequence[s];
     const uint32_t inside = unit - sequence.first_unit, kv = inside / sequence.parts, global = inside % sequence.parts * queries_a_unit + query;
-    const bool real = global < sequence.rows * a.group;
-    uint16_t* out = static_cast<uint16_t*>(a.out) + (real ? size_t(sequence.first_row + global / a.group) * a.out_stride + size_t(kv * a.group + global % a.group) * D : 0) + threadIdx.x;
     asm volatile("griddepcontrol.wait;" ::: "memory");   // (in every block: what is launched behind this one counts on the decode's end too)
+    if (global >= sequence.rows * a.group) return;
+    uint16_t* out = static_cast<uint16_t*>(a.out) + size_t(sequence.first_row + global / a.group) * a.out_stride + size_t(kv * a.group + global % a.group) * D;
     if (!sequence.tiles) {
-        if (real) *out = 0;
+        if (threadIdx.x < kColumns) *reinterpret_cast<uint2*>(out + 4 * threadIdx.x) = make_uint2(0, 0);
         return;
     }
     const uint64_t begin = sequence.first_tile + uint64_t(inside) * sequence.tiles, end = begin + sequence.tiles;
-    const uint32_t first = uint32_t(begin / a.tiles_a_block), last = uint32_t((end - 1) / a.tiles_a_block);
-    if (first == last) return;
+    const uint32_t first = uint32_t(begin / a.tiles_a_warp), pieces = uint32_t((end - 1) / a.tiles_a_warp) - first + 1;
+    if (pieces == 1) return;
     const float2* sums = reinterpret_cast<const float2*>(a.sums) + (size_t(first) + unit) * queries_a_unit + query;
-    const float* partial = a.partial + ((size_t(first) + unit) * queries_a_unit + query) * D + threadIdx.x;
-    const uint32_t pieces = last - first + 1;
-    float top = -INFINITY;
-    for (uint32_t p = 0; p < pieces; ++p) top = fmaxf(top, sums[size_t(p) * queries_a_unit].x);
-    float total = 0.0f, weight = 0.0f;
-    #pragma unroll 4
-    for (uint32_t p = 0; p < pieces; ++p) {
-        const float2 v = sums[size_t(p) * queries_a_unit];
-        const float factor = v.x == -INFINITY ? 0.0f : fast_exp2(v.x - top);
-        weight += v.y == 0.0f ? 0.0f : (v.x == -INFINITY ? 1.0f : factor) * v.y;
-        total = fmaf(factor, partial[size_t(p) * queries_a_unit * D], total);
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, column = threadIdx.x % kColumns, group = threadIdx.x / kColumns;
+    const float4* partial = reinterpret_cast<const float4*>(a.partial + ((size_t(first) + unit) * queries_a_unit + query) * D) + column;
+    // the first partials are asked for before the maximum is known
+    constexpr int kAhead = 4;
+    float4 v[kAhead];
+    #pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
+        const uint32_t p = group + i * kGroups;
+        v[i] = p < pieces ? partial[size_t(p) * queries_a_unit * kColumns] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
+    float2 mine[(kMostWarps + kJoinThreads - 1) / kJoinThreads];
+    float top = -INFINITY;
+    #pragma unroll
+    for (int i = 0; i < (kMostWarps + kJoinThreads - 1) / kJoinThreads; ++i) {
+        const uint32_t p = threadIdx.x + i * kJoinThreads;
+        mine[i] = p < pieces ? sums[size_t(p) * queries_a_unit] : make_float2(-INFINITY, 0.0f);
+        top = fmaxf(top, mine[i].x);
+    }
+    #pragma unroll
+    for (int offset = 16; offset; offset /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, offset));
+    if (lane == 0) tops[warp] = top;
+    __syncthreads();
+    top = tops[0];
+    #pragma unroll
+    for (int w = 1; w < kJoinThreads / 32; ++w) top = fmaxf(top, tops[w]);
+    float weight = 0.0f;
+    #pragma unroll
+    for (int i = 0; i < (kMostWarps + kJoinThreads - 1) / kJoinThreads; ++i) {
+        const uint32_t p = threadIdx.x + i * kJoinThreads;
+        // (nothing seen in a piece: no weight; scores that are all NaN leave a NaN sum, which stays)
+        const float factor = mine[i].y == 0.0f ? 0.0f : mine[i].x == -INFINITY ? 1.0f : fast_exp2(mine[i].x - top);
+        if (p < pieces) factors[p] = factor;
+        weight = fmaf(factor, mine[i].y, weight);
+    }
+    #pragma unroll
+    for (int offset = 16; offset; offset /= 2) weight += __shfl_xor_sync(0xffffffffu, weight, offset);
+    if (lane == 0) weights[warp] = weight;
+    __syncthreads();
+    weight = 0.0f;
+    #pragma unroll
+    for (int w = 0; w < kJoinThreads / 32; ++w) weight += weights[w];
+    float4 total = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    for (uint32_t from = group; from < pieces; from += kAhead * kGroups) {
+        float4 next[kAhead];
+        #pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const uint32_t p = from + (kAhead + i) * kGroups;
+            next[i] = p < pieces ? partial[size_t(p) * queries_a_unit * kColumns] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        }
+        #pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+            const uint32_t p = from + i * kGroups;
+            const float factor = p < pieces ? factors[p] : 0.0f;
+            total.x = fmaf(factor, v[i].x, total.x); total.y = fmaf(factor, v[i].y, total.y);
+            total.z = fmaf(factor, v[i].z, total.z); total.w = fmaf(factor, v[i].w, total.w);
+            v[i] = next[i];
+        }
+    }
+    totals[group][column] = total;
+    __syncthreads();
     if (a.scores && threadIdx.x == 0) *reinterpret_cast<float2*>(a.stats + (size_t(unit) * queries_a_unit + query) * 2) = make_float2(top, weight);
-    if (!real) return;
-    const float result = weight > 0.0f ? total / weight : weight == 0.0f ? 0.0f : weight;
-    if (a.bf16) *reinterpret_cast<__nv_bfloat16*>(out) = __float2bfloat16_rn(result);
-    else *reinterpret_cast<__half*>(out) = __float2half_rn(result);
+    if (threadIdx.x >= kColumns) return;
+    #pragma unroll
+    for (int i = 1; i < kGroups; ++i) {
+        const float4 other = totals[i][column];
+        total.x += other.x; total.y += other.y; total.z += other.z; total.w += other.w;
+    }
+    const float inverse = inverse_of(weight);
+    *reinterpret_cast<uint2*>(out + 4 * column) = a.bf16 ? make_uint2(pack_bf16x2(total.x * inverse, total.y * inverse), pack_bf16x2(total.z * inverse, total.w * inverse))
+                                                       : make_uint2(pack_half2(total.x * inverse, total.y * inverse), pack_half2(total.z * inverse, total.w * inverse));
 }
 
 // Thread = (K/V head, seen key): the key's weights over a K/V head's query rows, from the scores the attention left, added to the running sums.
@@ -483,13 +558,15 @@ __global__ void __launch_bounds__(256) kv8_weights_kernel(const __grid_constant_
     const uint32_t key = tile * TILE + at % TILE;
     if (key >= sequence.length) return;
     float total = 0.0f;
+    const uint32_t kept = sequence.score_queries;
     for (uint32_t part = 0; part < sequence.parts; ++part) {
         const uint32_t inside = kv * sequence.parts + part;
         const uint32_t queries = min(uint32_t(QUERIES), sequence.rows * a.group - part * QUERIES);
-        const float4* scores = reinterpret_cast<const float4*>(a.scores + (sequence.first_tile + uint64_t(inside) * sequence.tiles) * (TILE * QUERIES) + size_t(at) * QUERIES);
+        const float4* scores = reinterpret_cast<const float4*>(a.scores + sequence.first_score + (uint64_t(inside) * sequence.tiles * TILE + at) * kept);
         const float2* stats = reinterpret_cast<const float2*>(a.stats) + size_t(sequence.first_unit + inside) * QUERIES;
         #pragma unroll
         for (int i = 0; i < QUERIES / 4; ++i) {
+            if (uint32_t(4 * i) >= queries) break;
             const float4 v = scores[i];
             const float x[4] = {v.x, v.y, v.z, v.w};
             #pragma unroll
@@ -507,7 +584,7 @@ __global__ void __launch_bounds__(256) kv8_weights_kernel(const __grid_constant_
 template<int D, int NT, int CODE> static void launch_decode(Device& d, AttentionArgs& args, bool weights) {
     using S = Shape<D, NT>;
     args.units = 0; args.tiles = 0;
-    uint64_t most_keys = 0;
+    uint64_t most_keys = 0, score_floats = 0;
     bool empty = false;
     for (uint32_t s = 0; s < args.sequences; ++s) {
         AttentionSequence& q = args.sequence[s];
@@ -520,21 +597,25 @@ template<int D, int NT, int CODE> static void launch_decode(Device& d, Attention
         q.parts = (q.rows * args.group + S::kQueries - 1) / S::kQueries;
         q.first_unit = args.units;
         q.first_tile = args.tiles;
+        q.score_queries = std::min<uint32_t>(S::kQueries, (q.rows * args.group + 3) / 4 * 4);
+        q.first_score = score_floats;
+        score_floats += uint64_t(args.kv_heads) * q.parts * q.tiles * S::kTile * q.score_queries;
         args.units += args.kv_heads * q.parts;
         args.tiles += uint64_t(args.kv_heads) * q.parts * q.tiles;
         most_keys = std::max(most_keys, uint64_t(q.tiles) * S::kTile * args.kv_heads);
         empty |= !q.tiles;
     }
     // One block an SM; a warp takes a tile at least
-    const uint64_t blocks = std::max<uint64_t>(1, std::min<uint64_t>(d.sms, (args.tiles + kWarps - 1) / kWarps));
-    args.tiles_a_block = std::max<uint64_t>(1, (args.tiles + blocks - 1) / blocks);
-    const size_t slots = blocks + args.units;
-    bool cut = false;   // a unit that several blocks work on
+    const uint64_t warps = std::max<uint64_t>(1, std::min<uint64_t>(std::min<uint64_t>(uint64_t(d.sms) * kWarps, kMostWarps), args.tiles));
+    const uint64_t blocks = std::min<uint64_t>(uint64_t(d.sms), warps);
+    args.tiles_a_warp = std::max<uint64_t>(1, (args.tiles + warps - 1) / warps);
+    const size_t slots = blocks * kWarps + args.units;
+    bool cut = false;   // a unit that several warps work on
     for (uint32_t s = 0; s < args.sequences && !cut; ++s) {
         const AttentionSequence& q = args.sequence[s];
         for (uint32_t u = 0; u < args.kv_heads * q.parts && q.tiles && !cut; ++u) {
             const uint64_t begin = q.first_tile + uint64_t(u) * q.tiles;
-            cut = begin / args.tiles_a_block != (begin + q.tiles - 1) / args.tiles_a_block;
+            cut = begin / args.tiles_a_warp != (begin + q.tiles - 1) / args.tiles_a_warp;
         }
     }
     const size_t partial_floats = cut ? slots * S::kQueries * D : 0, sums_floats = cut ? slots * S::kQueries * 2 : 0;
@@ -543,8 +624,7 @@ template<int D, int NT, int CODE> static void launch_decode(Device& d, Attention
     args.sums = partial + partial_floats;
     args.scores = args.stats = nullptr;
     if (weights && args.tiles) {
-        const size_t score_floats = checked_product({args.tiles, uint64_t(S::kTile), uint64_t(S::kQueries)});
-        args.scores = static_cast<float*>(workspace(d, d.kv8_scores, (score_floats + size_t(args.units) * S::kQueries * 2) * 4));
+        args.scores = static_cast<float*>(workspace(d, d.kv8_scores, checked_product({score_floats + uint64_t(args.units) * S::kQueries * 2, 4})));
         args.stats = args.scores + score_floats;
     }
     static bool configured[64] = {};
@@ -564,7 +644,7 @@ template<int D, int NT, int CODE> static void launch_decode(Device& d, Attention
     if (cut || empty) {
         cudaLaunchConfig_t config{};
         config.gridDim = dim3(args.units, S::kQueries);
-        config.blockDim = dim3(D);
+        config.blockDim = dim3(kJoinThreads);
         config.stream = d.stream;
         config.attrs = &attribute;
         config.numAttrs = behind ? 1 : 0;

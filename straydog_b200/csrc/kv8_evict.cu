@@ -5,10 +5,11 @@
 // their order, to positions 0 .. keep - 1 of another state. A target block takes the largest scale among the blocks its rows come from,
 // and rows from a block with a smaller scale have their codes rounded again in it: the rule of an append to a begun block.
 //
-// kv8_evict_select_kernel: a cluster of 1 to 8 blocks a (sequence, head) finds the weight of the last place by sixteen steps of two bits each
-// (how many weights are at or above three candidate values), with the weights in registers: a step is a few compares a weight and one
-// exchange. Counting by compares costs no atomics, whatever the weights look like (a histogram's atomics meet in one bin when most weights are
-// equal, as the weights of never-attended rows are). Then ballots give every kept position its place in order.
+// kv8_evict_select_kernel: a cluster of 1 to 8 blocks a (sequence, head) finds the weight of the last place in three steps of 11, 11 and 10
+// bits, with the weights in registers: a histogram in shared memory of the weights that agree with the bits found so far, summed over the cluster,
+// and the bin where the places run out. A warp whose weights are all in one bin (weights of never-attended rows are all 0) adds them with one
+// atomic. (Sixteen steps of two bits by compares, without atomics, took 65 us for 16 sequences x 8 heads x 16384: eight issue slots a weight and
+// step.) Then ballots give every kept position its place in order.
 // kv8_evict_move_kernel: a block of 128 threads a (sequence, plane, target block of 32 rows): bound by memory, rows of `dim` bytes gathered.
 #include "kv8.cuh"
 #include "../../include/straydog_gpu_b200.h"
@@ -32,6 +33,7 @@ struct EvictArgs {
 };
 
 constexpr int kSelectThreads = 1024, kSelectWarps = 32, kHeld = 32, kMostCluster = 8;   // weights a thread holds; blocks a head
+constexpr int kBins = 2048, kCopies = 4;   // a histogram's bins; copies that a block's warps share out, so that they meet less
 
 // weights in an order of unsigned integers: NaN 0, then -inf .. +inf; the two zeros are equal
 __device__ __forceinline__ uint32_t order_of(float w) {
@@ -44,10 +46,9 @@ template<bool HELD>
 __global__ void __launch_bounds__(kSelectThreads, 1) kv8_evict_select_kernel(const __grid_constant__ EvictArgs a, uint32_t ctas) {
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
-    __shared__ uint32_t warp_counts[kSelectWarps][3];
-    __shared__ uint32_t shares[2][kMostCluster][3];   // every block's counts, written by that block into each block's copy; by parity of the step
+    __shared__ uint32_t histogram[kCopies][kBins];
+    __shared__ uint32_t warp_counts[kSelectWarps][2], block_counts[2], found[2];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    if (ctas > 1) cluster.sync();   // (no block stores into another's shared memory before that one runs)
     const uint32_t unit = blockIdx.x / ctas, rank = blockIdx.x % ctas, s = unit / a.kv_heads, head = unit % a.kv_heads;
     const EvictSequence& sequence = a.sequence[s];
     const uint32_t length = sequence.length, lane = threadIdx.x % 32, warp = threadIdx.x / 32;
@@ -72,69 +73,94 @@ __global__ void __launch_bounds__(kSelectThreads, 1) kv8_evict_select_kernel(con
         #pragma unroll
         for (int j = 0; j < kHeld; ++j) key[j] = uint32_t(j) < each ? load(j) : 0u;
     }
-    auto count_at = [&](const uint32_t (&bound)[3], uint32_t (&counts)[3]) {
-        counts[0] = counts[1] = counts[2] = 0;
-        auto add = [&](uint32_t k) {
-            #pragma unroll
-            for (int c = 0; c < 3; ++c) counts[c] += k >= bound[c];
-        };
+    auto each_key = [&](auto&& act) {
         if (HELD) {
             #pragma unroll
-            for (int j = 0; j < kHeld; ++j) if (uint32_t(j) < each) add(key[j]);
+            for (int j = 0; j < kHeld; ++j) {
+                if (uint32_t(j) >= each) break;
+                act(uint32_t(j), key[j]);
+            }
         } else {
-            for (uint32_t j = 0; j < each; ++j) add(load(j));
+            for (uint32_t j = 0; j < each; ++j) act(j, load(j));
         }
     };
-    int step = 0;
-    // sums of three counts over the head's weights; every block of the cluster gets them, and its own blocks' shares stay in shares[]
-    auto sum = [&](uint32_t (&counts)[3], uint32_t (&total)[3], uint32_t (&before)[3]) {
-        #pragma unroll
-        for (int c = 0; c < 3; ++c) counts[c] = __reduce_add_sync(0xffffffffu, counts[c]);
-        if (lane == 0) { warp_counts[warp][0] = counts[0]; warp_counts[warp][1] = counts[1]; warp_counts[warp][2] = counts[2]; }
+    uint32_t last = 0, missing = want;   // the key of the last place, its bits from the top; places left among the keys that agree with them
+    #pragma unroll 1
+    for (int step = 0; want && step < 3; ++step) {
+        const int shift = step == 0 ? 21 : step == 1 ? 10 : 0, bits = step == 2 ? 10 : 11;
+        for (int i = threadIdx.x; i < kCopies * kBins; i += kSelectThreads) (&histogram[0][0])[i] = 0;
         __syncthreads();
-        const int parity = step++ & 1;
-        if (warp == 0) {
+        uint32_t* mine_counts = histogram[warp % kCopies];
+        each_key([&](uint32_t j, uint32_t k) {
+            const bool counts = first + j * 32 + lane < between && (step == 0 || (k >> (shift + bits)) == (last >> (shift + bits)));
+            const uint32_t bin = counts ? (k >> shift) & ((1u << bits) - 1u) : 0xffffffffu;
+            const uint32_t live = __ballot_sync(0xffffffffu, counts);
+            if (!live) return;
+            const uint32_t leader = uint32_t(__ffs(int(live)) - 1), common = __shfl_sync(0xffffffffu, bin, int(leader));
+            const uint32_t same = __ballot_sync(0xffffffffu, bin == common);
+            if (lane == leader) atomicAdd(&mine_counts[common], uint32_t(__popc(same)));
+            if (counts && bin != common) atomicAdd(&mine_counts[bin], 1u);
+        });
+        __syncthreads();
+        for (int i = threadIdx.x; i < kBins; i += kSelectThreads) {
+            uint32_t sum = 0;
             #pragma unroll
-            for (int c = 0; c < 3; ++c) {
-                const uint32_t block_total = __reduce_add_sync(0xffffffffu, warp_counts[lane][c]);
-                if (lane < ctas) cluster.map_shared_rank(&shares[0][0][0], lane)[(parity * kMostCluster + rank) * 3 + c] = block_total;
-            }
+            for (int c = 0; c < kCopies; ++c) sum += histogram[c][i];
+            histogram[0][i] = sum;
         }
         if (ctas > 1) cluster.sync(); else __syncthreads();
+        // thread t: the bins 2047 - 2t and 2046 - 2t (from the greatest down), over the cluster
+        uint32_t high = 0, low = 0;
+        for (uint32_t r = 0; r < ctas; ++r) {
+            const uint32_t* counts = ctas > 1 ? cluster.map_shared_rank(&histogram[0][0], r) : &histogram[0][0];
+            high += counts[kBins - 1 - 2 * threadIdx.x]; low += counts[kBins - 2 - 2 * threadIdx.x];
+        }
+        uint32_t above = high + low;   // inclusive sums over the threads
         #pragma unroll
-        for (int c = 0; c < 3; ++c) {
-            total[c] = before[c] = 0;
-            for (uint32_t r = 0; r < ctas; ++r) { const uint32_t v = shares[parity][r][c]; total[c] += v; if (r < rank) before[c] += v; }
+        for (int offset = 1; offset < 32; offset *= 2) { const uint32_t other = __shfl_up_sync(0xffffffffu, above, offset); if (lane >= uint32_t(offset)) above += other; }
+        if (lane == 31) warp_counts[warp][0] = above;
+        __syncthreads();
+        for (uint32_t w = 0; w < warp; ++w) above += warp_counts[w][0];
+        const uint32_t before_high = above - high - low, before_low = above - low;
+        if (before_high < missing && missing <= above) {   // one thread: the places run out in one of its bins
+            const bool in_high = missing <= before_low;
+            found[0] = in_high ? kBins - 1 - 2 * threadIdx.x : kBins - 2 - 2 * threadIdx.x;
+            found[1] = missing - (in_high ? before_high : before_low);
         }
-    };
-    uint32_t last = 0xffffffffu;   // the key of the last place: the greatest value that `want` keys or more reach
-    uint32_t counts[3], total[3], before[3];
-    if (want) {
-        last = 0;
-        #pragma unroll 1
-        for (int shift = 30; shift >= 0; shift -= 2) {
-            const uint32_t bound[3] = {last | 1u << shift, last | 2u << shift, last | 3u << shift};
-            count_at(bound, counts);
-            sum(counts, total, before);
-            last = total[2] >= want ? bound[2] : total[1] >= want ? bound[1] : total[0] >= want ? bound[0] : last;
-        }
+        if (ctas > 1) cluster.sync(); else __syncthreads();   // (also: every block has read the others' counts before they are zeroed)
+        last |= found[0] << shift;
+        missing = found[1];
     }
-    // places: keys above `last` all stay, of those equal to it the first want - above
+    // places: keys above `last` all stay, of those equal to it the first `missing` in order
     {
-        const uint32_t bound[3] = {last, last == 0xffffffffu ? last : last + 1, 0xffffffffu};   // (no key is 2^32 - 1)
-        count_at(bound, counts);
-        // weights past the end count as key 0, behind every weight: they only matter when `last` is 0, and then lie behind the places wanted
-        sum(counts, total, before);
-        uint32_t reach = before[0], above = before[1];
+        uint32_t reach = 0, above = 0;
+        if (want) each_key([&](uint32_t j, uint32_t k) {
+            const bool real = first + j * 32 + lane < between;
+            reach += real && k >= last; above += real && k > last;
+        });
+        reach = __reduce_add_sync(0xffffffffu, reach);
+        above = __reduce_add_sync(0xffffffffu, above);
+        if (lane == 0) { warp_counts[warp][0] = reach; warp_counts[warp][1] = above; }
+        __syncthreads();
+        if (warp == 0) {
+            const uint32_t all_reach = __reduce_add_sync(0xffffffffu, warp_counts[lane][0]), all_above = __reduce_add_sync(0xffffffffu, warp_counts[lane][1]);
+            if (lane == 0) { block_counts[0] = all_reach; block_counts[1] = all_above; }
+        }
+        if (ctas > 1) cluster.sync();
+        reach = above = 0;
+        for (uint32_t r = 0; r < rank; ++r) {
+            const uint32_t* counts = cluster.map_shared_rank(&block_counts[0], r);
+            reach += counts[0]; above += counts[1];
+        }
         for (uint32_t w = 0; w < warp; ++w) { reach += warp_counts[w][0]; above += warp_counts[w][1]; }
-        const uint32_t ties = want - min(want, total[1]);
+        const uint32_t ties = want ? missing : 0;
         uint32_t equal = reach - above;
         uint32_t place = sinks + above + min(equal, ties);
         const uint32_t below = (1u << lane) - 1u;
-        auto put = [&](uint32_t j, uint32_t k) {
-            const bool greater = want && k > last, tie = want && k == last;
+        if (want) each_key([&](uint32_t j, uint32_t k) {
+            const bool real = first + j * 32 + lane < between, tie = real && k == last;
             const uint32_t ties_here = __ballot_sync(0xffffffffu, tie);
-            const bool stays = greater || (tie && equal + __popc(ties_here & below) < ties);
+            const bool stays = (real && k > last) || (tie && equal + __popc(ties_here & below) < ties);
             const uint32_t staying = __ballot_sync(0xffffffffu, stays);
             if (stays) {
                 const uint32_t i = first + j * 32 + lane, at = place + __popc(staying & below);
@@ -143,15 +169,9 @@ __global__ void __launch_bounds__(kSelectThreads, 1) kv8_evict_select_kernel(con
             }
             equal += __popc(ties_here);
             place += __popc(staying);
-        };
-        if (HELD) {
-            #pragma unroll
-            for (int j = 0; j < kHeld; ++j) if (uint32_t(j) < each) put(j, key[j]);
-        } else {
-            for (uint32_t j = 0; j < each; ++j) put(j, load(j));
-        }
+        });
     }
-    if (ctas > 1) cluster.sync();   // (no block leaves while another may still store into its shares)
+    if (ctas > 1) cluster.sync();   // (no block leaves while another may still read its counts)
 }
 
 template<int D, int CODE>

@@ -4,13 +4,18 @@
 // Row i of a sequence with n keys and r rows sits at p = n - r + i and sees key j < n when j <= p and j > p - window, or when j < prefix.
 //   s = scale * q . k;  s = cap * tanh(s / cap);  s -= slope[head] * |p - j|;  out = softmax over the seen keys . v, zeros where none is seen
 //
-// A block owns 256 M-rows as two tiles of 128 (one tile for 256 columns): 128 / group consecutive rows times the `group` query heads of one K/V
-// head, so K and V are fetched once for all of them and the diagonal is thin. It walks the union of its rows' keys in tiles of 128:
+// A unit is 256 M-rows of one K/V head as two tiles of 128 (one tile for 256 columns): 128 / group consecutive rows times the `group` query heads, so
+// K and V are fetched once for all of them and the diagonal is thin. Its work is the union of its rows' keys in tiles of 128:
 //   S[128 x 128] = Q . K^T    D / 16 tcgen05.mma, Q and K in shared memory (TMA, 128-byte swizzle), FP32 in TMEM
 //   O[128 x D]  += P . V      8 tcgen05.mma, P in TMEM over the columns of its S, V in shared memory
-// Two tiles a block: while one tile's softmax runs, the tensor pipe works on the other's products. With 256 columns TMEM holds one O and two S,
-// and the softmax of one key tile runs beside the products of the next.
-// Warps: 0-3 and 4-7 softmax, a thread a row; 8 issues the products; 9 the TMA loads; 10-11 look after values that no row may see (below).
+// Two tiles a unit: while one tile's softmax runs, the tensor pipe works on the other's products. With 256 columns TMEM holds one O and two S,
+// the softmax of one key tile runs beside the products of the next.
+// Persistent blocks, one an SM: the units' tiles laid end to end are cut into equal runs (a unit counts two tiles more, for its first products, its masked
+// tiles and its output). A block walks its run without stopping: the next unit's first products are issued while the last one's output is written. A unit that
+// two or more blocks share leaves FP32 partials for a second kernel. (A block a unit left the last of 1.7 waves a third empty for a chunk of 2048
+// rows, 285 us, and spent half of 184 us on first loads and outputs for packed documents of 8 tiles a unit.)
+// Warps: 0-3 and 4-7 softmax, a thread a row (half a row with 256 columns); 8 issues the products; 9 the TMA loads; 10-11 look after values that
+// some row may not see (below).
 //
 // Roundings: scores, maxima, sums and O are FP32. P is rounded to the operands' type once (FP16 or BF16), at 2^7 times its size so that FP16 keeps
 // 11 bits down to 2^-21 of the largest weight. O is multiplied in TMEM only when a row's maximum grew by more than 2^8. The keys' scales of an 8-bit
@@ -23,51 +28,60 @@
 #include "../../include/straydog_gpu_b200.h"
 
 #include <cuda.h>
-#include <mutex>
+#include <type_traits>
 
 namespace sdb {
 namespace attn {
 
 constexpr int kThreads = 384, kTileKeys = 128, kM = 128;
+constexpr int kIssueWarp = 8, kLoadWarp = 9, kLookWarp = 10;
 constexpr float kLift = 7.0f, kRescale = 8.0f;
 constexpr unsigned kSequences = 64;   // sequences a launch
-constexpr int kFlagged = 32;          // tiles of one block with masked values that are not finite (borders: at most a dozen)
+constexpr int kFlagged = 16;          // slots of one piece that are looked at for values that are not finite (borders: at most a dozen)
 
 template<int D> struct Shape {
-    static constexpr int kTiles = D == 256 ? 1 : 2;                  // query tiles a block
+    static constexpr int kTiles = D == 256 ? 1 : 2;                  // query tiles a unit
     static constexpr int kSlotKeys = D == 256 ? 64 : 128;            // keys of a ring slot: 32 KB (16 KB for 64 columns)
     static constexpr int kHalves = kTileKeys / kSlotKeys;            // slots of a key tile
     static constexpr int kSlots = D == 256 ? 5 : 4;
     static constexpr int kSlotBytes = kSlotKeys * D * 2, kQueryBytes = kM * D * 2;
     static constexpr int kOffRing = kTiles * kQueryBytes, kOffBars = kOffRing + kSlots * kSlotBytes;
-    static constexpr int kOffFlags = kOffBars + 512;
-    static constexpr size_t kSmem = kOffFlags + kFlagged * 32 + 1024;   // + slack to align the base to 1024 bytes
+    static constexpr int kOffFlags = kOffBars + 256, kOffStats = kOffFlags + kFlagged * 32;
+    static constexpr int kSlack = kTiles == 1 ? 0 : 1024;             // to align the base to 1024 bytes where there is room (the runtime aligns it anyway)
+    static constexpr size_t kSmem = kOffStats + (kTiles == 1 ? 2 * 2 * kM * 4 : 0) + kSlack;
+    static_assert(kSmem <= 227 * 1024, "shared memory");
     static constexpr int kS = 0, kO = 256;                           // TMEM columns: S of tile (or buffer) b at 128 b, O of tile b at 256 + D b
 };
 
 struct KernelSequence {
-    uint32_t rows, length, prefix, first_row, first_key, first_unit, blocks, first_block;   // first_block: of the unpacked blocks of 32 keys
+    uint32_t rows, length, prefix, first_row, first_key, first_unit, blocks, first_block;   // blocks of rows; first_block: of the unpacked blocks of 32 keys
 };
+constexpr unsigned kMostBlocks = 160;   // blocks of a launch (one an SM)
+struct Cut { uint32_t unit, tile; };                   // where a block's run begins
+struct Shared { uint32_t unit, first, pieces; };       // a unit that blocks first .. first + pieces - 1 share
 struct Args {
     CUtensorMap q_map, k_map, v_map;
     KernelSequence sequence[kSequences];
     uint32_t sequences, heads, kv_heads, group, tokens;   // tokens: rows of a query tile
-    uint32_t splits, window;
+    uint32_t window, shares, zero;   // zero: 0, unknown to the compiler
+    Cut cut[kMostBlocks + 1];
+    Shared share[kMostBlocks];
     void* out;
     size_t out_stride;
+    int wide_out;                // output rows on 32-byte boundaries
     const float* slopes;
-    const float4* block_table;   // 8-bit states: [kv_heads][blocks of 32 keys] key scale, log2 and inverse of the value scale over the head's largest
+    const float* block_table;    // 8-bit states: [kv_heads][tiles of four blocks of 32 keys][12]: four key scales, then log2 and inverse of four value scales over the head's largest
     const float* value_top;      // 8-bit states: [sequence][kv_heads] the largest value scale
     uint32_t table_blocks;
     const uint16_t* values;      // 16-bit rows: the values again, for the rows that see one that is not finite
     size_t value_stride;
     float scale_log2, cap, scale_over_cap;
-    float* partial;              // [unit][split][M-rows][D], then [unit][split][M-rows][2]
-    float* sums;
+    float* partial;              // [2 * block + (the unit goes on in the next block)][M-rows][D]: a block shares its first and its last unit at most
+    float* sums;                 // the same [M-rows][2]
     int* status;
 };
 
-enum { kQFull = 0, kSFull = 1, kPFull = 3, kPvDone = 5, kLook = 7, kClean = 8, kRing = 9 };   // barriers: then full and free of every slot
+enum { kQFull = 0, kSFull = 1, kPFull = 3, kPvDone = 5, kLook = 7, kClean = 8, kQFree = 9, kOFree = 10, kRing = 12 };   // barriers: then full and free of every slot
 
 constexpr uint32_t kDescHigh = 0x40004040u;   // 128-byte swizzle, 1024 bytes between groups of 8 rows (see csrc/qsa_prompt_tc.cu)
 __device__ __forceinline__ uint32_t desc_low(uint32_t address, uint32_t leading_bytes) { return ((address & 0x3ffffu) >> 4) | ((leading_bytes >> 4) << 16); }
@@ -119,78 +133,124 @@ __device__ __forceinline__ void tmem_store16(uint32_t address, const uint32_t* r
 }
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+__device__ __forceinline__ void store32(void* to, const uint32_t* w) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), SDB_I8(w, 0) : "memory");
+}
 // A tile of a packed array: x (columns) on a 16-byte boundary always (a multiple of 64 elements); rows past the array read as zeros.
 __device__ __forceinline__ void tma_load(void* to, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
                  ::"r"(smem_u32(to)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar)) : "memory");
 }
 
-__device__ __forceinline__ float fast_rcp(float x) {
-    float y;
-    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
+// the low `count` bits set (none below 0, all from 32 on)
+__device__ __forceinline__ uint32_t first_bits(int count) { return count <= 0 ? 0u : count >= 32 ? 0xffffffffu : (1u << count) - 1u; }
+__device__ __forceinline__ float max3(float a, float b, float c) {   // (as fmaxf: a NaN is no maximum)
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
-
-// The walk of a block (and split) over its key tiles, the same for every role.
-struct Walk {
-    uint32_t s, unit, kv, block, split;
-    int first, last;                     // positions of the block's first and last row
-    uint32_t head_tiles, jump, begin, end;
-    template<int TILES> __device__ __forceinline__ void find(const Args& a) {
-        unit = blockIdx.x / a.splits;
-        split = blockIdx.x % a.splits;
+// A unit: its rows and the key tiles that any of them sees, the same for every role (and on the host, which cuts the runs).
+struct Unit {
+    uint32_t s, kv, row;                 // sequence, K/V head, first row
+    int first, last, length, prefix;     // positions of the first and the last row; the sequence's
+    uint32_t head_tiles, jump, tiles;    // tiles from head_tiles on are `jump` tiles further on
+    __host__ __device__ __forceinline__ void find(const Args& a, uint32_t unit, uint32_t rows_a_unit) {
         s = 0;
         uint32_t high = a.sequences;
         while (high - s > 1) { const uint32_t mid = (s + high) / 2; if (a.sequence[mid].first_unit <= unit) s = mid; else high = mid; }
-        const KernelSequence& q = a.sequence[s];
-        const uint32_t inside = unit - q.first_unit;
+        const uint32_t inside = unit - a.sequence[s].first_unit;
         kv = inside % a.kv_heads;
-        block = q.blocks - 1 - inside / a.kv_heads;   // the longest first
-        const uint32_t row = block * TILES * a.tokens;
-        first = int(q.length) - int(q.rows) + int(row);
-        last = int(q.length) - int(q.rows) + int(min(q.rows, row + TILES * a.tokens)) - 1;
-        const uint32_t reach = max(uint32_t(max(last + 1, 0)), q.prefix), low = a.window ? uint32_t(max(0, first - int(a.window) + 1)) : 0u;
-        const uint32_t all = (reach + kTileKeys - 1) / kTileKeys;
-        head_tiles = (q.prefix + kTileKeys - 1) / kTileKeys;
-        const uint32_t body = min(all, max(head_tiles, low / kTileKeys));
+        row = inside / a.kv_heads * rows_a_unit;
+        fill(a, rows_a_unit);
+    }
+    __device__ __forceinline__ void next(const Args& a, uint32_t rows_a_unit) {
+        if (++kv < a.kv_heads) return;   // (the same rows: the same tiles)
+        kv = 0;
+        row += rows_a_unit;
+        if (row >= a.sequence[s].rows) { ++s; row = 0; }
+        fill(a, rows_a_unit);
+    }
+    __host__ __device__ __forceinline__ void fill(const Args& a, uint32_t rows_a_unit) {
+        const KernelSequence& q = a.sequence[s];
+        length = int(q.length); prefix = int(q.prefix);
+        const uint32_t end = q.rows < row + rows_a_unit ? q.rows : row + rows_a_unit;
+        first = length - int(q.rows) + int(row);
+        last = length - int(q.rows) + int(end) - 1;
+        const int causal = last + 1, reach = causal > prefix ? causal : prefix;
+        const uint32_t low = a.window && first >= int(a.window) ? uint32_t(first - int(a.window) + 1) : 0u;
+        const uint32_t all = uint32_t((reach > 0 ? reach : 0) + kTileKeys - 1) / kTileKeys;
+        head_tiles = uint32_t(prefix + kTileKeys - 1) / kTileKeys;
+        uint32_t body = low / kTileKeys > head_tiles ? low / kTileKeys : head_tiles;
+        if (body > all) body = all;
         jump = body - head_tiles;
-        const uint32_t total = all - jump;
-        begin = uint32_t(uint64_t(split) * total / a.splits);
-        end = uint32_t(uint64_t(split + 1) * total / a.splits);
+        tiles = all - jump;
     }
     __device__ __forceinline__ uint32_t key(uint32_t tile) const { return (tile < head_tiles ? tile : tile + jump) * kTileKeys; }
-    // whether every row of the block sees every key of the tile at key0
+    // whether every row of the unit sees every key of the tile at key0
     __device__ __forceinline__ bool open(const Args& a, uint32_t key0) const {
-        const KernelSequence& q = a.sequence[s];
         const int end_key = int(key0) + kTileKeys - 1;
-        return (end_key <= first && end_key < int(q.length) && (!a.window || int(key0) > last - int(a.window))) || end_key < int(q.prefix);
+        return (end_key <= first && end_key < length && (!a.window || int(key0) > last - int(a.window))) || end_key < prefix;
     }
 };
 
-template<int D, bool BF16>
+// A block's run, piece by piece: a piece is the part of a unit's tiles that lies in the run.
+template<int ROWS> struct Run {
+    uint32_t unit, begin, end;   // the piece's tiles
+    Cut to;
+    bool whole;
+    Unit u;
+    __device__ __forceinline__ bool start(const Args& a) {
+        const Cut from = a.cut[blockIdx.x];
+        to = a.cut[blockIdx.x + 1];
+        unit = from.unit;
+        if (done()) return false;
+        u.find(a, unit, ROWS * a.tokens);
+        set(from.tile);
+        return true;
+    }
+    __device__ __forceinline__ bool next(const Args& a) {
+        ++unit;
+        if (done()) return false;
+        u.next(a, ROWS * a.tokens);
+        set(0);
+        return true;
+    }
+    __device__ __forceinline__ bool done() const { return unit > to.unit || (unit == to.unit && !to.tile); }
+    __device__ __forceinline__ void set(uint32_t from) {
+        begin = from;
+        end = unit == to.unit ? to.tile : u.tiles;
+        whole = !begin && end == u.tiles;
+    }
+};
+
+template<int D, bool BF16, bool RULE>
 __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __grid_constant__ Args a) {
     using S = Shape<D>;
-    constexpr int T = S::kTiles;
-    extern __shared__ uint8_t smem_raw[];
+    constexpr int T = S::kTiles, kGroups = T == 2 ? 4 : 2;   // a softmax thread's groups of 32 columns of S
+    extern __shared__ __align__(1024) uint8_t smem_raw[];
+    if (!S::kSlack && smem_u32(smem_raw) % 1024) {   // (no operand layout without it: reported, not computed)
+        if (threadIdx.x == 0) atomicExch(a.status, 1);
+        return;
+    }
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kOffBars);
     constexpr int kFull = kRing, kFree = kRing + S::kSlots, kBars = kRing + 2 * S::kSlots;
-    static_assert(kBars * 8 + 16 <= 512, "barriers");
+    static_assert(kBars * 8 + 16 <= 256, "barriers");
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBars);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-    uint32_t* flagged_count = tmem_slot + 2;
-    uint32_t* flagged = reinterpret_cast<uint32_t*>(smem + S::kOffFlags);   // [entry]: key of the slot, then 4 words of keys
+    volatile uint32_t* flagged_piece = tmem_slot + 2;                       // the piece (counted from 1) that `flagged` belongs to
+    uint32_t* flagged = reinterpret_cast<uint32_t*>(smem + S::kOffFlags);   // [slot looked at]: its first key, then four words of keys
 
     const int tid = threadIdx.x, warp = tid / 32, lane = tid % 32;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (tid == 0) {
-        for (int i = 0; i < kBars; ++i) mbar_init(&bars[i], i == kPFull || i == kPFull + 1 ? 4 : i == kClean ? 2 : 1);
+        for (int i = 0; i < kBars; ++i)
+            mbar_init(&bars[i], i == kPFull || i == kPFull + 1 || i == kOFree || i == kOFree + 1 ? (T == 2 ? 4 : 8) : i == kClean ? 2 : 1);
         *abort_flag = 0;
-        *flagged_count = 0;
+        *flagged_piece = 0;
     }
-    for (int i = tid; i < kFlagged * 8; i += kThreads) flagged[i] = 0;
     fence_barrier_init();
-    if (warp == 8) {
+    if (warp == kIssueWarp) {
         asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(tmem_slot)), "r"(512u) : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
@@ -198,11 +258,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
     __syncthreads();
     fence_after();
     const uint32_t tmem = *tmem_slot;
-    Walk walk;
-    walk.find<T>(a);
-    const KernelSequence& sequence = a.sequence[walk.s];
-    const uint32_t tiles = walk.end - walk.begin;
-    asm volatile("griddepcontrol.wait;" ::: "memory");   // (unpacked rows are the kernel's before)
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // (everything read from here on may be the kernel's before)
 
     auto wait = [&](int bar, uint32_t parity) -> bool {   // bounded, and ended by another role's giving up
         if (mbar_try_wait(&bars[bar], parity)) return true;
@@ -215,186 +271,283 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
             if (global_timer_ns() - start > 2000000000ull) { *abort_flag = 1; atomicExch(a.status, 1); return false; }
         }
     };
+    Run<T> run;
+    bool alive = true;
+    uint32_t done = 0;    // key tiles of the pieces before (each role counts for itself: the barriers' parities follow it)
+    uint32_t piece = 0;   // pieces with tiles before
 
     if (warp < 8) {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");
-        const int tile_of = T == 2 ? warp / 4 : 0;
-        if (warp < 4 * T) {
-            // ================= softmax: a thread a row =================
-            const int m = (warp & 3) * 32 + lane;
-            const uint32_t token = (walk.block * T + tile_of) * a.tokens + m / a.group, head = walk.kv * a.group + m % a.group;
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");   // (8 warps x 208 and 4 x 88: what 12 are launched with at 168)
+        // ================= softmax: a thread a row (T 2: a warpgroup a query tile), or half a row (T 1: a warpgroup a half of the columns) =================
+        const int tile_of = T == 2 ? warp / 4 : 0, half = T == 2 ? 0 : warp / 4, m = (warp & 3) * 32 + lane;
+        const uint32_t lane_base = tmem + (uint32_t((warp & 3) * 32) << 16);
+        constexpr int kOColumns = T == 2 ? D : D / 2;                          // a thread's columns of O
+        const uint32_t o_base = lane_base + S::kO + tile_of * D + half * kOColumns;
+        float* stats = reinterpret_cast<float*>(smem + S::kOffStats) + m;      // T 1: [turn's parity][half][row], what the two threads of a row tell each other
+        auto other_half = [&](float mine, uint32_t turn) -> float {
+            if (T == 2) return mine;
+            stats[((turn & 1) * 2 + half) * kM] = mine;
+            asm volatile("bar.sync %0, 64;" ::"r"(1 + (warp & 3)) : "memory");
+            return stats[((turn & 1) * 2 + (half ^ 1)) * kM];
+        };
+        auto any_of_rows = [&](bool mine) -> bool {   // of the warp's rows (T 1: of the two warps that share them)
+            if (T == 2) return __any_sync(0xffffffffu, mine);
+            uint32_t any;
+            asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbar.red.or.pred q, %2, 64, p;\n\tselp.u32 %0, 1, 0, q;\n\t}"
+                         : "=r"(any) : "r"(uint32_t(mine)), "r"(1 + (warp & 3)) : "memory");
+            return any != 0;
+        };
+        uint32_t turn = 0;
+        for (bool more = run.start(a); more && alive; more = run.next(a)) {
+            const Unit& u = run.u;
+            const KernelSequence& sequence = a.sequence[u.s];
+            const uint32_t tiles = run.end - run.begin;
+            const uint32_t token = u.row + tile_of * a.tokens + m / a.group, head = u.kv * a.group + m % a.group;
             const bool valid = token < sequence.rows && uint32_t(m) < a.tokens * a.group;
-            const int position = int(sequence.length) - int(sequence.rows) + int(token);
-            const uint32_t lane_base = tmem + (uint32_t((warp & 3) * 32) << 16);
-            const uint32_t o_base = lane_base + S::kO + tile_of * D;
-            const float slope = a.slopes && valid ? a.slopes[head] * 1.4426950408889634f : 0.0f;
+            const int position = u.length - int(sequence.rows) + int(token);
+            const float slope = RULE && a.slopes && valid ? a.slopes[head] * 1.4426950408889634f : 0.0f;
+            // 8-bit states: a tile's factors are 12 floats, [scores' | weights' log2 | sums'] x [four groups of 32 keys]; a thread has kGroups of each
+            const float* table_at = a.block_table ? a.block_table + (size_t(u.kv) * a.table_blocks + sequence.first_block) * 3 + half * 2 : nullptr;
             float top_run = -INFINITY, sum_run = 0.0f;
-            bool alive = true;
             #pragma unroll 1
-            for (uint32_t i = 0; i < tiles && alive; ++i) {
-                const uint32_t key0 = walk.key(walk.begin + i);
-                const int buffer = T == 2 ? tile_of : int(i & 1);
-                float4 table[4];
-                if (a.block_table) {
+            for (uint32_t i = 0; i < tiles; ++i) {
+                const uint32_t key0 = u.key(run.begin + i), it = done + i;
+                const int buffer = T == 2 ? tile_of : int(it & 1);
+                float to_score[kGroups], shift[kGroups], to_sum[kGroups];
+                #pragma unroll
+                for (int g = 0; g < kGroups; ++g) { to_score[g] = 1.0f; shift[g] = 0.0f; to_sum[g] = 1.0f; }
+                if (table_at) {
+                    const float* table = table_at + key0 / 32 * 3;
                     #pragma unroll
-                    for (int g = 0; g < 4; ++g) table[g] = __ldg(a.block_table + size_t(walk.kv) * a.table_blocks + sequence.first_block + key0 / 32 + g);
+                    for (int g = 0; g < kGroups; g += 2) {
+                        const float2 x = __ldg(reinterpret_cast<const float2*>(table + g)), y = __ldg(reinterpret_cast<const float2*>(table + 4 + g)),
+                                     z = __ldg(reinterpret_cast<const float2*>(table + 8 + g));
+                        to_score[g] = x.x; to_score[g + 1] = x.y; shift[g] = y.x; shift[g + 1] = y.y; to_sum[g] = z.x; to_sum[g + 1] = z.y;
+                    }
                 }
-                if (!wait(kSFull + buffer, T == 2 ? i & 1 : (i >> 1) & 1)) { alive = false; break; }
+                if (!wait(kSFull + buffer, T == 2 ? it & 1 : (it >> 1) & 1)) { alive = false; break; }
                 fence_after();
-                const uint32_t s_base = lane_base + S::kS + buffer * 128;
-                uint32_t bits[128];
-                #pragma unroll
-                for (int g = 0; g < 4; ++g) tmem_load32(s_base + 32 * g, bits + 32 * g);
-                #pragma unroll
-                for (int g = 0; g < 4; ++g) tmem_load_wait(bits + 32 * g);
-                float s[128];
-                #pragma unroll
-                for (int n = 0; n < 128; ++n) s[n] = __uint_as_float(bits[n]);
-                float c[4];
-                #pragma unroll
-                for (int g = 0; g < 4; ++g) c[g] = a.scale_log2 * (a.block_table ? table[g].x : 1.0f);
-                if (a.cap > 0.0f) {   // cap * tanh(s / cap), tanh(y) = 1 - 2 / (1 + e^(2 y)): off by 2^-23 of the cap at most
+                const uint32_t s_base = lane_base + S::kS + buffer * 128 + half * 64;
+                const bool open = u.open(a, key0);
+                // Weights are computed from the maximum so far, in one pass over the scores that finds the tile's own on the way. Where that is above by
+                // more than 2^8, where there is none yet, and in tiles with a mask, a cap or a bias, the scores are finished and the maximum found
+                // first, O is multiplied, and the pass runs over what went back to TMEM.
+                bool first = i == 0 || !open || RULE;
+                if (!first) {
+                    const float under = top_run == -INFINITY ? 0.0f : top_run - kLift;
+                    uint32_t packed[16 * kGroups];
+                    float top = -INFINITY, sum = 0.0f;
                     #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const float inner = a.scale_over_cap * 2.8853900817779268f * (a.block_table ? table[g].x : 1.0f);
+                    for (int g = 0; g < kGroups; ++g) {
+                        uint32_t bits[32];
+                        // (the address waits for the weights before: loads moved further up would take the registers of all groups at once)
+                        tmem_load32(s_base + 32 * g + (g ? packed[16 * g - 1] & a.zero : 0u), bits);
+                        const float c = a.scale_log2 * to_score[g], d = shift[g] - under;
+                        tmem_load_wait(bits);
+                        float sum0 = 0.0f, sum1 = 0.0f, most = -INFINITY;
                         #pragma unroll
-                        for (int n = 32 * g; n < 32 * g + 32; ++n) s[n] = fmaf(-2.0f * a.cap, fast_rcp(1.0f + fast_exp2(s[n] * inner)), a.cap);
-                        c[g] = 1.0f;
+                        for (int n = 0; n < 16; ++n) {
+                            const float x0 = fmaf(__uint_as_float(bits[2 * n]), c, d), x1 = fmaf(__uint_as_float(bits[2 * n + 1]), c, d);
+                            most = max3(most, x0, x1);
+                            const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
+                            packed[16 * g + n] = BF16 ? pack_bf16x2(p0, p1) : pack_half2(p0, p1);
+                            sum0 += p0; sum1 += p1;
+                        }
+                        top = fmaxf(top, most - shift[g]);
+                        sum = fmaf(sum0 + sum1, to_sum[g], sum);
+                    }
+                    first = any_of_rows(top > (top_run == -INFINITY ? -INFINITY : kLift + kRescale));
+                    if (!first) {
+                        sum_run += sum;
+                        #pragma unroll
+                        for (int h = 0; h < kGroups / 2; ++h) tmem_store32(s_base + 64 * h, packed + 32 * h);   // (over scores that have been read)
                     }
                 }
-                if (a.slopes) {
-                    const float from = float(position - int(key0));
-                    #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
+                if (first) {
+                    auto of = [&](const float (&v)[kGroups], int g) -> float {   // (no register is addressed by a variable)
+                        float r = v[0];
                         #pragma unroll
-                        for (int n = 32 * g; n < 32 * g + 32; ++n) s[n] = fmaf(-slope, fabsf(from - float(n)), s[n] * c[g]);
-                        c[g] = 1.0f;
-                    }
-                }
-                if (!walk.open(a, key0)) {
-                    // relative to the tile: keys up to `to`, above `low`, or below `prefix` are seen
-                    const int to = valid ? min(position, int(sequence.length) - 1) - int(key0) : -1;
-                    const int low = a.window ? position - int(a.window) - int(key0) : -1, prefix = valid ? int(sequence.prefix) - int(key0) : 0;
-                    #pragma unroll
-                    for (int n = 0; n < 128; ++n)
-                        if (!((n <= to && n > low) || n < prefix)) s[n] = -INFINITY;
-                }
-                float top = -INFINITY;
-                #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    float t0 = s[32 * g], t1 = s[32 * g + 1];
-                    #pragma unroll
-                    for (int n = 32 * g + 2; n < 32 * g + 32; n += 2) { t0 = fmaxf(t0, s[n]); t1 = fmaxf(t1, s[n + 1]); }
-                    top = fmaxf(top, fmaxf(t0, t1) * c[g]);
-                }
-                // the old maximum serves while the new one is within 2^8 of it: no pass over O
-                const bool grow = top > top_run + kRescale || (top_run == -INFINITY && top > -INFINITY);
-                const float use = grow ? top : top_run;
-                if (__any_sync(0xffffffffu, grow && top_run != -INFINITY)) {
-                    if (!wait(kPvDone + tile_of, (i - 1) & 1)) { alive = false; break; }
-                    fence_after();
-                    const float factor = grow && top_run != -INFINITY ? fast_exp2(top_run - use) : 1.0f;
+                        for (int x = 1; x < kGroups; ++x) r = g == x ? v[x] : r;
+                        return r;
+                    };
+                    const bool finish = !open || RULE;
+                    float top = -INFINITY;
                     #pragma unroll 1
-                    for (int b = 0; b < D / 32; ++b) {
-                        uint32_t o[32];
-                        tmem_load32(o_base + 32 * b, o);
-                        tmem_load_wait(o);
+                    for (int g = 0; g < kGroups; ++g) {
+                        uint32_t bits[32];
+                        tmem_load32(s_base + 32 * g, bits);
+                        tmem_load_wait(bits);
+                        float c = of(to_score, g);
+                        if (RULE && a.cap > 0.0f) {   // cap * tanh(s / cap): the cap (in the exp2 domain) stays outside
+                            c *= a.scale_over_cap;
+                            float most = 0.0f;
+                            #pragma unroll
+                            for (int n = 0; n < 32; n += 2) most = max3(most, fabsf(__uint_as_float(bits[n])), fabsf(__uint_as_float(bits[n + 1])));
+                            if (__all_sync(0xffffffffu, most * c <= kSmallTanh)) {   // (the usual case, scores well below the cap: the series to y^7, on the FMA pipe)
+                                #pragma unroll
+                                for (int n = 0; n < 32; ++n) {
+                                    const float y = __uint_as_float(bits[n]) * c, z = y * y;
+                                    bits[n] = __float_as_uint(fmaf(fmaf(fmaf(z, -17.0f / 315.0f, 2.0f / 15.0f), z, -1.0f / 3.0f) * z, y, y));
+                                }
+                            } else {
+                                #pragma unroll
+                                for (int n = 0; n < 32; ++n) bits[n] = __float_as_uint(any_tanh(__uint_as_float(bits[n]) * c));
+                            }
+                            c = a.cap;
+                        } else {
+                            c *= a.scale_log2;
+                        }
+                        if (RULE && a.slopes) {
+                            const float from = float(position - int(key0) - half * 64 - 32 * g);
+                            #pragma unroll
+                            for (int n = 0; n < 32; ++n) bits[n] = __float_as_uint(fmaf(-slope, fabsf(from - float(n)), __uint_as_float(bits[n]) * c));
+                            c = 1.0f;
+                        }
+                        if (!open) {
+                            // a bit a column: keys up to `to` and above `low`, or below `prefix`, relative to the group
+                            const int base = int(key0) + half * 64 + 32 * g;
+                            const int to = min(position, u.length - 1) - base, low = a.window ? position - int(a.window) - base : -1, prefix = u.prefix - base;
+                            uint32_t seen = (first_bits(to + 1) & ~first_bits(low + 1)) | first_bits(prefix);
+                            if (!valid) seen = 0;
+                            #pragma unroll
+                            for (int n = 0; n < 32; ++n)
+                                if (!(seen & (1u << n))) bits[n] = 0xff800000u;
+                        }
+                        if (finish) tmem_store32(s_base + 32 * g, bits);
+                        float t = __uint_as_float(bits[0]);
                         #pragma unroll
-                        for (int n = 0; n < 32; ++n) o[n] = __float_as_uint(__uint_as_float(o[n]) * factor);
-                        tmem_store32(o_base + 32 * b, o);
+                        for (int n = 1; n < 31; n += 2) t = max3(t, __uint_as_float(bits[n]), __uint_as_float(bits[n + 1]));
+                        top = max3(top, t * c, __uint_as_float(bits[31]) * c);
                     }
-                    tmem_store_wait();
-                    sum_run *= factor;
-                }
-                top_run = use;
-                const float under = use == -INFINITY ? 0.0f : use - kLift;
-                #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const float shift = (a.block_table ? table[g].y : 0.0f) - under;
-                    uint32_t packed[16];
-                    float sums[2] = {0.0f, 0.0f};
-                    #pragma unroll
-                    for (int n = 0; n < 16; ++n) {
-                        const float p0 = fast_exp2(fmaf(s[32 * g + 2 * n], c[g], shift)), p1 = fast_exp2(fmaf(s[32 * g + 2 * n + 1], c[g], shift));
-                        packed[n] = BF16 ? pack_bf16x2(p0, p1) : pack_half2(p0, p1);
-                        sums[0] += p0; sums[1] += p1;
+                    if (finish) tmem_store_wait();
+                    top = fmaxf(top, other_half(top, turn++));
+                    const bool grow = top > top_run + kRescale || (top_run == -INFINITY && top > -INFINITY);
+                    const float use = grow ? top : top_run;
+                    if (i > 0 && __any_sync(0xffffffffu, grow && top_run != -INFINITY)) {
+                        if (!wait(kPvDone + tile_of, (it - 1) & 1)) { alive = false; break; }
+                        fence_after();
+                        const float factor = grow && top_run != -INFINITY ? fast_exp2(top_run - use) : 1.0f;
+                        #pragma unroll 1
+                        for (int b = 0; b < kOColumns / 32; ++b) {
+                            uint32_t o[32];
+                            tmem_load32(o_base + 32 * b, o);
+                            tmem_load_wait(o);
+                            #pragma unroll
+                            for (int n = 0; n < 32; ++n) o[n] = __float_as_uint(__uint_as_float(o[n]) * factor);
+                            tmem_store32(o_base + 32 * b, o);
+                        }
+                        tmem_store_wait();
+                        sum_run *= factor;
                     }
-                    sum_run += (sums[0] + sums[1]) * (a.block_table ? table[g].z : 1.0f);
-                    tmem_store16(s_base + 16 * g, packed);
+                    top_run = use;
+                    const float under = use == -INFINITY ? 0.0f : use - kLift;
+                    #pragma unroll 1
+                    for (int g = 0; g < kGroups; ++g) {
+                        uint32_t bits[32];
+                        tmem_load32(s_base + 32 * g, bits);
+                        const float c = RULE && a.slopes ? 1.0f : RULE && a.cap > 0.0f ? a.cap : a.scale_log2 * of(to_score, g), d = of(shift, g) - under;
+                        tmem_load_wait(bits);
+                        float sum0 = 0.0f, sum1 = 0.0f;
+                        #pragma unroll
+                        for (int n = 0; n < 16; ++n) {
+                            const float p0 = fast_exp2(fmaf(__uint_as_float(bits[2 * n]), c, d)), p1 = fast_exp2(fmaf(__uint_as_float(bits[2 * n + 1]), c, d));
+                            bits[n] = BF16 ? pack_bf16x2(p0, p1) : pack_half2(p0, p1);
+                            sum0 += p0; sum1 += p1;
+                        }
+                        sum_run = fmaf(sum0 + sum1, of(to_sum, g), sum_run);
+                        tmem_store16(s_base + 64 * (g / 2) + 16 * (g % 2), bits);
+                    }
                 }
                 tmem_store_wait();
                 fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&bars[kPFull + buffer]);
             }
+            if (!alive) break;
             // ---- O / sum ----
-            // (the last scores were issued behind all products but the last two of one tile: both are waited for in turn, a barrier's parity
-            //  tells neighbouring phases apart only)
-            if (T == 1 && alive && tiles > 1 && !wait(kPvDone, (tiles - 2) & 1)) alive = false;
-            if (alive && tiles && !wait(kPvDone + tile_of, (tiles - 1) & 1)) alive = false;
+            // (T 1: the last scores were issued behind all products but the last two: both are waited for in turn, a barrier's parity tells
+            //  neighbouring phases apart only)
+            if (T == 1 && tiles > 1 && !wait(kPvDone, (done + tiles - 2) & 1)) { alive = false; break; }
+            if (tiles && !wait(kPvDone + tile_of, (done + tiles - 1) & 1)) { alive = false; break; }
             fence_after();
-            if (alive) {
-                const float lift = a.value_top ? a.value_top[walk.s * a.kv_heads + walk.kv] : 1.0f;
-                const float inverse = a.splits > 1 ? lift : sum_run > 0.0f ? lift / sum_run : sum_run == 0.0f ? 0.0f : sum_run;
-                const size_t slot = (size_t(blockIdx.x) * T + tile_of) * kM + m;
-                const uint32_t patches = min(*reinterpret_cast<volatile uint32_t*>(flagged_count), uint32_t(kFlagged));
-                #pragma unroll 1
-                for (int b = 0; b < D / 32; ++b) {
-                    uint32_t bits[32];
-                    float o[32];
-                    if (tiles) { tmem_load32(o_base + 32 * b, bits); tmem_load_wait(bits); }
-                    #pragma unroll
-                    for (int n = 0; n < 32; ++n) o[n] = tiles ? __uint_as_float(bits[n]) : 0.0f;
-                    if (!valid) continue;
-                    for (uint32_t p = 0; p < patches; ++p) {
-                        // values that were taken out of a tile: back for the rows that see them (rare: nothing here is fast)
+            if (T == 1) sum_run += other_half(sum_run, turn++);
+            const float lift = a.value_top ? a.value_top[u.s * a.kv_heads + u.kv] : 1.0f;
+            const float inverse = !run.whole ? lift : sum_run > 0.0f ? lift / sum_run : sum_run == 0.0f ? 0.0f : sum_run;
+            const size_t slot = ((2 * size_t(blockIdx.x) + (run.begin ? 0 : 1)) * T + tile_of) * kM + m;
+            const bool patches = tiles && *flagged_piece == piece + 1;
+            auto leave = [&] {   // O (and `flagged`) may be written again
+                fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&bars[kOFree + tile_of]);
+            };
+            #pragma unroll 1
+            for (int b = 0; b < kOColumns / 32; ++b) {
+                uint32_t bits[32];
+                float o[32];
+                if (tiles) { tmem_load32(o_base + 32 * b, bits); tmem_load_wait(bits); }
+                #pragma unroll
+                for (int n = 0; n < 32; ++n) o[n] = tiles ? __uint_as_float(bits[n]) : 0.0f;
+                if (b + 1 == kOColumns / 32 && tiles && !patches) leave();
+                const int column = half * kOColumns + 32 * b;
+                if (patches && valid) {
+                    // values that were taken out of a tile: back for the rows that see them (rare: nothing here is fast)
+                    for (int p = 0; p < kFlagged; ++p) {
                         const int base = int(flagged[8 * p]);
                         for (int n = 0; n < S::kSlotKeys; ++n) {
                             if (!(flagged[8 * p + 1 + n / 32] >> (n % 32) & 1)) continue;
                             const int key = base + n;
-                            const bool seen = key < int(sequence.length) && ((key <= position && (!a.window || key > position - int(a.window))) || key < int(sequence.prefix));
+                            const bool seen = key < u.length && ((key <= position && (!a.window || key > position - int(a.window))) || key < u.prefix);
                             if (!seen) continue;
-                            const uint16_t* v = a.values + (size_t(sequence.first_key) + key) * a.value_stride + walk.kv * D + 32 * b;
+                            const uint16_t* v = a.values + (size_t(sequence.first_key) + key) * a.value_stride + u.kv * D + column;
+                            #pragma unroll 1
                             for (int x = 0; x < 32; ++x) {
                                 const float f = BF16 ? __uint_as_float(uint32_t(v[x]) << 16) : __half2float(__ushort_as_half(v[x]));
-                                if (!(fabsf(f) <= FLT_MAX)) o[x] += f;
+                                if (fabsf(f) <= FLT_MAX) continue;
+                                #pragma unroll
+                                for (int y = 0; y < 32; ++y) if (y == x) o[y] += f;   // (no register is addressed by a variable)
                             }
                         }
                     }
-                    if (a.splits > 1) {
-                        float4* to = reinterpret_cast<float4*>(a.partial + slot * D + 32 * b);
+                }
+                if (!valid) continue;
+                if (!run.whole) {
+                    float4* to = reinterpret_cast<float4*>(a.partial + slot * D + column);
+                    #pragma unroll
+                    for (int n = 0; n < 8; ++n) to[n] = make_float4(o[4 * n] * inverse, o[4 * n + 1] * inverse, o[4 * n + 2] * inverse, o[4 * n + 3] * inverse);
+                } else {
+                    uint16_t* to = static_cast<uint16_t*>(a.out) + (size_t(sequence.first_row) + token) * a.out_stride + size_t(head) * D + column;
+                    uint32_t w[16];
+                    #pragma unroll
+                    for (int n = 0; n < 16; ++n) w[n] = BF16 ? pack_bf16x2(o[2 * n] * inverse, o[2 * n + 1] * inverse) : pack_half2(o[2 * n] * inverse, o[2 * n + 1] * inverse);
+                    if (a.wide_out) { store32(to, w); store32(to + 16, w + 8); }   // (whole sectors)
+                    else {
                         #pragma unroll
-                        for (int n = 0; n < 8; ++n) to[n] = make_float4(o[4 * n] * inverse, o[4 * n + 1] * inverse, o[4 * n + 2] * inverse, o[4 * n + 3] * inverse);
-                    } else {
-                        uint4* to = reinterpret_cast<uint4*>(static_cast<uint16_t*>(a.out) + (size_t(sequence.first_row) + token) * a.out_stride + size_t(head) * D + 32 * b);
-                        #pragma unroll
-                        for (int n = 0; n < 4; ++n) {
-                            uint32_t w[4];
-                            #pragma unroll
-                            for (int x = 0; x < 4; ++x)
-                                w[x] = BF16 ? pack_bf16x2(o[8 * n + 2 * x] * inverse, o[8 * n + 2 * x + 1] * inverse) : pack_half2(o[8 * n + 2 * x] * inverse, o[8 * n + 2 * x + 1] * inverse);
-                            to[n] = make_uint4(w[0], w[1], w[2], w[3]);
-                        }
+                        for (int n = 0; n < 4; ++n) reinterpret_cast<uint4*>(to)[n] = make_uint4(w[4 * n], w[4 * n + 1], w[4 * n + 2], w[4 * n + 3]);
                     }
                 }
-                if (a.splits > 1 && valid) *reinterpret_cast<float2*>(a.sums + slot * 2) = make_float2(top_run, sum_run);
+            }
+            if (!run.whole && valid && half == 0) *reinterpret_cast<float2*>(a.sums + slot * 2) = make_float2(top_run, sum_run);
+            if (patches) leave();
+            if (tiles) {
+                ++piece;
+                done += tiles;
             }
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
         const uint32_t ring = smem_u32(smem + S::kOffRing);
-        // The ring's order, for all roles below: K of the first tile (of two tiles with 256 columns), then V of tile i and K of the next.
-        constexpr int kAhead = T == 2 ? 1 : 2;
-        if (warp == 8) {
+        // The ring's order within a piece, for all roles below: K of the first tile (of two tiles with 256 columns), then V of tile i and K of a later one.
+        constexpr uint32_t kAhead = T == 2 ? 1 : 2;
+        uint32_t items = 0;   // slots used by the pieces before
+        if (warp == kIssueWarp) {
             // ================= the products =================
-            if (lane == 0 && tiles) {
+            if (lane == 0) {
                 const uint32_t idesc_s = instr_desc(kM, S::kSlotKeys, BF16, false), idesc_o = instr_desc(kM, D, BF16, true);
                 const uint32_t queries = smem_u32(smem);
-                uint32_t item = 0, looked = 0;
-                bool alive = wait(kQFull, 0);
+                uint32_t looked = 0;
                 auto score = [&](int tile, int buffer, uint32_t first_item) -> bool {
                     for (int h = 0; h < S::kHalves; ++h) {
-                        const uint32_t at = first_item + h, slot = at % S::kSlots;
+                        const uint32_t at = items + first_item + h, slot = at % S::kSlots;
                         if (!wait(kFull + slot, (at / S::kSlots) & 1)) return false;
                         fence_after();
                         const uint32_t b = desc_low(ring + slot * S::kSlotBytes, 16), q = desc_low(queries + tile * S::kQueryBytes, 16);
@@ -407,123 +560,148 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
                     umma_commit(&bars[kSFull + buffer]);
                     return true;
                 };
-                // K tiles: the first kAhead at items 0 .., K(i) for i >= kAhead behind V(i - kAhead)
-                auto k_item = [&](uint32_t i) -> uint32_t { return i < uint32_t(kAhead) ? i * S::kHalves : (kAhead + 2 * (i - kAhead) + 1) * S::kHalves; };
-                auto v_item = [&](uint32_t i) -> uint32_t {
-                    const uint32_t ahead = min(uint32_t(kAhead), tiles);   // (K tiles before V(0); the last V tiles have no K between them)
-                    const uint32_t k_before = min(i, tiles - ahead);
-                    return (ahead + i + k_before) * S::kHalves;
-                };
-                for (int f = 0; f < kAhead && uint32_t(f) < tiles && alive; ++f) {
-                    if (T == 2) { alive = alive && score(0, 0, 0); alive = alive && score(1, 1, 0); }
-                    else alive = alive && score(0, f, k_item(f));
-                }
-                #pragma unroll 1
-                for (uint32_t i = 0; i < tiles && alive; ++i) {
-                    const bool look = a.values && !walk.open(a, walk.key(walk.begin + i));
-                    item = v_item(i);
-                    if (look) {   // (the tile's values are there: they are looked at while the softmax runs)
-                        for (int h = 0; h < S::kHalves && alive; ++h) alive = wait(kFull + (item + h) % S::kSlots, ((item + h) / S::kSlots) & 1);
-                        if (!alive) break;
-                        mbar_arrive(&bars[kLook]);
+                for (bool more = run.start(a); more && alive; more = run.next(a)) {
+                    const uint32_t tiles = run.end - run.begin;
+                    if (!tiles) continue;
+                    if (!wait(kQFull, piece & 1)) { alive = false; break; }
+                    const uint32_t ahead = min(kAhead, tiles);
+                    // K tiles: the first `ahead` at items 0 .., K(i) for i >= kAhead behind V(i - kAhead)
+                    auto k_item = [&](uint32_t i) -> uint32_t { return (i < kAhead ? i : 2 * i + 1 - kAhead) * S::kHalves; };
+                    for (uint32_t f = 0; f < ahead && alive; ++f) {
+                        if (T == 2) { alive = alive && score(0, 0, 0); alive = alive && score(1, 1, 0); }
+                        else alive = alive && score(0, int((done + f) & 1), k_item(f));
                     }
+                    if (alive && tiles <= kAhead) umma_commit(&bars[kQFree]);
                     #pragma unroll 1
-                    for (int tile = 0; tile < T && alive; ++tile) {
-                        const int buffer = T == 2 ? tile : int(i & 1);
-                        if (!wait(kPFull + buffer, T == 2 ? i & 1 : (i >> 1) & 1)) { alive = false; break; }
-                        for (int h = 0; h < S::kHalves && alive; ++h) {
-                            const uint32_t slot = (item + h) % S::kSlots;
-                            if (tile == 0) {
-                                if (!wait(kFull + slot, ((item + h) / S::kSlots) & 1)) { alive = false; break; }
-                                if (look && h == 0) {
-                                    if (!wait(kClean, looked & 1)) { alive = false; break; }
-                                    ++looked;
-                                }
-                            }
-                            fence_after();
-                            const uint32_t v = desc_low(ring + slot * S::kSlotBytes, S::kSlotKeys * 128);
-                            #pragma unroll
-                            for (int kk = 0; kk < S::kSlotKeys / 16; ++kk)
-                                umma_a_tmem(tmem + S::kO + tile * D, tmem + S::kS + buffer * 128 + h * (S::kSlotKeys / 2) + kk * 8,
-                                            desc_of(v + ((kk * (16 * 128)) >> 4)), idesc_o, i > 0 || h > 0 || kk > 0);
-                            if (T == 1 || tile == 1) umma_commit(&bars[kFree + slot]);
+                    for (uint32_t i = 0; i < tiles && alive; ++i) {
+                        const bool look = a.values && !run.u.open(a, run.u.key(run.begin + i));
+                        const uint32_t item = items + (ahead + i + min(i, tiles - ahead)) * S::kHalves, it = done + i;   // V(i)
+                        if (i == 0 && piece) {   // the outputs of the piece before have left O (and `flagged`)
+                            for (int tile = 0; tile < T && alive; ++tile) alive = wait(kOFree + tile, (piece - 1) & 1);
+                            if (!alive) break;
                         }
-                        if (!alive) break;
-                        umma_commit(&bars[kPvDone + tile]);
-                        if (i + kAhead < tiles) alive = score(tile, buffer, k_item(i + kAhead));
+                        if (look) {   // (the tile's values are there: they are looked at while the softmax runs)
+                            for (int h = 0; h < S::kHalves && alive; ++h) alive = wait(kFull + (item + h) % S::kSlots, ((item + h) / S::kSlots) & 1);
+                            if (!alive) break;
+                            mbar_arrive(&bars[kLook]);
+                        }
+                        #pragma unroll 1
+                        for (int tile = 0; tile < T && alive; ++tile) {
+                            const int buffer = T == 2 ? tile : int(it & 1);
+                            if (!wait(kPFull + buffer, T == 2 ? it & 1 : (it >> 1) & 1)) { alive = false; break; }
+                            for (int h = 0; h < S::kHalves && alive; ++h) {
+                                const uint32_t slot = (item + h) % S::kSlots;
+                                if (tile == 0) {
+                                    if (!wait(kFull + slot, ((item + h) / S::kSlots) & 1)) { alive = false; break; }
+                                    if (look && h == 0) {
+                                        if (!wait(kClean, looked & 1)) { alive = false; break; }
+                                        ++looked;
+                                    }
+                                }
+                                fence_after();
+                                const uint32_t v = desc_low(ring + slot * S::kSlotBytes, S::kSlotKeys * 128);
+                                #pragma unroll
+                                for (int kk = 0; kk < S::kSlotKeys / 16; ++kk)
+                                    umma_a_tmem(tmem + S::kO + tile * D, tmem + S::kS + buffer * 128 + (h * S::kSlotKeys + kk * 16) / 64 * 64 + (h * S::kSlotKeys + kk * 16) % 64 / 2,
+                                                desc_of(v + ((kk * (16 * 128)) >> 4)), idesc_o, i > 0 || h > 0 || kk > 0);
+                                if (T == 1 || tile == 1) umma_commit(&bars[kFree + slot]);
+                            }
+                            if (!alive) break;
+                            umma_commit(&bars[kPvDone + tile]);
+                            if (i + kAhead < tiles) {
+                                alive = score(tile, buffer, k_item(i + kAhead));
+                                if (alive && tile == T - 1 && i + kAhead + 1 == tiles) umma_commit(&bars[kQFree]);
+                            }
+                        }
                     }
+                    items += 2 * tiles * S::kHalves;
+                    done += tiles;
+                    ++piece;
                 }
             }
-        } else if (warp == 9) {
+        } else if (warp == kLoadWarp) {
             // ================= the loads =================
-            if (lane == 0 && tiles) {
-                mbar_expect_tx(&bars[kQFull], uint32_t(T * (D / 64)) * a.tokens * a.group * 128);
-                #pragma unroll 1
-                for (int tile = 0; tile < T; ++tile)
-                    for (int x = 0; x < D / 64; ++x)
-                        tma_load(smem + tile * S::kQueryBytes + x * (kM * 128), &a.q_map, 64 * x, int(walk.kv * a.group),
-                                 int(sequence.first_row + (walk.block * T + tile) * a.tokens), &bars[kQFull]);
-                uint32_t item = 0;
-                bool alive = true;
-                auto load = [&](const CUtensorMap& map, uint32_t i) {
-                    const int key = int(sequence.first_key + walk.key(walk.begin + i));
-                    for (int h = 0; h < S::kHalves && alive; ++h, ++item) {
-                        const uint32_t slot = item % S::kSlots;
-                        if (item >= uint32_t(S::kSlots) && !wait(kFree + slot, (item / S::kSlots - 1) & 1)) { alive = false; return; }
-                        mbar_expect_tx(&bars[kFull + slot], S::kSlotBytes);
+            if (lane == 0) {
+                for (bool more = run.start(a); more && alive; more = run.next(a)) {
+                    const uint32_t tiles = run.end - run.begin;
+                    if (!tiles) continue;
+                    const KernelSequence& sequence = a.sequence[run.u.s];
+                    if (piece && !wait(kQFree, (piece - 1) & 1)) { alive = false; break; }
+                    mbar_expect_tx(&bars[kQFull], uint32_t(T * (D / 64)) * a.tokens * a.group * 128);
+                    #pragma unroll 1
+                    for (int tile = 0; tile < T; ++tile)
                         for (int x = 0; x < D / 64; ++x)
-                            tma_load(smem + S::kOffRing + slot * S::kSlotBytes + x * (S::kSlotKeys * 128), &map, 64 * x, int(walk.kv), key + h * S::kSlotKeys, &bars[kFull + slot]);
+                            tma_load(smem + tile * S::kQueryBytes + x * (kM * 128), &a.q_map, 64 * x, int(run.u.kv * a.group),
+                                     int(sequence.first_row + run.u.row + tile * a.tokens), &bars[kQFull]);
+                    auto load = [&](const CUtensorMap& map, uint32_t i) {
+                        const int key = int(sequence.first_key + run.u.key(run.begin + i));
+                        for (int h = 0; h < S::kHalves && alive; ++h, ++items) {
+                            const uint32_t slot = items % S::kSlots;
+                            if (items >= uint32_t(S::kSlots) && !wait(kFree + slot, (items / S::kSlots - 1) & 1)) { alive = false; return; }
+                            mbar_expect_tx(&bars[kFull + slot], S::kSlotBytes);
+                            for (int x = 0; x < D / 64; ++x)
+                                tma_load(smem + S::kOffRing + slot * S::kSlotBytes + x * (S::kSlotKeys * 128), &map, 64 * x, int(run.u.kv), key + h * S::kSlotKeys, &bars[kFull + slot]);
+                        }
+                    };
+                    for (uint32_t i = 0; i < kAhead && i < tiles && alive; ++i) load(a.k_map, i);
+                    #pragma unroll 1
+                    for (uint32_t i = 0; i < tiles && alive; ++i) {
+                        load(a.v_map, i);
+                        if (alive && i + kAhead < tiles) load(a.k_map, i + kAhead);
                     }
-                };
-                for (uint32_t i = 0; i < uint32_t(kAhead) && i < tiles; ++i) load(a.k_map, i);
-                #pragma unroll 1
-                for (uint32_t i = 0; i < tiles && alive; ++i) {
-                    load(a.v_map, i);
-                    if (alive && i + kAhead < tiles) load(a.k_map, i + kAhead);
+                    ++piece;
                 }
             }
         } else if (a.values) {
             // ================= masked values that are not finite =================
-            const int t = (warp - 10) * 32 + lane;
-            const uint32_t ahead = min(uint32_t(kAhead), tiles);
-            int edge = 0;          // slots looked at: the entry of `flagged` is the slot's own
+            const int t = (warp - kLookWarp) * 32 + lane;
             uint32_t looked = 0;   // tiles looked at (the next is not asked for before this one is done: the barriers' parities cannot be missed)
-            bool alive = true;
-            #pragma unroll 1
-            for (uint32_t i = 0; i < tiles && alive; ++i) {
-                const uint32_t key0 = walk.key(walk.begin + i);
-                if (walk.open(a, key0)) continue;
-                if (!wait(kLook, looked & 1)) break;
-                ++looked;
-                for (int h = 0; h < S::kHalves; ++h) {
-                    const uint32_t at = (ahead + i + min(i, tiles - ahead)) * S::kHalves + h, slot = at % S::kSlots;
-                    if (!wait(kFull + slot, (at / S::kSlots) & 1)) { alive = false; break; }
-                    uint4* rows = reinterpret_cast<uint4*>(smem + S::kOffRing + slot * S::kSlotBytes);   // [64 columns of ..][key][8 pieces of 16 bytes]
-                    constexpr uint32_t kExponent = BF16 ? 0x7f807f80u : 0x7c007c00u, kCarry = BF16 ? 0x00800080u : 0x04000400u;
-                    #pragma unroll 1
-                    for (int piece = t; piece < S::kSlotBytes / 16 && edge < kFlagged; piece += 64) {
-                        const uint4 v = rows[piece];
-                        uint32_t w[4] = {v.x, v.y, v.z, v.w}, hit = 0;
-                        #pragma unroll
-                        for (int x = 0; x < 4; ++x) hit |= (w[x] & kExponent) + kCarry;
-                        if (!(hit & 0x80008000u)) continue;
-                        #pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            const uint32_t bad = (w[x] & kExponent) + kCarry;
-                            if (bad & 0x8000u) w[x] &= 0xffff0000u;
-                            if (bad & 0x80000000u) w[x] &= 0x0000ffffu;
-                        }
-                        rows[piece] = make_uint4(w[0], w[1], w[2], w[3]);
-                        const int n = piece / 8 % S::kSlotKeys;
-                        flagged[8 * edge] = key0 + h * S::kSlotKeys;
-                        atomicOr(&flagged[8 * edge + 1 + n / 32], 1u << (n % 32));
-                        atomicMax(flagged_count, uint32_t(edge) + 1);
+            for (bool more = run.start(a); more && alive; more = run.next(a)) {
+                const uint32_t tiles = run.end - run.begin, ahead = min(kAhead, tiles);
+                if (!tiles) continue;
+                int edge = 0;      // slots of the piece looked at: the entry of `flagged` is the slot's own
+                #pragma unroll 1
+                for (uint32_t i = 0; i < tiles && alive; ++i) {
+                    const uint32_t key0 = run.u.key(run.begin + i);
+                    if (run.u.open(a, key0)) continue;
+                    if (!wait(kLook, looked & 1)) { alive = false; break; }
+                    ++looked;
+                    if (!edge) {   // (the outputs of the piece before are done: the issuing thread has waited for them)
+                        for (int e = t; e < kFlagged * 8; e += 64) flagged[e] = 0;
+                        asm volatile("bar.sync 9, 64;" ::: "memory");
                     }
-                    ++edge;
+                    for (int h = 0; h < S::kHalves; ++h) {
+                        const uint32_t at = items + (ahead + i + min(i, tiles - ahead)) * S::kHalves + h, slot = at % S::kSlots;
+                        if (!wait(kFull + slot, (at / S::kSlots) & 1)) { alive = false; break; }
+                        uint4* rows = reinterpret_cast<uint4*>(smem + S::kOffRing + slot * S::kSlotBytes);   // [64 columns of ..][key][8 pieces of 16 bytes]
+                        constexpr uint32_t kExponent = BF16 ? 0x7f807f80u : 0x7c007c00u, kCarry = BF16 ? 0x00800080u : 0x04000400u;
+                        #pragma unroll 4
+                        for (int at_piece = t; at_piece < S::kSlotBytes / 16; at_piece += 64) {
+                            const uint4 v = rows[at_piece];
+                            uint32_t w[4] = {v.x, v.y, v.z, v.w}, hit = 0;
+                            #pragma unroll
+                            for (int x = 0; x < 4; ++x) hit |= (w[x] & kExponent) + kCarry;
+                            if (!(hit & 0x80008000u) || edge >= kFlagged) continue;
+                            #pragma unroll
+                            for (int x = 0; x < 4; ++x) {
+                                const uint32_t bad = (w[x] & kExponent) + kCarry;
+                                if (bad & 0x8000u) w[x] &= 0xffff0000u;
+                                if (bad & 0x80000000u) w[x] &= 0x0000ffffu;
+                            }
+                            rows[at_piece] = make_uint4(w[0], w[1], w[2], w[3]);
+                            const int n = at_piece / 8 % S::kSlotKeys;
+                            flagged[8 * edge] = key0 + h * S::kSlotKeys;
+                            atomicOr(&flagged[8 * edge + 1 + n / 32], 1u << (n % 32));
+                            *flagged_piece = piece + 1;
+                        }
+                        ++edge;
+                    }
+                    fence_proxy_async();   // (the tensor core reads the slots through the async proxy)
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(&bars[kClean]);
                 }
-                fence_proxy_async();   // (the tensor core reads the slots through the async proxy)
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bars[kClean]);
+                items += 2 * tiles * S::kHalves;
+                ++piece;
             }
         }
     }
@@ -531,38 +709,35 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
     if (*abort_flag) drain_delay();   // (copies that were in flight when a role gave up)
     fence_before();
     __syncthreads();
-    if (warp == 8) {
+    if (warp == kIssueWarp) {
         fence_after();
         asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(512u) : "memory");
     }
 }
 
-// Warp = M-row: joins the splits of a block's key range.
+// Warp = M-row of a shared unit: joins its pieces, in the order of the keys.
 template<int D, bool BF16>
 __global__ void __launch_bounds__(256) masked_attention_join_kernel(const __grid_constant__ Args a) {
     constexpr int T = Shape<D>::kTiles, kEach = D / 32;
-    const uint32_t lane = threadIdx.x % 32, index = blockIdx.x * 8 + threadIdx.x / 32, unit = index / (T * kM), tile = index / kM % T, m = index % kM;
-    uint32_t s = 0;
-    {
-        uint32_t high = a.sequences;
-        while (high - s > 1) { const uint32_t mid = (s + high) / 2; if (a.sequence[mid].first_unit <= unit) s = mid; else high = mid; }
-    }
-    const KernelSequence& sequence = a.sequence[s];
-    const uint32_t inside = unit - sequence.first_unit, kv = inside % a.kv_heads, block = sequence.blocks - 1 - inside / a.kv_heads;
-    const uint32_t token = (block * T + tile) * a.tokens + m / a.group, head = kv * a.group + m % a.group;
+    const uint32_t lane = threadIdx.x % 32, index = blockIdx.x * 8 + threadIdx.x / 32, tile = index / kM % T, m = index % kM;
+    const Shared share = a.share[index / (T * kM)];
+    Unit u;
+    u.find(a, share.unit, T * a.tokens);
+    const KernelSequence& sequence = a.sequence[u.s];
+    const uint32_t token = u.row + tile * a.tokens + m / a.group, head = u.kv * a.group + m % a.group;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (token >= sequence.rows || m >= a.tokens * a.group) return;
+    auto slot = [&](uint32_t p) -> size_t { return ((2 * (size_t(share.first) + p) + (p == 0 ? 1 : 0)) * T + tile) * kM + m; };
     float top = -INFINITY, weight = 0.0f, total[kEach];
     #pragma unroll
     for (int e = 0; e < kEach; ++e) total[e] = 0.0f;
-    const size_t first = (size_t(unit) * a.splits * T + tile) * kM + m, step = size_t(T) * kM;
-    for (uint32_t p = 0; p < a.splits; ++p) top = fmaxf(top, a.sums[(first + p * step) * 2]);
+    for (uint32_t p = 0; p < share.pieces; ++p) top = fmaxf(top, a.sums[slot(p) * 2]);
     #pragma unroll 2
-    for (uint32_t p = 0; p < a.splits; ++p) {
-        const float2 v = *reinterpret_cast<const float2*>(a.sums + (first + p * step) * 2);
+    for (uint32_t p = 0; p < share.pieces; ++p) {
+        const float2 v = *reinterpret_cast<const float2*>(a.sums + slot(p) * 2);
         const float factor = v.x == -INFINITY ? (v.y == 0.0f ? 0.0f : 1.0f) : fast_exp2(v.x - top);   // (scores that are all NaN leave a NaN sum)
         weight = fmaf(factor, v.y, weight);
-        const float* from = a.partial + (first + p * step) * D;
+        const float* from = a.partial + slot(p) * D;
         #pragma unroll
         for (int e = 0; e < kEach; e += 2) {
             const float2 o = *reinterpret_cast<const float2*>(from + (e / 2 * 32 + lane) * 2);
@@ -586,7 +761,7 @@ struct UnpackArgs {
     UnpackSequence sequence[kSequences];
     uint32_t sequences, kv_heads, blocks;
     uint16_t* rows;       // [2 * kv_heads][blocks * 32][D]
-    float4* table;
+    float* table;
     float* top;
 };
 
@@ -623,11 +798,12 @@ __global__ void __launch_bounds__(128) kv8_unpack_kernel(const __grid_constant__
         top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
         if (!(top > 0.0f)) top = 1.0f;
         if (threadIdx.x == 0) a.top[size_t(blockIdx.x) * a.kv_heads + kv] = top;
-        float4* to = a.table + size_t(kv) * a.blocks + q.first_block;
+        float* to = a.table + (size_t(kv) * a.blocks + q.first_block) * 3;
         for (uint32_t i = threadIdx.x; i < q.blocks; i += 128) {
             // (a block of zeros counts as one of scale `top`: its values add nothing. Below 2^-64 of the largest a value scale is taken as that.)
             const float ratio = i < real && v[i] > 0.0f ? fmaxf(v[i] / top, 5.421010862427522e-20f) : 1.0f, down = log2f(ratio);
-            to[i] = make_float4(i < real ? fmaxf(k[i], 1e-30f) : 1e-30f, down, 1.0f / fast_exp2(down), 0.0f);
+            float* at = to + i / 4 * 12 + i % 4;
+            at[0] = i < real ? fmaxf(k[i], 1e-30f) : 1e-30f; at[4] = down; at[8] = 1.0f / fast_exp2(down);
         }
         return;
     }
@@ -696,25 +872,59 @@ template<int D, bool BF16> static void launch(Device& d, Args& args, bool behind
     using S = Shape<D>;
     static bool configured[64] = {};
     if (!configured[d.ordinal & 63]) {
-        SDB_CHECK(cudaFuncSetAttribute(masked_attention_kernel<D, BF16>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(S::kSmem)));
+        SDB_CHECK(cudaFuncSetAttribute(masked_attention_kernel<D, BF16, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(S::kSmem)));
+        SDB_CHECK(cudaFuncSetAttribute(masked_attention_kernel<D, BF16, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(S::kSmem)));
         configured[d.ordinal & 63] = true;
     }
-    uint32_t units = 0, longest = 0;
+    uint32_t units = 0;
+    const uint32_t rows_a_unit = S::kTiles * args.tokens;
     for (uint32_t s = 0; s < args.sequences; ++s) {
         KernelSequence& q = args.sequence[s];
-        const uint32_t tokens = S::kTiles * args.tokens;
-        q.blocks = (q.rows + tokens - 1) / tokens;
+        q.blocks = (q.rows + rows_a_unit - 1) / rows_a_unit;
         q.first_unit = units;
         if (uint64_t(units) + uint64_t(q.blocks) * args.kv_heads >= uint64_t(1) << 30) throw std::runtime_error("too many attention rows in one call");
         units += q.blocks * args.kv_heads;
-        const uint32_t seen = args.window ? std::min(q.length, args.window + tokens + q.prefix) : q.length;
-        longest = std::max(longest, (seen + kTileKeys - 1) / kTileKeys);
     }
-    // Few blocks: the key range is cut, so that every SM has one; a cut of fewer than four tiles would be mostly prologue
-    args.splits = std::max<uint32_t>(1, std::min<uint32_t>(uint32_t(d.sms) / units, longest / 4));
+    // The runs: a unit weighs its tiles and two more. The units of a block of rows, one a K/V head, are alike.
+    constexpr uint32_t kUnitTiles = 2;   // what a unit's first products, masked tiles and output cost more, in tiles
+    uint64_t weight = 0;
+    auto each_block = [&](auto&& act) {   // act(first unit, tiles of each of its kv_heads units); false ends
+        for (uint32_t s = 0; s < args.sequences; ++s)
+            for (uint32_t b = 0; b < args.sequence[s].blocks; ++b) {
+                Unit u;
+                u.find(args, args.sequence[s].first_unit + b * args.kv_heads, rows_a_unit);
+                if (!act(args.sequence[s].first_unit + b * args.kv_heads, u.tiles)) return;
+            }
+    };
+    each_block([&](uint32_t, uint32_t tiles) { weight += uint64_t(tiles + kUnitTiles) * args.kv_heads; return true; });
+    constexpr uint64_t kLeast = 4;   // tiles (and unit) a run is worth a block of its own
+    const uint32_t blocks = uint32_t(std::max<uint64_t>(1, std::min<uint64_t>(std::min<uint64_t>(uint64_t(d.sms), kMostBlocks), std::max<uint64_t>(weight / kLeast, std::min<uint64_t>(units, weight / 2)))));
+    uint64_t passed = 0;
+    uint32_t next = 1;
+    args.cut[0] = Cut{0, 0};
+    each_block([&](uint32_t first, uint32_t tiles) {
+        const uint64_t each = tiles + kUnitTiles, end = passed + each * args.kv_heads;
+        for (; next < blocks; ++next) {
+            const uint64_t target = weight * next / blocks;
+            if (target >= end) break;
+            const uint64_t inside = (target - passed) / each, offset = (target - passed) % each;   // (offset 0 is the unit's own start)
+            // a piece of less than two tiles is left to the neighbour
+            const uint32_t tile = offset <= kUnitTiles + 1 ? 0 : uint32_t(offset) - kUnitTiles;
+            args.cut[next] = tile && tile + 2 <= tiles ? Cut{first + uint32_t(inside), tile} : Cut{first + uint32_t(inside) + (tile ? 1 : 0), 0};
+        }
+        passed = end;
+        return next < blocks;
+    });
+    for (; next <= blocks; ++next) args.cut[next] = Cut{units, 0};
+    args.shares = 0;
+    for (uint32_t b = 1; b < blocks; ++b) {
+        if (!args.cut[b].tile) continue;
+        if (args.shares && args.share[args.shares - 1].unit == args.cut[b].unit) ++args.share[args.shares - 1].pieces;
+        else args.share[args.shares++] = Shared{args.cut[b].unit, b - 1, 2};
+    }
     args.status = status_word(d);
-    if (args.splits > 1) {
-        const size_t rows = size_t(units) * args.splits * S::kTiles * kM;
+    if (args.shares) {
+        const size_t rows = size_t(2) * blocks * S::kTiles * kM;
         args.partial = static_cast<float*>(workspace(d, d.kv8_partial, rows * (D + 2) * 4));
         args.sums = args.partial + rows * D;
     }
@@ -722,16 +932,16 @@ template<int D, bool BF16> static void launch(Device& d, Args& args, bool behind
     attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attribute.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t config{};
-    config.gridDim = dim3(units * args.splits);
+    config.gridDim = dim3(blocks);
     config.blockDim = dim3(kThreads);
     config.dynamicSmemBytes = S::kSmem;
     config.stream = d.stream;
     config.attrs = &attribute;
     config.numAttrs = behind ? 1 : 0;
-    SDB_CHECK(cudaLaunchKernelEx(&config, masked_attention_kernel<D, BF16>, args));
+    SDB_CHECK(cudaLaunchKernelEx(&config, args.slopes || args.cap > 0.0f ? masked_attention_kernel<D, BF16, true> : masked_attention_kernel<D, BF16, false>, args));
     ++d.launches;
-    if (args.splits > 1) {
-        config.gridDim = dim3(units * S::kTiles * kM / 8);
+    if (args.shares) {
+        config.gridDim = dim3(args.shares * S::kTiles * kM / 8);
         config.blockDim = dim3(256);
         config.dynamicSmemBytes = 0;
         config.numAttrs = 1;
@@ -753,6 +963,7 @@ static Args rule_args(uint64_t heads, uint64_t kv_heads, uint64_t dim, float sca
     args.heads = uint32_t(heads); args.kv_heads = uint32_t(kv_heads); args.group = uint32_t(heads / kv_heads); args.tokens = uint32_t(kM / args.group);
     args.window = uint32_t(std::min<uint64_t>(window, uint64_t(1) << 30));
     args.out = out; args.out_stride = out_stride; args.slopes = slopes;
+    args.wide_out = reinterpret_cast<uintptr_t>(out) % 32 == 0 && out_stride % 16 == 0;
     args.scale_log2 = scale * 1.4426950408889634f;
     args.cap = cap * 1.4426950408889634f;
     args.scale_over_cap = cap > 0.0f ? scale / cap : 0.0f;
@@ -783,10 +994,10 @@ void attend_kv8(Device& d, const std::vector<Sequence>& sequences, uint64_t head
         unpack.blocks = uint32_t(blocks);
         args.block_table = nullptr; args.value_top = nullptr;
         if (blocks) {
-            const size_t row_bytes = checked_product({2 * kv_heads, blocks, 32, dim, 2}), table_bytes = checked_product({kv_heads, blocks, 16});
+            const size_t row_bytes = checked_product({2 * kv_heads, blocks, 32, dim, 2}), table_bytes = checked_product({kv_heads, blocks, 12});
             auto* space = static_cast<uint8_t*>(workspace(d, d.kv8_rows, row_bytes + table_bytes + args.sequences * kv_heads * 4));
             unpack.rows = reinterpret_cast<uint16_t*>(space);
-            unpack.table = reinterpret_cast<float4*>(space + row_bytes);
+            unpack.table = reinterpret_cast<float*>(space + row_bytes);
             unpack.top = reinterpret_cast<float*>(space + row_bytes + table_bytes);
             const dim3 grid{unsigned(std::max<uint64_t>(blocks, args.sequences)), unsigned(3 * kv_heads)};
             const bool bf16 = type == kv8::kBf16, int8 = code == kv8::kInt8;

@@ -23,5 +23,23 @@ void check_rows(Device& d, const void* pointer, uint64_t rows, uint64_t stride, 
 void attend_kv8(Device& d, const std::vector<Sequence>& sequences, uint64_t heads, uint64_t kv_heads, uint64_t dim, int code, float scale,
                 float cap, const float* slopes, uint64_t window, const void* q, uint64_t q_stride, void* out, uint64_t out_stride, int type);
 
+#if defined(__CUDACC__)
+// tanh(y) in two forms. Up to |y| = 1/4 the odd series to y^9: the next term is below 2^-28 of y, and it runs on the FMA pipe alone. For any y
+// 1 - 2 / (1 + e^(2y)): off by 2^-22 at most (an exponential and a reciprocal of 2^-22 and 2^-23 each).
+constexpr float kSmallTanh = 0.25f;
+__device__ __forceinline__ float small_tanh(float y) {
+    const float z = y * y;
+    float p = fmaf(z, 62.0f / 2835.0f, -17.0f / 315.0f);
+    p = fmaf(p, z, 2.0f / 15.0f);
+    p = fmaf(p, z, -1.0f / 3.0f);
+    return fmaf(p * z, y, y);
+}
+__device__ __forceinline__ float any_tanh(float y) {
+    float r;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(1.0f + fast_exp2(y * 2.8853900817779268f)));
+    return fmaf(-2.0f, r, 1.0f);
+}
+#endif
+
 }  // namespace attn
 }  // namespace sdb
