@@ -14,15 +14,15 @@
 // tiles and its output). A block walks its run without stopping: the next unit's first products are issued while the last one's output is written. A unit that
 // two or more blocks share leaves FP32 partials for a second kernel. (A block a unit left the last of 1.7 waves a third empty for a chunk of 2048
 // rows, 285 us, and spent half of 184 us on first loads and outputs for packed documents of 8 tiles a unit.)
-// Warps: 0-3 and 4-7 softmax, a thread a row (half a row with 256 columns); 8 issues the products; 9 the TMA loads; 10-11 look after values that
-// some row may not see (below).
+// Warps: 0-3 and 4-7 softmax, a thread a row (half a row with 256 columns); 8 and 9 issue the products of a query tile each; 10 the TMA loads; 11
+// looks after values that some row may not see (below).
 //
 // Roundings: scores, maxima, sums and O are FP32. P is rounded to the operands' type once (FP16 or BF16), at 2^7 times its size so that FP16 keeps
 // 11 bits down to 2^-21 of the largest weight. O is multiplied in TMEM only when a row's maximum grew by more than 2^8. The keys' scales of an 8-bit
 // state multiply the scores, a block of 32 a factor; the values' scales, relative to the largest of the K/V head, join the exponent of P.
 //
-// A weight of 0 times a value that is infinite or NaN is NaN. In tiles where some row does not see some key (the diagonal, a border), two warps
-// replace such values by 0 before the product reads them; the rows that do see them get them back at the end. What no row sees does not reach it.
+// A weight of 0 times a value that is infinite or NaN is NaN. In tiles where some row does not see some key (the diagonal, a border), a warp
+// replaces such values by 0 before the product reads them; the rows that do see them get them back at the end. What no row sees does not reach it.
 #include "kv8.cuh"
 #include "masked_attention.cuh"
 #include "../../include/straydog_gpu_b200.h"
@@ -33,24 +33,24 @@
 namespace sdb {
 namespace attn {
 
-constexpr int kThreads = 384, kTileKeys = 128, kM = 128;
-constexpr int kIssueWarp = 8, kLoadWarp = 9, kLookWarp = 10;
+constexpr int kThreads = 384, kM = 128, kStep = 64;   // kStep: keys of a step, what the softmax works on at a time
+constexpr int kIssueWarp = 8, kLoadWarp = 10, kLookWarp = 11;   // (one or two issuing warps, a query tile each)
 constexpr float kLift = 7.0f, kRescale = 8.0f;
 constexpr unsigned kSequences = 64;   // sequences a launch
 constexpr int kFlagged = 16;          // slots of one piece that are looked at for values that are not finite (borders: at most a dozen)
 
 template<int D> struct Shape {
-    static constexpr int kTiles = D == 256 ? 1 : 2;                  // query tiles a unit
-    static constexpr int kSlotKeys = D == 256 ? 64 : 128;            // keys of a ring slot: 32 KB (16 KB for 64 columns)
-    static constexpr int kHalves = kTileKeys / kSlotKeys;            // slots of a key tile
-    static constexpr int kSlots = D == 256 ? 5 : 4;
-    static constexpr int kSlotBytes = kSlotKeys * D * 2, kQueryBytes = kM * D * 2;
-    static constexpr int kOffRing = kTiles * kQueryBytes, kOffBars = kOffRing + kSlots * kSlotBytes;
-    static constexpr int kOffFlags = kOffBars + 256, kOffStats = kOffFlags + kFlagged * 32;
+    static constexpr int kTiles = D == 256 ? 1 : 2;                   // query tiles a unit
+    static constexpr int kKSlots = D == 256 ? 3 : 5, kVSlots = D == 256 ? 4 : 5;   // two rings in shared memory, a step's keys or values a slot
+    static constexpr int kSlotBytes = kStep * D * 2, kQueryBytes = kM * D * 2;
+    static constexpr bool kQInTmem = D == 256;                        // (64 KB that K and V need more; and it is read twice as fast there)
+    static constexpr int kOffK = kQInTmem ? 0 : kTiles * kQueryBytes, kOffV = kOffK + kKSlots * kSlotBytes, kOffBars = kOffV + kVSlots * kSlotBytes;
+    static constexpr int kOffFlags = kOffBars + 512, kOffStats = kOffFlags + kFlagged * 32;
     static constexpr int kSlack = kTiles == 1 ? 0 : 1024;             // to align the base to 1024 bytes where there is room (the runtime aligns it anyway)
     static constexpr size_t kSmem = kOffStats + (kTiles == 1 ? 2 * 2 * kM * 4 : 0) + kSlack;
     static_assert(kSmem <= 227 * 1024, "shared memory");
-    static constexpr int kS = 0, kO = 256;                           // TMEM columns: S of tile (or buffer) b at 128 b, O of tile b at 256 + D b
+    static constexpr int kO = 256, kQ = 128;                          // TMEM columns: two S buffers a tile from 0, Q of 256 columns at 128, O of tile t at 256 + D t
+    static __device__ __forceinline__ uint32_t scores(int tile, int buffer) { return tile * 128 + buffer * kStep; }
 };
 
 struct KernelSequence {
@@ -63,7 +63,7 @@ struct Args {
     CUtensorMap q_map, k_map, v_map;
     KernelSequence sequence[kSequences];
     uint32_t sequences, heads, kv_heads, group, tokens;   // tokens: rows of a query tile
-    uint32_t window, shares, zero;   // zero: 0, unknown to the compiler
+    uint32_t window, shares;
     Cut cut[kMostBlocks + 1];
     Shared share[kMostBlocks];
     void* out;
@@ -73,6 +73,8 @@ struct Args {
     const float* block_table;    // 8-bit states: [kv_heads][tiles of four blocks of 32 keys][12]: four key scales, then log2 and inverse of four value scales over the head's largest
     const float* value_top;      // 8-bit states: [sequence][kv_heads] the largest value scale
     uint32_t table_blocks;
+    const uint16_t* queries;     // the query rows again, where they do not come through the map
+    size_t query_stride;
     const uint16_t* values;      // 16-bit rows: the values again, for the rows that see one that is not finite
     size_t value_stride;
     float scale_log2, cap, scale_over_cap;
@@ -81,7 +83,9 @@ struct Args {
     int* status;
 };
 
-enum { kQFull = 0, kSFull = 1, kPFull = 3, kPvDone = 5, kLook = 7, kClean = 8, kQFree = 9, kOFree = 10, kRing = 12 };   // barriers: then full and free of every slot
+// Barriers: S, P and the value product of (tile, buffer), values looked at, Q, O of a tile, the rings' slots. A barrier tells a phase from its
+// neighbours only: whoever waits for one has to know that the phase before is over and that the one after cannot be.
+enum { kQFull = 0, kSFull = 1, kPFull = 5, kPvDone = 9, kLook = 13, kClean = 14, kQFree = 15, kOFree = 16, kKFull = 18, kKFree = 23, kVFull = 28, kVFree = 33, kBars = 38 };
 
 constexpr uint32_t kDescHigh = 0x40004040u;   // 128-byte swizzle, 1024 bytes between groups of 8 rows (see csrc/qsa_prompt_tc.cu)
 __device__ __forceinline__ uint32_t desc_low(uint32_t address, uint32_t leading_bytes) { return ((address & 0x3ffffu) >> 4) | ((leading_bytes >> 4) << 16); }
@@ -106,6 +110,11 @@ __device__ __forceinline__ void umma_a_tmem(uint32_t d_tmem, uint32_t a_tmem, ui
 }
 __device__ __forceinline__ void umma_commit(uint64_t* bar) {
     asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ bool elect_one() {
+    uint32_t pred;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(pred));
+    return pred != 0;
 }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -142,6 +151,44 @@ __device__ __forceinline__ void tma_load(void* to, const CUtensorMap* map, int x
                  ::"r"(smem_u32(to)), "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar)) : "memory");
 }
 
+// two FP32 operations an instruction
+__device__ __forceinline__ uint64_t pair(float x, float y) {
+    uint64_t p;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(p) : "f"(x), "f"(y));
+    return p;
+}
+__device__ __forceinline__ void unpair(uint64_t p, float& x, float& y) { asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(p)); }
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ uint64_t both(float x) { return pair(x, x); }
+// small_tanh of two numbers
+__device__ __forceinline__ uint64_t small_tanh2(uint64_t y) {
+    const uint64_t z = mul2(y, y);
+    uint64_t p = fma2(z, both(-17.0f / 315.0f), both(2.0f / 15.0f));
+    p = fma2(p, z, both(-1.0f / 3.0f));
+    return fma2(mul2(p, z), y, y);
+}
+// of two pairs of 16-bit floats, the larger magnitudes; a NaN if either is
+template<bool BF16> __device__ __forceinline__ uint32_t largest(uint32_t a, uint32_t b) {
+    uint32_t d;
+    a &= 0x7fff7fffu; b &= 0x7fff7fffu;
+    if (BF16) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    else asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
 // the low `count` bits set (none below 0, all from 32 on)
 __device__ __forceinline__ uint32_t first_bits(int count) { return count <= 0 ? 0u : count >= 32 ? 0xffffffffu : (1u << count) - 1u; }
 __device__ __forceinline__ float max3(float a, float b, float c) {   // (as fmaxf: a NaN is no maximum)
@@ -178,17 +225,17 @@ struct Unit {
         last = length - int(q.rows) + int(end) - 1;
         const int causal = last + 1, reach = causal > prefix ? causal : prefix;
         const uint32_t low = a.window && first >= int(a.window) ? uint32_t(first - int(a.window) + 1) : 0u;
-        const uint32_t all = uint32_t((reach > 0 ? reach : 0) + kTileKeys - 1) / kTileKeys;
-        head_tiles = uint32_t(prefix + kTileKeys - 1) / kTileKeys;
-        uint32_t body = low / kTileKeys > head_tiles ? low / kTileKeys : head_tiles;
+        const uint32_t all = uint32_t((reach > 0 ? reach : 0) + kStep - 1) / kStep;
+        head_tiles = uint32_t(prefix + kStep - 1) / kStep;
+        uint32_t body = low / kStep > head_tiles ? low / kStep : head_tiles;
         if (body > all) body = all;
         jump = body - head_tiles;
         tiles = all - jump;
     }
-    __device__ __forceinline__ uint32_t key(uint32_t tile) const { return (tile < head_tiles ? tile : tile + jump) * kTileKeys; }
+    __device__ __forceinline__ uint32_t key(uint32_t tile) const { return (tile < head_tiles ? tile : tile + jump) * kStep; }
     // whether every row of the unit sees every key of the tile at key0
     __device__ __forceinline__ bool open(const Args& a, uint32_t key0) const {
-        const int end_key = int(key0) + kTileKeys - 1;
+        const int end_key = int(key0) + kStep - 1;
         return (end_key <= first && end_key < length && (!a.window || int(key0) > last - int(a.window))) || end_key < prefix;
     }
 };
@@ -226,7 +273,7 @@ template<int ROWS> struct Run {
 template<int D, bool BF16, bool RULE>
 __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __grid_constant__ Args a) {
     using S = Shape<D>;
-    constexpr int T = S::kTiles, kGroups = T == 2 ? 4 : 2;   // a softmax thread's groups of 32 columns of S
+    constexpr int T = S::kTiles, kGroups = T;   // a softmax thread's groups of 32 columns of S
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     if (!S::kSlack && smem_u32(smem_raw) % 1024) {   // (no operand layout without it: reported, not computed)
         if (threadIdx.x == 0) atomicExch(a.status, 1);
@@ -234,8 +281,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
     }
     uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
     uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::kOffBars);
-    constexpr int kFull = kRing, kFree = kRing + S::kSlots, kBars = kRing + 2 * S::kSlots;
-    static_assert(kBars * 8 + 16 <= 256, "barriers");
+    static_assert(kBars * 8 + 16 <= S::kOffFlags - S::kOffBars, "barriers");
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + kBars);
     volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
     volatile uint32_t* flagged_piece = tmem_slot + 2;                       // the piece (counted from 1) that `flagged` belongs to
@@ -245,7 +291,8 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     if (tid == 0) {
         for (int i = 0; i < kBars; ++i)
-            mbar_init(&bars[i], i == kPFull || i == kPFull + 1 || i == kOFree || i == kOFree + 1 ? (T == 2 ? 4 : 8) : i == kClean ? 2 : 1);
+            mbar_init(&bars[i], (i >= kPFull && i < kPFull + 4) || i == kOFree || i == kOFree + 1 ? (T == 2 ? 4 : 8) : i == kQFull ? (S::kQInTmem ? 8 : 1) :
+                                i == kLook || i == kQFree || (i >= kKFree && i < kVFull) || i >= kVFree ? T : 1);
         *abort_flag = 0;
         *flagged_piece = 0;
     }
@@ -273,12 +320,14 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
     };
     Run<T> run;
     bool alive = true;
-    uint32_t done = 0;    // key tiles of the pieces before (each role counts for itself: the barriers' parities follow it)
-    uint32_t piece = 0;   // pieces with tiles before
+    uint32_t done = 0;            // steps of the pieces before (each role counts for itself: the barriers' parities follow these)
+    uint32_t used[2] = {0, 0};    // uses of the two S buffers by the pieces before (a piece's step i takes buffer i % 2)
+    uint32_t piece = 0;           // pieces with steps before
 
     if (warp < 8) {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 208;");   // (8 warps x 208 and 4 x 88: what 12 are launched with at 168)
         // ================= softmax: a thread a row (T 2: a warpgroup a query tile), or half a row (T 1: a warpgroup a half of the columns) =================
+        uint32_t next_queries = 0;
         const int tile_of = T == 2 ? warp / 4 : 0, half = T == 2 ? 0 : warp / 4, m = (warp & 3) * 32 + lane;
         const uint32_t lane_base = tmem + (uint32_t((warp & 3) * 32) << 16);
         constexpr int kOColumns = T == 2 ? D : D / 2;                          // a thread's columns of O
@@ -298,7 +347,35 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
             return any != 0;
         };
         uint32_t turn = 0;
-        for (bool more = run.start(a); more && alive; more = run.next(a)) {
+        // 256 columns: the queries of the next piece that has steps go to TMEM as soon as the scores before are done, ahead of the outputs
+        auto bring_queries = [&](Run<T> next, bool more) {
+            while (more && next.begin == next.end) more = next.next(a);
+            if (!more || !alive) return;
+            if (next_queries && !wait(kQFree, (next_queries - 1) & 1)) { alive = false; return; }
+            ++next_queries;
+            fence_after();
+            const KernelSequence& sequence = a.sequence[next.u.s];
+            const uint32_t token = next.u.row + m / a.group, head = next.u.kv * a.group + m % a.group;
+            const bool real = token < sequence.rows && uint32_t(m) < a.tokens * a.group;
+            const uint4* from = reinterpret_cast<const uint4*>(a.queries + (real ? (size_t(sequence.first_row) + token) * a.query_stride + size_t(head) * D + half * (D / 2) : 0));
+            #pragma unroll 1
+            for (int b = 0; b < D / 2 / 64; ++b) {
+                uint32_t w[32];
+                #pragma unroll
+                for (int n = 0; n < 8; ++n) {
+                    const uint4 v = real ? __ldg(from + 8 * b + n) : make_uint4(0, 0, 0, 0);
+                    w[4 * n] = v.x; w[4 * n + 1] = v.y; w[4 * n + 2] = v.z; w[4 * n + 3] = v.w;
+                }
+                tmem_store32(lane_base + S::kQ + half * (D / 4) + 32 * b, w);
+            }
+            tmem_store_wait();
+            fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&bars[kQFull]);
+        };
+        bool more = run.start(a);
+        if (S::kQInTmem) bring_queries(run, more);
+        for (; more && alive; more = run.next(a)) {
             const Unit& u = run.u;
             const KernelSequence& sequence = a.sequence[u.s];
             const uint32_t tiles = run.end - run.begin;
@@ -306,61 +383,83 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
             const bool valid = token < sequence.rows && uint32_t(m) < a.tokens * a.group;
             const int position = u.length - int(sequence.rows) + int(token);
             const float slope = RULE && a.slopes && valid ? a.slopes[head] * 1.4426950408889634f : 0.0f;
-            // 8-bit states: a tile's factors are 12 floats, [scores' | weights' log2 | sums'] x [four groups of 32 keys]; a thread has kGroups of each
-            const float* table_at = a.block_table ? a.block_table + (size_t(u.kv) * a.table_blocks + sequence.first_block) * 3 + half * 2 : nullptr;
+            // 8-bit states: a tile's factors are 12 floats, [scores' | weights' log2 | sums'] x [four groups of 32 keys]
+            const float* table_at = a.block_table ? a.block_table + (size_t(u.kv) * a.table_blocks + sequence.first_block) * 3 + half : nullptr;
             float top_run = -INFINITY, sum_run = 0.0f;
             #pragma unroll 1
             for (uint32_t i = 0; i < tiles; ++i) {
-                const uint32_t key0 = u.key(run.begin + i), it = done + i;
-                const int buffer = T == 2 ? tile_of : int(it & 1);
+                const uint32_t key0 = u.key(run.begin + i);
+                const int buffer = int(i & 1), ready = 2 * tile_of + buffer;
                 float to_score[kGroups], shift[kGroups], to_sum[kGroups];
                 #pragma unroll
                 for (int g = 0; g < kGroups; ++g) { to_score[g] = 1.0f; shift[g] = 0.0f; to_sum[g] = 1.0f; }
                 if (table_at) {
-                    const float* table = table_at + key0 / 32 * 3;
+                    const float* table = table_at + key0 / 128 * 12 + key0 / 64 % 2 * 2;
                     #pragma unroll
-                    for (int g = 0; g < kGroups; g += 2) {
-                        const float2 x = __ldg(reinterpret_cast<const float2*>(table + g)), y = __ldg(reinterpret_cast<const float2*>(table + 4 + g)),
-                                     z = __ldg(reinterpret_cast<const float2*>(table + 8 + g));
-                        to_score[g] = x.x; to_score[g + 1] = x.y; shift[g] = y.x; shift[g + 1] = y.y; to_sum[g] = z.x; to_sum[g + 1] = z.y;
-                    }
+                    for (int g = 0; g < kGroups; ++g) { to_score[g] = __ldg(table + g); shift[g] = __ldg(table + 4 + g); to_sum[g] = __ldg(table + 8 + g); }
                 }
-                if (!wait(kSFull + buffer, T == 2 ? it & 1 : (it >> 1) & 1)) { alive = false; break; }
+                if (!wait(kSFull + ready, (used[buffer] + (i >> 1)) & 1)) { alive = false; break; }
                 fence_after();
-                const uint32_t s_base = lane_base + S::kS + buffer * 128 + half * 64;
+                const uint32_t s_base = lane_base + S::scores(tile_of, buffer) + half * 32;
                 const bool open = u.open(a, key0);
                 // Weights are computed from the maximum so far, in one pass over the scores that finds the tile's own on the way. Where that is above by
                 // more than 2^8, where there is none yet, and in tiles with a mask, a cap or a bias, the scores are finished and the maximum found
                 // first, O is multiplied, and the pass runs over what went back to TMEM.
-                bool first = i == 0 || !open || RULE;
+                bool first = i == 0 || !open;
                 if (!first) {
                     const float under = top_run == -INFINITY ? 0.0f : top_run - kLift;
                     uint32_t packed[16 * kGroups];
-                    float top = -INFINITY, sum = 0.0f;
+                    float top = -INFINITY, sum = 0.0f, steep = 0.0f;
                     #pragma unroll
                     for (int g = 0; g < kGroups; ++g) {
                         uint32_t bits[32];
-                        // (the address waits for the weights before: loads moved further up would take the registers of all groups at once)
-                        tmem_load32(s_base + 32 * g + (g ? packed[16 * g - 1] & a.zero : 0u), bits);
-                        const float c = a.scale_log2 * to_score[g], d = shift[g] - under;
+                        tmem_load32(s_base + 32 * g, bits);
+                        const float d = shift[g] - under;
+                        float c = a.scale_log2 * to_score[g];
                         tmem_load_wait(bits);
-                        float sum0 = 0.0f, sum1 = 0.0f, most = -INFINITY;
+                        if (RULE && a.cap > 0.0f) {   // cap * tanh(s / cap), the cap (in the exp2 domain) kept for the exponent's argument
+                            const float inner = a.scale_over_cap * to_score[g];
+                            const uint64_t inner2 = pair(inner, inner);
+                            #pragma unroll
+                            for (int n = 0; n < 16; ++n) {
+                                const uint64_t y = mul2(pair(__uint_as_float(bits[2 * n]), __uint_as_float(bits[2 * n + 1])), inner2);
+                                float y0, y1;
+                                unpair(y, y0, y1);
+                                steep = max3(steep, fabsf(y0), fabsf(y1));
+                                unpair(small_tanh2(y), y0, y1);
+                                bits[2 * n] = __float_as_uint(y0); bits[2 * n + 1] = __float_as_uint(y1);
+                            }
+                            c = a.cap;
+                        }
+                        if (RULE && a.slopes) {
+                            const float from = float(position - int(key0) - half * 32 - 32 * g);
+                            #pragma unroll
+                            for (int n = 0; n < 32; ++n) bits[n] = __float_as_uint(fmaf(-slope, fabsf(from - float(n)), __uint_as_float(bits[n]) * c));
+                            c = 1.0f;
+                        }
+                        const uint64_t c2 = pair(c, c), d2 = pair(d, d);
+                        uint64_t sums = pair(0.0f, 0.0f);
+                        float most = -INFINITY;
                         #pragma unroll
                         for (int n = 0; n < 16; ++n) {
-                            const float x0 = fmaf(__uint_as_float(bits[2 * n]), c, d), x1 = fmaf(__uint_as_float(bits[2 * n + 1]), c, d);
+                            const uint64_t x = fma2(pair(__uint_as_float(bits[2 * n]), __uint_as_float(bits[2 * n + 1])), c2, d2);
+                            float x0, x1;
+                            unpair(x, x0, x1);
                             most = max3(most, x0, x1);
-                            const float p0 = fast_exp2(x0), p1 = fast_exp2(x1);
-                            packed[16 * g + n] = BF16 ? pack_bf16x2(p0, p1) : pack_half2(p0, p1);
-                            sum0 += p0; sum1 += p1;
+                            x0 = fast_exp2(x0); x1 = fast_exp2(x1);
+                            sums = add2(sums, pair(x0, x1));
+                            packed[16 * g + n] = BF16 ? pack_bf16x2(x0, x1) : pack_half2(x0, x1);
                         }
+                        float sum0, sum1;
+                        unpair(sums, sum0, sum1);
                         top = fmaxf(top, most - shift[g]);
                         sum = fmaf(sum0 + sum1, to_sum[g], sum);
                     }
-                    first = any_of_rows(top > (top_run == -INFINITY ? -INFINITY : kLift + kRescale));
+                    first = any_of_rows(top > (top_run == -INFINITY ? -INFINITY : kLift + kRescale) || (RULE && steep > kSmallTanh));
                     if (!first) {
                         sum_run += sum;
-                        #pragma unroll
-                        for (int h = 0; h < kGroups / 2; ++h) tmem_store32(s_base + 64 * h, packed + 32 * h);   // (over scores that have been read)
+                        // (over scores that have been read)
+                        if constexpr (T == 2) tmem_store32(s_base, packed); else tmem_store16(s_base, packed);
                     }
                 }
                 if (first) {
@@ -398,14 +497,14 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
                             c *= a.scale_log2;
                         }
                         if (RULE && a.slopes) {
-                            const float from = float(position - int(key0) - half * 64 - 32 * g);
+                            const float from = float(position - int(key0) - half * 32 - 32 * g);
                             #pragma unroll
                             for (int n = 0; n < 32; ++n) bits[n] = __float_as_uint(fmaf(-slope, fabsf(from - float(n)), __uint_as_float(bits[n]) * c));
                             c = 1.0f;
                         }
                         if (!open) {
                             // a bit a column: keys up to `to` and above `low`, or below `prefix`, relative to the group
-                            const int base = int(key0) + half * 64 + 32 * g;
+                            const int base = int(key0) + half * 32 + 32 * g;
                             const int to = min(position, u.length - 1) - base, low = a.window ? position - int(a.window) - base : -1, prefix = u.prefix - base;
                             uint32_t seen = (first_bits(to + 1) & ~first_bits(low + 1)) | first_bits(prefix);
                             if (!valid) seen = 0;
@@ -424,7 +523,8 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
                     const bool grow = top > top_run + kRescale || (top_run == -INFINITY && top > -INFINITY);
                     const float use = grow ? top : top_run;
                     if (i > 0 && __any_sync(0xffffffffu, grow && top_run != -INFINITY)) {
-                        if (!wait(kPvDone + tile_of, (it - 1) & 1)) { alive = false; break; }
+                        // (the products two steps back were over before these scores were made)
+                        if (!wait(kPvDone + 2 * tile_of + (buffer ^ 1), (used[buffer ^ 1] + ((i - 1) >> 1)) & 1)) { alive = false; break; }
                         fence_after();
                         const float factor = grow && top_run != -INFINITY ? fast_exp2(top_run - use) : 1.0f;
                         #pragma unroll 1
@@ -455,20 +555,24 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
                             sum0 += p0; sum1 += p1;
                         }
                         sum_run = fmaf(sum0 + sum1, of(to_sum, g), sum_run);
-                        tmem_store16(s_base + 64 * (g / 2) + 16 * (g % 2), bits);
+                        tmem_store16(s_base + 16 * g, bits);
                     }
                 }
                 tmem_store_wait();
                 fence_before();
                 __syncwarp();
-                if (lane == 0) mbar_arrive(&bars[kPFull + buffer]);
+                if (lane == 0) mbar_arrive(&bars[kPFull + ready]);
             }
             if (!alive) break;
             // ---- O / sum ----
-            // (T 1: the last scores were issued behind all products but the last two: both are waited for in turn, a barrier's parity tells
-            //  neighbouring phases apart only)
-            if (T == 1 && tiles > 1 && !wait(kPvDone, (done + tiles - 2) & 1)) { alive = false; break; }
-            if (tiles && !wait(kPvDone + tile_of, (done + tiles - 1) & 1)) { alive = false; break; }
+            if (S::kQInTmem && tiles) {
+                Run<T> next = run;
+                const bool any = next.next(a);
+                bring_queries(next, any);
+                if (!alive) break;
+            }
+            // (the last product is over when all are)
+            if (tiles && !wait(kPvDone + 2 * tile_of + int(tiles - 1 & 1), (used[tiles - 1 & 1] + ((tiles - 1) >> 1)) & 1)) { alive = false; break; }
             fence_after();
             if (T == 1) sum_run += other_half(sum_run, turn++);
             const float lift = a.value_top ? a.value_top[u.s * a.kv_heads + u.kv] : 1.0f;
@@ -493,7 +597,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
                     // values that were taken out of a tile: back for the rows that see them (rare: nothing here is fast)
                     for (int p = 0; p < kFlagged; ++p) {
                         const int base = int(flagged[8 * p]);
-                        for (int n = 0; n < S::kSlotKeys; ++n) {
+                        for (int n = 0; n < kStep; ++n) {
                             if (!(flagged[8 * p + 1 + n / 32] >> (n % 32) & 1)) continue;
                             const int key = base + n;
                             const bool seen = key < u.length && ((key <= position && (!a.window || key > position - int(a.window))) || key < u.prefix);
@@ -530,94 +634,73 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
             if (patches) leave();
             if (tiles) {
                 ++piece;
-                done += tiles;
+                used[0] += (tiles + 1) / 2; used[1] += tiles / 2;
             }
         }
     } else {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;");
-        const uint32_t ring = smem_u32(smem + S::kOffRing);
-        // The ring's order within a piece, for all roles below: K of the first tile (of two tiles with 256 columns), then V of tile i and K of a later one.
-        constexpr uint32_t kAhead = T == 2 ? 1 : 2;
-        uint32_t items = 0;   // slots used by the pieces before
-        if (warp == kIssueWarp) {
-            // ================= the products =================
-            if (lane == 0) {
-                const uint32_t idesc_s = instr_desc(kM, S::kSlotKeys, BF16, false), idesc_o = instr_desc(kM, D, BF16, true);
-                const uint32_t queries = smem_u32(smem);
-                uint32_t looked = 0;
-                auto score = [&](int tile, int buffer, uint32_t first_item) -> bool {
-                    for (int h = 0; h < S::kHalves; ++h) {
-                        const uint32_t at = items + first_item + h, slot = at % S::kSlots;
-                        if (!wait(kFull + slot, (at / S::kSlots) & 1)) return false;
-                        fence_after();
-                        const uint32_t b = desc_low(ring + slot * S::kSlotBytes, 16), q = desc_low(queries + tile * S::kQueryBytes, 16);
-                        #pragma unroll
-                        for (int kk = 0; kk < D / 16; ++kk)
-                            umma(tmem + S::kS + buffer * 128 + h * S::kSlotKeys, desc_of(q + (((kk / 4) * (kM * 128) + (kk % 4) * 32) >> 4)),
-                                 desc_of(b + (((kk / 4) * (S::kSlotKeys * 128) + (kk % 4) * 32) >> 4)), idesc_s, kk > 0);
-                        if (T == 1 || tile == 1) umma_commit(&bars[kFree + slot]);
+        constexpr uint32_t kAhead = 2;   // score products issued ahead of the value products
+        if (warp == kIssueWarp || (T == 2 && warp == kIssueWarp + 1)) {
+            // ================= the products of a query tile =================
+            // The whole warp walks, one elected lane issues: addresses and descriptors stay in uniform registers, which the instruction takes. (One
+            // thread walking alone moved every operand there, 70 cycles a product, and was what bound the kernel.)
+            const int tile = warp - kIssueWarp;
+            const bool leader = elect_one();
+            const uint32_t idesc_o = instr_desc(kM, D, BF16, true);
+            const uint32_t tmem_base = __shfl_sync(0xffffffffu, tmem, 0), base = __shfl_sync(0xffffffffu, smem_u32(smem), 0);
+            const uint32_t queries = desc_low(base + tile * S::kQueryBytes, 16);
+            uint32_t looked = 0;
+            const uint32_t idesc_s = instr_desc(kM, kStep, BF16, false);
+            auto score = [&](uint32_t i, uint32_t tiles) -> bool {
+                const uint32_t at = done + i, slot = at % S::kKSlots;
+                if (!wait(kKFull + slot, (at / S::kKSlots) & 1)) return false;
+                fence_after();
+                const int buffer = int(i & 1);
+                const uint32_t k = desc_low(base + S::kOffK + slot * S::kSlotBytes, 16), d = tmem_base + S::scores(tile, buffer);
+                if (leader) {
+                    #pragma unroll
+                    for (int kk = 0; kk < D / 16; ++kk) {
+                        const uint64_t k_desc = desc_of(k + (((kk / 4) * (kStep * 128) + (kk % 4) * 32) >> 4));
+                        if (S::kQInTmem) umma_a_tmem(d, tmem_base + S::kQ + kk * 8, k_desc, idesc_s, kk > 0);
+                        else umma(d, desc_of(queries + (((kk / 4) * (kM * 128) + (kk % 4) * 32) >> 4)), k_desc, idesc_s, kk > 0);
                     }
-                    umma_commit(&bars[kSFull + buffer]);
-                    return true;
-                };
-                for (bool more = run.start(a); more && alive; more = run.next(a)) {
-                    const uint32_t tiles = run.end - run.begin;
-                    if (!tiles) continue;
-                    if (!wait(kQFull, piece & 1)) { alive = false; break; }
-                    const uint32_t ahead = min(kAhead, tiles);
-                    // K tiles: the first `ahead` at items 0 .., K(i) for i >= kAhead behind V(i - kAhead)
-                    auto k_item = [&](uint32_t i) -> uint32_t { return (i < kAhead ? i : 2 * i + 1 - kAhead) * S::kHalves; };
-                    for (uint32_t f = 0; f < ahead && alive; ++f) {
-                        if (T == 2) { alive = alive && score(0, 0, 0); alive = alive && score(1, 1, 0); }
-                        else alive = alive && score(0, int((done + f) & 1), k_item(f));
-                    }
-                    if (alive && tiles <= kAhead) umma_commit(&bars[kQFree]);
-                    #pragma unroll 1
-                    for (uint32_t i = 0; i < tiles && alive; ++i) {
-                        const bool look = a.values && !run.u.open(a, run.u.key(run.begin + i));
-                        const uint32_t item = items + (ahead + i + min(i, tiles - ahead)) * S::kHalves, it = done + i;   // V(i)
-                        if (i == 0 && piece) {   // the outputs of the piece before have left O (and `flagged`)
-                            for (int tile = 0; tile < T && alive; ++tile) alive = wait(kOFree + tile, (piece - 1) & 1);
-                            if (!alive) break;
-                        }
-                        if (look) {   // (the tile's values are there: they are looked at while the softmax runs)
-                            for (int h = 0; h < S::kHalves && alive; ++h) alive = wait(kFull + (item + h) % S::kSlots, ((item + h) / S::kSlots) & 1);
-                            if (!alive) break;
-                            mbar_arrive(&bars[kLook]);
-                        }
-                        #pragma unroll 1
-                        for (int tile = 0; tile < T && alive; ++tile) {
-                            const int buffer = T == 2 ? tile : int(it & 1);
-                            if (!wait(kPFull + buffer, T == 2 ? it & 1 : (it >> 1) & 1)) { alive = false; break; }
-                            for (int h = 0; h < S::kHalves && alive; ++h) {
-                                const uint32_t slot = (item + h) % S::kSlots;
-                                if (tile == 0) {
-                                    if (!wait(kFull + slot, ((item + h) / S::kSlots) & 1)) { alive = false; break; }
-                                    if (look && h == 0) {
-                                        if (!wait(kClean, looked & 1)) { alive = false; break; }
-                                        ++looked;
-                                    }
-                                }
-                                fence_after();
-                                const uint32_t v = desc_low(ring + slot * S::kSlotBytes, S::kSlotKeys * 128);
-                                #pragma unroll
-                                for (int kk = 0; kk < S::kSlotKeys / 16; ++kk)
-                                    umma_a_tmem(tmem + S::kO + tile * D, tmem + S::kS + buffer * 128 + (h * S::kSlotKeys + kk * 16) / 64 * 64 + (h * S::kSlotKeys + kk * 16) % 64 / 2,
-                                                desc_of(v + ((kk * (16 * 128)) >> 4)), idesc_o, i > 0 || h > 0 || kk > 0);
-                                if (T == 1 || tile == 1) umma_commit(&bars[kFree + slot]);
-                            }
-                            if (!alive) break;
-                            umma_commit(&bars[kPvDone + tile]);
-                            if (i + kAhead < tiles) {
-                                alive = score(tile, buffer, k_item(i + kAhead));
-                                if (alive && tile == T - 1 && i + kAhead + 1 == tiles) umma_commit(&bars[kQFree]);
-                            }
-                        }
-                    }
-                    items += 2 * tiles * S::kHalves;
-                    done += tiles;
-                    ++piece;
+                    umma_commit(&bars[kSFull + 2 * tile + buffer]);
+                    umma_commit(&bars[kKFree + slot]);
+                    if (i + 1 == tiles) umma_commit(&bars[kQFree]);
                 }
+                return true;
+            };
+            for (bool more = run.start(a); more && alive; more = run.next(a)) {
+                const uint32_t tiles = run.end - run.begin;
+                if (!tiles) continue;
+                if (!wait(kQFull, piece & 1)) { alive = false; break; }
+                fence_after();
+                for (uint32_t f = 0; f < kAhead && f < tiles && alive; ++f) alive = score(f, tiles);
+                #pragma unroll 1
+                for (uint32_t i = 0; i < tiles && alive; ++i) {
+                    const bool look = a.values && !run.u.open(a, run.u.key(run.begin + i));
+                    const uint32_t at = done + i, slot = at % S::kVSlots;
+                    const int buffer = int(i & 1);
+                    // the outputs of the piece before have left O (and `flagged`)
+                    if (i == 0 && piece && !wait(kOFree + tile, (piece - 1) & 1)) { alive = false; break; }
+                    if (!wait(kVFull + slot, (at / S::kVSlots) & 1)) { alive = false; break; }
+                    if (look && leader) mbar_arrive(&bars[kLook]);   // (the step's values are looked at while the softmax runs)
+                    if (!wait(kPFull + 2 * tile + buffer, (used[buffer] + (i >> 1)) & 1)) { alive = false; break; }
+                    if (look && !wait(kClean, looked++ & 1)) { alive = false; break; }
+                    fence_after();
+                    const uint32_t v = desc_low(base + S::kOffV + slot * S::kSlotBytes, kStep * 128), p = tmem_base + S::scores(tile, buffer), o = tmem_base + S::kO + tile * D;
+                    if (leader) {
+                        #pragma unroll
+                        for (int kk = 0; kk < kStep / 16; ++kk)
+                            umma_a_tmem(o, p + (T == 2 ? kk * 8 : kk / 2 * 32 + kk % 2 * 8), desc_of(v + ((kk * (16 * 128)) >> 4)), idesc_o, i > 0 || kk > 0);
+                        umma_commit(&bars[kPvDone + 2 * tile + buffer]);
+                        umma_commit(&bars[kVFree + slot]);
+                    }
+                    if (i + kAhead < tiles) alive = score(i + kAhead, tiles);
+                }
+                done += tiles;
+                used[0] += (tiles + 1) / 2; used[1] += tiles / 2;
+                ++piece;
             }
         } else if (warp == kLoadWarp) {
             // ================= the loads =================
@@ -626,81 +709,88 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
                     const uint32_t tiles = run.end - run.begin;
                     if (!tiles) continue;
                     const KernelSequence& sequence = a.sequence[run.u.s];
-                    if (piece && !wait(kQFree, (piece - 1) & 1)) { alive = false; break; }
-                    mbar_expect_tx(&bars[kQFull], uint32_t(T * (D / 64)) * a.tokens * a.group * 128);
-                    #pragma unroll 1
-                    for (int tile = 0; tile < T; ++tile)
-                        for (int x = 0; x < D / 64; ++x)
-                            tma_load(smem + tile * S::kQueryBytes + x * (kM * 128), &a.q_map, 64 * x, int(run.u.kv * a.group),
-                                     int(sequence.first_row + run.u.row + tile * a.tokens), &bars[kQFull]);
-                    auto load = [&](const CUtensorMap& map, uint32_t i) {
-                        const int key = int(sequence.first_key + run.u.key(run.begin + i));
-                        for (int h = 0; h < S::kHalves && alive; ++h, ++items) {
-                            const uint32_t slot = items % S::kSlots;
-                            if (items >= uint32_t(S::kSlots) && !wait(kFree + slot, (items / S::kSlots - 1) & 1)) { alive = false; return; }
-                            mbar_expect_tx(&bars[kFull + slot], S::kSlotBytes);
+                    if (!S::kQInTmem) {
+                        if (piece && !wait(kQFree, (piece - 1) & 1)) { alive = false; break; }
+                        mbar_expect_tx(&bars[kQFull], uint32_t(T * (D / 64)) * a.tokens * a.group * 128);
+                        #pragma unroll 1
+                        for (int tile = 0; tile < T; ++tile)
                             for (int x = 0; x < D / 64; ++x)
-                                tma_load(smem + S::kOffRing + slot * S::kSlotBytes + x * (S::kSlotKeys * 128), &map, 64 * x, int(run.u.kv), key + h * S::kSlotKeys, &bars[kFull + slot]);
-                        }
+                                tma_load(smem + tile * S::kQueryBytes + x * (kM * 128), &a.q_map, 64 * x, int(run.u.kv * a.group),
+                                         int(sequence.first_row + run.u.row + tile * a.tokens), &bars[kQFull]);
+                    }
+                    auto key_of = [&](uint32_t i) -> int { return int(sequence.first_key + run.u.key(run.begin + i)); };
+                    auto load_k = [&](uint32_t i) {
+                        const uint32_t at = done + i, slot = at % S::kKSlots;
+                        if (at >= uint32_t(S::kKSlots) && !wait(kKFree + slot, (at / S::kKSlots - 1) & 1)) { alive = false; return; }
+                        mbar_expect_tx(&bars[kKFull + slot], S::kSlotBytes);
+                        for (int x = 0; x < D / 64; ++x)
+                            tma_load(smem + S::kOffK + slot * S::kSlotBytes + x * (kStep * 128), &a.k_map, 64 * x, int(run.u.kv), key_of(i), &bars[kKFull + slot]);
                     };
-                    for (uint32_t i = 0; i < kAhead && i < tiles && alive; ++i) load(a.k_map, i);
+                    for (uint32_t i = 0; i < kAhead && i < tiles && alive; ++i) load_k(i);
                     #pragma unroll 1
                     for (uint32_t i = 0; i < tiles && alive; ++i) {
-                        load(a.v_map, i);
-                        if (alive && i + kAhead < tiles) load(a.k_map, i + kAhead);
+                        const uint32_t at = done + i, slot = at % S::kVSlots;
+                        if (at >= uint32_t(S::kVSlots) && !wait(kVFree + slot, (at / S::kVSlots - 1) & 1)) { alive = false; break; }
+                        mbar_expect_tx(&bars[kVFull + slot], S::kSlotBytes);
+                        for (int x = 0; x < D / 64; ++x)
+                            tma_load(smem + S::kOffV + slot * S::kSlotBytes + x * (kStep * 128), &a.v_map, 64 * x, int(run.u.kv), key_of(i), &bars[kVFull + slot]);
+                        if (i + kAhead < tiles) load_k(i + kAhead);
                     }
+                        done += tiles;
                     ++piece;
                 }
             }
-        } else if (a.values) {
+        } else if (warp == kLookWarp && a.values) {
             // ================= masked values that are not finite =================
-            const int t = (warp - kLookWarp) * 32 + lane;
-            uint32_t looked = 0;   // tiles looked at (the next is not asked for before this one is done: the barriers' parities cannot be missed)
+            uint32_t looked = 0;   // steps looked at (the next is not asked for before this one is done: the barriers' parities cannot be missed)
             for (bool more = run.start(a); more && alive; more = run.next(a)) {
-                const uint32_t tiles = run.end - run.begin, ahead = min(kAhead, tiles);
+                const uint32_t tiles = run.end - run.begin;
                 if (!tiles) continue;
-                int edge = 0;      // slots of the piece looked at: the entry of `flagged` is the slot's own
+                int edge = 0;      // the piece's steps looked at: the entry of `flagged` is the step's own
                 #pragma unroll 1
-                for (uint32_t i = 0; i < tiles && alive; ++i) {
-                    const uint32_t key0 = run.u.key(run.begin + i);
+                for (uint32_t i = 0; i < tiles; ++i) {
+                    const uint32_t key0 = run.u.key(run.begin + i), at = done + i, slot = at % S::kVSlots;
                     if (run.u.open(a, key0)) continue;
-                    if (!wait(kLook, looked & 1)) { alive = false; break; }
+                    if (!wait(kLook, looked & 1) || !wait(kVFull + slot, (at / S::kVSlots) & 1)) { alive = false; break; }
                     ++looked;
-                    if (!edge) {   // (the outputs of the piece before are done: the issuing thread has waited for them)
-                        for (int e = t; e < kFlagged * 8; e += 64) flagged[e] = 0;
-                        asm volatile("bar.sync 9, 64;" ::: "memory");
+                    if (!edge) {   // (the outputs of the piece before are done: the issuing warps have waited for them)
+                        for (int e = lane; e < kFlagged * 8; e += 32) flagged[e] = 0;
+                        __syncwarp();
                     }
-                    for (int h = 0; h < S::kHalves; ++h) {
-                        const uint32_t at = items + (ahead + i + min(i, tiles - ahead)) * S::kHalves + h, slot = at % S::kSlots;
-                        if (!wait(kFull + slot, (at / S::kSlots) & 1)) { alive = false; break; }
-                        uint4* rows = reinterpret_cast<uint4*>(smem + S::kOffRing + slot * S::kSlotBytes);   // [64 columns of ..][key][8 pieces of 16 bytes]
-                        constexpr uint32_t kExponent = BF16 ? 0x7f807f80u : 0x7c007c00u, kCarry = BF16 ? 0x00800080u : 0x04000400u;
-                        #pragma unroll 4
-                        for (int at_piece = t; at_piece < S::kSlotBytes / 16; at_piece += 64) {
+                    uint4* rows = reinterpret_cast<uint4*>(smem + S::kOffV + slot * S::kSlotBytes);   // [64 columns of ..][key][8 pieces of 16 bytes]
+                    constexpr uint32_t kExponent = BF16 ? 0x7f807f80u : 0x7c007c00u, kCarry = BF16 ? 0x00800080u : 0x04000400u;
+                    uint32_t most = 0;   // the largest magnitude of either half, as a NaN if there is one
+                    #pragma unroll 8
+                    for (int at_piece = lane; at_piece < S::kSlotBytes / 16; at_piece += 32) {
+                        const uint4 v = rows[at_piece];
+                        most = largest<BF16>(largest<BF16>(largest<BF16>(most, v.x), largest<BF16>(v.y, v.z)), v.w);
+                    }
+                    if (__any_sync(0xffffffffu, ((most & kExponent) + kCarry) & 0x80008000u) && edge < kFlagged) {
+                        #pragma unroll 1
+                        for (int at_piece = lane; at_piece < S::kSlotBytes / 16; at_piece += 32) {
                             const uint4 v = rows[at_piece];
                             uint32_t w[4] = {v.x, v.y, v.z, v.w}, hit = 0;
                             #pragma unroll
-                            for (int x = 0; x < 4; ++x) hit |= (w[x] & kExponent) + kCarry;
-                            if (!(hit & 0x80008000u) || edge >= kFlagged) continue;
-                            #pragma unroll
                             for (int x = 0; x < 4; ++x) {
                                 const uint32_t bad = (w[x] & kExponent) + kCarry;
+                                hit |= bad & 0x80008000u;
                                 if (bad & 0x8000u) w[x] &= 0xffff0000u;
                                 if (bad & 0x80000000u) w[x] &= 0x0000ffffu;
                             }
+                            if (!hit) continue;
                             rows[at_piece] = make_uint4(w[0], w[1], w[2], w[3]);
-                            const int n = at_piece / 8 % S::kSlotKeys;
-                            flagged[8 * edge] = key0 + h * S::kSlotKeys;
+                            const int n = at_piece / 8 % kStep;
+                            flagged[8 * edge] = key0;
                             atomicOr(&flagged[8 * edge + 1 + n / 32], 1u << (n % 32));
                             *flagged_piece = piece + 1;
                         }
-                        ++edge;
                     }
-                    fence_proxy_async();   // (the tensor core reads the slots through the async proxy)
+                    ++edge;
+                    fence_proxy_async();   // (the tensor core reads the slot through the async proxy)
                     __syncwarp();
                     if (lane == 0) mbar_arrive(&bars[kClean]);
                 }
-                items += 2 * tiles * S::kHalves;
+                done += tiles;
                 ++piece;
             }
         }
@@ -886,7 +976,7 @@ template<int D, bool BF16> static void launch(Device& d, Args& args, bool behind
         units += q.blocks * args.kv_heads;
     }
     // The runs: a unit weighs its tiles and two more. The units of a block of rows, one a K/V head, are alike.
-    constexpr uint32_t kUnitTiles = 2;   // what a unit's first products, masked tiles and output cost more, in tiles
+    constexpr uint32_t kUnitTiles = 4;   // what a unit's first products, masked steps and output cost more, in steps
     uint64_t weight = 0;
     auto each_block = [&](auto&& act) {   // act(first unit, tiles of each of its kv_heads units); false ends
         for (uint32_t s = 0; s < args.sequences; ++s)
@@ -897,7 +987,7 @@ template<int D, bool BF16> static void launch(Device& d, Args& args, bool behind
             }
     };
     each_block([&](uint32_t, uint32_t tiles) { weight += uint64_t(tiles + kUnitTiles) * args.kv_heads; return true; });
-    constexpr uint64_t kLeast = 4;   // tiles (and unit) a run is worth a block of its own
+    constexpr uint64_t kLeast = 8;   // what a run weighs at least, unless there are units enough
     const uint32_t blocks = uint32_t(std::max<uint64_t>(1, std::min<uint64_t>(std::min<uint64_t>(uint64_t(d.sms), kMostBlocks), std::max<uint64_t>(weight / kLeast, std::min<uint64_t>(units, weight / 2)))));
     uint64_t passed = 0;
     uint32_t next = 1;
@@ -963,6 +1053,7 @@ static Args rule_args(uint64_t heads, uint64_t kv_heads, uint64_t dim, float sca
     args.heads = uint32_t(heads); args.kv_heads = uint32_t(kv_heads); args.group = uint32_t(heads / kv_heads); args.tokens = uint32_t(kM / args.group);
     args.window = uint32_t(std::min<uint64_t>(window, uint64_t(1) << 30));
     args.out = out; args.out_stride = out_stride; args.slopes = slopes;
+    args.queries = static_cast<const uint16_t*>(q); args.query_stride = q_stride;
     args.wide_out = reinterpret_cast<uintptr_t>(out) % 32 == 0 && out_stride % 16 == 0;
     args.scale_log2 = scale * 1.4426950408889634f;
     args.cap = cap * 1.4426950408889634f;
@@ -983,7 +1074,7 @@ void attend_kv8(Device& d, const std::vector<Sequence>& sequences, uint64_t head
         uint64_t blocks = 0;
         for (; at < sequences.size() && args.sequences < kSequences; ++at) {
             const Sequence& q = sequences[at];
-            const uint64_t more = (q.length + kTileKeys - 1) / kTileKeys * 4;
+            const uint64_t more = (q.length + 127) / 128 * 4;
             if (args.sequences && (blocks + more) * 32 * dim * 4 * kv_heads > kMostBytes) break;
             unpack.sequence[args.sequences] = UnpackSequence{q.state, uint32_t(q.context), uint32_t(q.length), uint32_t(blocks), uint32_t(more)};
             KernelSequence& to = args.sequence[args.sequences++];
@@ -1007,8 +1098,8 @@ void attend_kv8(Device& d, const std::vector<Sequence>& sequences, uint64_t head
             else go(int8 ? (bf16 ? kv8_unpack_kernel<256, 0, true> : kv8_unpack_kernel<256, 0, false>) : (bf16 ? kv8_unpack_kernel<256, 1, true> : kv8_unpack_kernel<256, 1, false>));
             ++d.launches;
             const uint64_t keys = blocks * 32;
-            args.k_map = tensor_map(unpack.rows, bf16, dim, kv_heads, keys, keys * dim, dim, 1, dim == 256 ? Shape<256>::kSlotKeys : kTileKeys);
-            args.v_map = tensor_map(unpack.rows + kv_heads * keys * dim, bf16, dim, kv_heads, keys, keys * dim, dim, 1, dim == 256 ? Shape<256>::kSlotKeys : kTileKeys);
+            args.k_map = tensor_map(unpack.rows, bf16, dim, kv_heads, keys, keys * dim, dim, 1, kStep);
+            args.v_map = tensor_map(unpack.rows + kv_heads * keys * dim, bf16, dim, kv_heads, keys, keys * dim, dim, 1, kStep);
             args.block_table = unpack.table;
             args.value_top = unpack.top;
             args.table_blocks = uint32_t(blocks);
@@ -1044,9 +1135,8 @@ static void masked(Device& d, const void* q, uint64_t q_stride, const void* k, u
         (keys && (kv8::overlap(out, out_bytes, k, ((keys - 1) * k_stride + kv_heads * dim) * 2) || kv8::overlap(out, out_bytes, v, ((keys - 1) * v_stride + kv_heads * dim) * 2))))
         throw std::runtime_error("an attention output lies over its queries, keys or values");
     Args args = rule_args(heads, kv_heads, dim, scale, cap, slopes, window, q, total, q_stride, out, out_stride, type);
-    const uint32_t slot_keys = dim == 256 ? Shape<256>::kSlotKeys : kTileKeys;
-    args.k_map = keys ? tensor_map(k, type == kv8::kBf16, dim, kv_heads, keys, dim, k_stride, 1, slot_keys) : args.q_map;
-    args.v_map = keys ? tensor_map(v, type == kv8::kBf16, dim, kv_heads, keys, dim, v_stride, 1, slot_keys) : args.q_map;
+    args.k_map = keys ? tensor_map(k, type == kv8::kBf16, dim, kv_heads, keys, dim, k_stride, 1, kStep) : args.q_map;
+    args.v_map = keys ? tensor_map(v, type == kv8::kBf16, dim, kv_heads, keys, dim, v_stride, 1, kStep) : args.q_map;
     args.values = static_cast<const uint16_t*>(v);
     args.value_stride = v_stride;
     uint64_t row = 0, key = 0;
