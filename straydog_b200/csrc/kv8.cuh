@@ -55,10 +55,10 @@ inline bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes
 #if defined(__CUDACC__)
 template<int CODE> constexpr float top_code() { return CODE == kInt8 ? 127.0f : 448.0f; }
 
-// x over scale in the block's code. The divide is the IEEE one: the codes are the definition's, bit for bit.
-template<int CODE> __device__ __forceinline__ uint32_t encode(float x, float scale) {
-    if (!(scale > 0.0f) || x != x) return 0;
-    const float y = __fdiv_rn(x, scale);
+// x over scale in the block's code: the IEEE quotient rounded to nearest even. A product with the scale's reciprocal (1 / scale, itself rounded once)
+// is within 2^-22 of the quotient; where both ends of that range round to the same code, so does the quotient, and only where they do not
+// (about one value in a thousand) is it divided. Scales without a normal number for their reciprocal divide always.
+template<int CODE> __device__ __forceinline__ uint32_t round_code(float y) {
     if (CODE == kInt8) {
         int q = __float2int_rn(y);
         q = q > 127 ? 127 : q < -127 ? -127 : q;
@@ -66,6 +66,34 @@ template<int CODE> __device__ __forceinline__ uint32_t encode(float x, float sca
     }
     return __nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
 }
+template<int CODE> __device__ __forceinline__ uint32_t encode(float x, float scale) {
+    if (!(scale > 0.0f) || x != x) return 0;
+    return round_code<CODE>(__fdiv_rn(x, scale));
+}
+struct Reciprocal {
+    float value;
+    bool normal;
+    __device__ __forceinline__ explicit Reciprocal(float scale) : value(scale > 0.0f ? 1.0f / scale : 0.0f), normal(scale > 1.2e-38f && scale < 8.5e37f) {}
+};
+// two values; the codes in the low two bytes
+template<int CODE> __device__ __forceinline__ uint32_t encode2(float x, float y, float scale, const Reciprocal& r) {
+    const float a = __fmul_rn(x, r.value), b = __fmul_rn(y, r.value);
+    constexpr float kDown = 1.0f - 3.6e-7f, kUp = 1.0f + 3.6e-7f;   // 1 -+ 3 * 2^-23
+    uint32_t low, high;
+    if (CODE == kInt8) {
+        // a sum with 1.5 * 2^23 rounds to an integer and leaves it in the low byte (clamped before: an infinity is the largest code)
+        const float a0 = fminf(fmaxf(a * kDown, -127.0f), 127.0f), a1 = fminf(fmaxf(a * kUp, -127.0f), 127.0f);
+        const float b0 = fminf(fmaxf(b * kDown, -127.0f), 127.0f), b1 = fminf(fmaxf(b * kUp, -127.0f), 127.0f);
+        low = prmt(__float_as_uint(__fadd_rn(a0, 12582912.0f)), __float_as_uint(__fadd_rn(b0, 12582912.0f)), 0x0040u) & 0xffffu;
+        high = prmt(__float_as_uint(__fadd_rn(a1, 12582912.0f)), __float_as_uint(__fadd_rn(b1, 12582912.0f)), 0x0040u) & 0xffffu;
+    } else {
+        low = __nv_cvt_float2_to_fp8x2(make_float2(a * kDown, b * kDown), __NV_SATFINITE, __NV_E4M3);
+        high = __nv_cvt_float2_to_fp8x2(make_float2(a * kUp, b * kUp), __NV_SATFINITE, __NV_E4M3);
+    }
+    if (low == high && r.normal && x == x && y == y) return low;
+    return encode<CODE>(x, scale) | encode<CODE>(y, scale) << 8;
+}
+
 // Sixteen codes of a row whose block takes a larger scale: their values in the old scale, rounded again in the new one (ratio = old / new
 // <= 1). Code times ratio in F32, then one rounding to the code: what encode(decode(c) * ratio, 1) gives, without the conversion unit where
 // it can be done without (its 16 results a clock an SM would bound an eviction). int8: a byte becomes 2^23 + 128 + c by a byte permute, and a

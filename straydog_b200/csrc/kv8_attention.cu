@@ -54,7 +54,7 @@ struct AttentionArgs {
     float* partial;          // [warp + unit][queries][D]: a run's next piece has the next unit, a unit's next piece the next warp
     float* sums;             // [warp + unit][queries][2]: maximum (exp2 domain, lifted), denominator
     float* scores;           // [tile][keys][score_queries] or null
-    float* stats;            // [unit][queries][2]: final maximum and denominator, for the weights
+    float* stats;            // [unit][queries][2]: final maximum and inverse of the sum, for the weights
 };
 
 __device__ __forceinline__ void copy16(uint32_t to, const void* from) {
@@ -66,23 +66,20 @@ __device__ __forceinline__ void copy4(uint32_t to, const void* from) {
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(to), "l"(from) : "memory");
 }
 
-// Two codes of a word as an FP16 pair: low bytes 0 and 1 or 2 and 3 (keys: neighbouring columns), bytes 0 and 2 or 1 and 3 (values:
-// one column of two keys). int8 exactly (x is the word xor 0x80808080: 1024 + 128 + c, less 1152); E4M3 at 2^-8 of its value, exactly
-// (its exponent and mantissa bits moved to FP16's places), which the caller's scale makes good.
-template<int CODE> __device__ __forceinline__ uint32_t pair_of(uint32_t x, uint32_t int8_selector, uint32_t e4m3_selector) {
+// The four codes of a word as two FP16 pairs, exactly: columns (0, 1) and (2, 3) of a key, or columns 0 and 1 of two keys (bytes (0, 2) and
+// (1, 3)) of values. int8: a byte behind 0x64 is 1024 + 128 + c of the word xor 0x80808080, less 1152; E4M3: the conversion instruction.
+template<int CODE, bool KEYS> __device__ __forceinline__ void pairs_of(uint32_t x, uint32_t& first, uint32_t& second) {
     if (CODE == kInt8) {
-        const uint32_t h = prmt(x, 0x64646464u, int8_selector);
-        const __half2 r = __hsub2(*reinterpret_cast<const __half2*>(&h), __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480)));
-        return *reinterpret_cast<const uint32_t*>(&r);
+        x ^= 0x80808080u;
+        const __half2 bias = __halves2half2(__ushort_as_half(0x6480), __ushort_as_half(0x6480));
+        const uint32_t h0 = prmt(x, 0x64646464u, KEYS ? 0x4140u : 0x4240u), h1 = prmt(x, 0x64646464u, KEYS ? 0x4342u : 0x4341u);
+        const __half2 r0 = __hsub2(*reinterpret_cast<const __half2*>(&h0), bias), r1 = __hsub2(*reinterpret_cast<const __half2*>(&h1), bias);
+        first = *reinterpret_cast<const uint32_t*>(&r0); second = *reinterpret_cast<const uint32_t*>(&r1);
+    } else {
+        if (!KEYS) x = prmt(x, 0u, 0x3120u);
+        asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}" : "=r"(first), "=r"(second) : "r"(x));
     }
-    const uint32_t y = prmt(x, 0u, e4m3_selector);   // each code in the high byte of its half
-    return (y & 0x80008000u) | ((y >> 1) & 0x3f803f80u);
 }
-template<int CODE> __device__ __forceinline__ uint32_t pair01(uint32_t x) { return pair_of<CODE>(x, 0x4140u, 0x1404u); }
-template<int CODE> __device__ __forceinline__ uint32_t pair23(uint32_t x) { return pair_of<CODE>(x, 0x4342u, 0x3424u); }
-template<int CODE> __device__ __forceinline__ uint32_t pair02(uint32_t x) { return pair_of<CODE>(x, 0x4240u, 0x2404u); }
-template<int CODE> __device__ __forceinline__ uint32_t pair13(uint32_t x) { return pair_of<CODE>(x, 0x4341u, 0x3414u); }
-template<int CODE> __device__ __forceinline__ uint32_t flipped(uint32_t x) { return CODE == kInt8 ? x ^ 0x80808080u : x; }
 
 template<int D, int NT> struct Shape {
     static constexpr int kTile = D == 256 ? 16 : 32;                  // keys a tile: 8 KB of keys and values for D 128 and 256, 4 KB for 64
@@ -201,7 +198,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
                     const uint4 v = real ? *reinterpret_cast<const uint4*>(from + c * 128 + i * 16) : make_uint4(0, 0, 0, 0);
                     qf[n][c * 8 + i * 4] = v.x; qf[n][c * 8 + i * 4 + 1] = v.y; qf[n][c * 8 + i * 4 + 2] = v.z; qf[n][c * 8 + i * 4 + 3] = v.w;
                 }
-            float down = CODE == kE4m3 ? 256.0f : 1.0f;
+            float down = 1.0f;
             if (a.bf16) {
                 uint32_t top = 0;   // magnitudes of BF16 values compare as their bits do
                 #pragma unroll
@@ -252,7 +249,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
             const int key0 = int(tile * S::kTile);
             const uint8_t* kt = ring + slot * S::kSlot;
             const uint32_t vt = ring_address + slot * S::kSlot + S::kPlane;
-            const float k_scale = ring_scales[slot * 2], v_scale = ring_scales[slot * 2 + 1] * (CODE == kE4m3 ? 256.0f : 1.0f);
+            const float k_scale = ring_scales[slot * 2], v_scale = ring_scales[slot * 2 + 1];
 
             // ---- scores ----
             float x[S::kTile / 16][NT][4];
@@ -266,11 +263,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
                     const int piece = D == 64 ? t : (4 * c + t) ^ (4 * (g & 1));
                     const uint4 r0 = *reinterpret_cast<const uint4*>(kt + (16 * h + g) * D + piece * 16);
                     const uint4 r1 = *reinterpret_cast<const uint4*>(kt + (16 * h + g + 8) * D + piece * 16);
-                    const uint32_t w0[4] = {flipped<CODE>(r0.x), flipped<CODE>(r0.y), flipped<CODE>(r0.z), flipped<CODE>(r0.w)};
-                    const uint32_t w1[4] = {flipped<CODE>(r1.x), flipped<CODE>(r1.y), flipped<CODE>(r1.z), flipped<CODE>(r1.w)};
+                    const uint32_t w0[4] = {r0.x, r0.y, r0.z, r0.w}, w1[4] = {r1.x, r1.y, r1.z, r1.w};
                     #pragma unroll
                     for (int i = 0; i < 4; ++i) {
-                        const uint32_t af[4] = {pair01<CODE>(w0[i]), pair01<CODE>(w1[i]), pair23<CODE>(w0[i]), pair23<CODE>(w1[i])};
+                        uint32_t af[4];
+                        pairs_of<CODE, true>(w0[i], af[0], af[2]);
+                        pairs_of<CODE, true>(w1[i], af[1], af[3]);
                         #pragma unroll
                         for (int n = 0; n < NT; ++n) mma_f16(acc[n], af, qf[n][c * 8 + 2 * i], qf[n][c * 8 + 2 * i + 1]);
                     }
@@ -387,10 +385,11 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
                     const uint32_t row = v_lane + 16 * h, piece = (2 * b + lane / 16) ^ (D == 64 ? (row >> 1) & 3 : row & 7);
                     uint32_t w[4];   // w[0], w[1]: columns 32b + 2g, + 1 of keys (2t, 2t + 1) and (2t + 8, 2t + 9); w[2], w[3]: columns 32b + 16 + 2g, + 1
                     ldmatrix_x4_trans(w, vt + row * D + piece * 16);
-                    #pragma unroll
-                    for (int i = 0; i < 4; ++i) w[i] = flipped<CODE>(w[i]);
-                    const uint32_t af[4] = {pair02<CODE>(w[0]), pair13<CODE>(w[0]), pair02<CODE>(w[1]), pair13<CODE>(w[1])};
-                    const uint32_t ag[4] = {pair02<CODE>(w[2]), pair13<CODE>(w[2]), pair02<CODE>(w[3]), pair13<CODE>(w[3])};
+                    uint32_t af[4], ag[4];
+                    pairs_of<CODE, false>(w[0], af[0], af[1]);
+                    pairs_of<CODE, false>(w[1], af[2], af[3]);
+                    pairs_of<CODE, false>(w[2], ag[0], ag[1]);
+                    pairs_of<CODE, false>(w[3], ag[2], ag[3]);
                     #pragma unroll
                     for (int n = 0; n < NT; ++n) {
                         mma_f16(acc[0][n], af, pf[h][n][0], pf[h][n][1]);
@@ -431,7 +430,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
                         const float v0 = o[b][n][i] * inverse, v1 = o[b][n][i + 2] * inverse;
                         *reinterpret_cast<uint32_t*>(to + 16 * b) = a.bf16 ? pack_bf16x2(v0, v1) : pack_half2(v0, v1);
                     }
-                    if (a.scores && g == 0) *reinterpret_cast<float2*>(a.stats + (size_t(at.unit) * S::kQueries + query) * 2) = make_float2(m[n][i], l[n][i]);
+                    if (a.scores && g == 0) *reinterpret_cast<float2*>(a.stats + (size_t(at.unit) * S::kQueries + query) * 2) = make_float2(m[n][i], inverse);
                 } else {
                     float* to = a.partial + (mine * S::kQueries + query) * D + 2 * g;
                     #pragma unroll
@@ -446,11 +445,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
 }
 
 // Block = (unit, query): joins the partials of a unit that several warps worked on, and zeroes the rows of a sequence without keys.
-constexpr int kJoinThreads = 512, kMostWarps = 2048;   // (warps of a launch: eight an SM)
-template<int D>
+// Few partials (a batch of many sequences): 128 threads, so that all blocks run at once; many (one long sequence): 512.
+constexpr int kMostWarps = 2048, kFewPieces = 32;   // warps of a launch (eight an SM)
+template<int D, int kJoinThreads>
 __global__ void __launch_bounds__(kJoinThreads) kv8_decode_join_kernel(const __grid_constant__ AttentionArgs a, uint32_t queries_a_unit) {
     constexpr int kColumns = D / 4, kGroups = kJoinThreads / kColumns;   // threads a partial row, partials at a time
-    __shared__ float factors[kMostWarps];
+    constexpr int kMost = kJoinThreads == 128 ? kFewPieces : kMostWarps, kSums = (kMost + kJoinThreads - 1) / kJoinThreads;
+    __shared__ float factors[kMost];
     __shared__ float tops[kJoinThreads / 32], weights[kJoinThreads / 32];
     __shared__ float4 totals[kGroups][kColumns];
     const uint32_t unit = blockIdx.x, query = blockIdx.y;
@@ -482,10 +483,10 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_decode_join_kernel(const __g
         const uint32_t p = group + i * kGroups;
         v[i] = p < pieces ? partial[size_t(p) * queries_a_unit * kColumns] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
-    float2 mine[(kMostWarps + kJoinThreads - 1) / kJoinThreads];
+    float2 mine[kSums];
     float top = -INFINITY;
     #pragma unroll
-    for (int i = 0; i < (kMostWarps + kJoinThreads - 1) / kJoinThreads; ++i) {
+    for (int i = 0; i < kSums; ++i) {
         const uint32_t p = threadIdx.x + i * kJoinThreads;
         mine[i] = p < pieces ? sums[size_t(p) * queries_a_unit] : make_float2(-INFINITY, 0.0f);
         top = fmaxf(top, mine[i].x);
@@ -499,7 +500,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_decode_join_kernel(const __g
     for (int w = 1; w < kJoinThreads / 32; ++w) top = fmaxf(top, tops[w]);
     float weight = 0.0f;
     #pragma unroll
-    for (int i = 0; i < (kMostWarps + kJoinThreads - 1) / kJoinThreads; ++i) {
+    for (int i = 0; i < kSums; ++i) {
         const uint32_t p = threadIdx.x + i * kJoinThreads;
         // (nothing seen in a piece: no weight; scores that are all NaN leave a NaN sum, which stays)
         const float factor = mine[i].y == 0.0f ? 0.0f : mine[i].x == -INFINITY ? 1.0f : fast_exp2(mine[i].x - top);
@@ -532,14 +533,14 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_decode_join_kernel(const __g
     }
     totals[group][column] = total;
     __syncthreads();
-    if (a.scores && threadIdx.x == 0) *reinterpret_cast<float2*>(a.stats + (size_t(unit) * queries_a_unit + query) * 2) = make_float2(top, weight);
+    const float inverse = inverse_of(weight);
+    if (a.scores && threadIdx.x == 0) *reinterpret_cast<float2*>(a.stats + (size_t(unit) * queries_a_unit + query) * 2) = make_float2(top, inverse);
     if (threadIdx.x >= kColumns) return;
     #pragma unroll
     for (int i = 1; i < kGroups; ++i) {
         const float4 other = totals[i][column];
         total.x += other.x; total.y += other.y; total.z += other.z; total.w += other.w;
     }
-    const float inverse = inverse_of(weight);
     *reinterpret_cast<uint2*>(out + 4 * column) = a.bf16 ? make_uint2(pack_bf16x2(total.x * inverse, total.y * inverse), pack_bf16x2(total.z * inverse, total.w * inverse))
                                                        : make_uint2(pack_half2(total.x * inverse, total.y * inverse), pack_half2(total.z * inverse, total.w * inverse));
 }
@@ -573,7 +574,7 @@ __global__ void __launch_bounds__(256) kv8_weights_kernel(const __grid_constant_
             for (int c = 0; c < 4; ++c) {
                 if (uint32_t(4 * i + c) >= queries) continue;
                 const float2 stat = stats[4 * i + c];
-                if (x[c] != -INFINITY) total += fast_exp2(x[c] - stat.x) / stat.y;
+                if (x[c] != -INFINITY) total = fmaf(fast_exp2(x[c] - stat.x), stat.y, total);
             }
         }
     }
@@ -610,14 +611,15 @@ template<int D, int NT, int CODE> static void launch_decode(Device& d, Attention
     const uint64_t blocks = std::min<uint64_t>(uint64_t(d.sms), warps);
     args.tiles_a_warp = std::max<uint64_t>(1, (args.tiles + warps - 1) / warps);
     const size_t slots = blocks * kWarps + args.units;
-    bool cut = false;   // a unit that several warps work on
-    for (uint32_t s = 0; s < args.sequences && !cut; ++s) {
+    uint64_t pieces = 0;   // of the unit that most warps work on
+    for (uint32_t s = 0; s < args.sequences; ++s) {
         const AttentionSequence& q = args.sequence[s];
-        for (uint32_t u = 0; u < args.kv_heads * q.parts && q.tiles && !cut; ++u) {
+        for (uint32_t u = 0; u < args.kv_heads * q.parts && q.tiles; ++u) {
             const uint64_t begin = q.first_tile + uint64_t(u) * q.tiles;
-            cut = begin / args.tiles_a_warp != (begin + q.tiles - 1) / args.tiles_a_warp;
+            pieces = std::max(pieces, (begin + q.tiles - 1) / args.tiles_a_warp - begin / args.tiles_a_warp + 1);
         }
     }
+    const bool cut = pieces > 1;
     const size_t partial_floats = cut ? slots * S::kQueries * D : 0, sums_floats = cut ? slots * S::kQueries * 2 : 0;
     float* partial = cut ? static_cast<float*>(workspace(d, d.kv8_partial, (partial_floats + sums_floats) * 4)) : nullptr;
     args.partial = partial;
@@ -644,11 +646,11 @@ template<int D, int NT, int CODE> static void launch_decode(Device& d, Attention
     if (cut || empty) {
         cudaLaunchConfig_t config{};
         config.gridDim = dim3(args.units, S::kQueries);
-        config.blockDim = dim3(kJoinThreads);
+        config.blockDim = dim3(pieces <= kFewPieces ? 128 : 512);
         config.stream = d.stream;
         config.attrs = &attribute;
         config.numAttrs = behind ? 1 : 0;
-        SDB_CHECK(cudaLaunchKernelEx(&config, kv8_decode_join_kernel<D>, args, uint32_t(S::kQueries)));
+        SDB_CHECK(cudaLaunchKernelEx(&config, pieces <= kFewPieces ? kv8_decode_join_kernel<D, 128> : kv8_decode_join_kernel<D, 512>, args, uint32_t(S::kQueries)));
         ++d.launches;
     }
     if (args.scores) {

@@ -5,9 +5,9 @@
 // c are rounded again: c * (old / scale). Positions behind the call's rows are not touched (whatever they hold is not counted on: the
 // sequence ends there).
 //
-// One block of 128 threads does one (sequence, plane, block of 32): the block's new rows stay in registers between the maximum and the
+// One block of 128 or 256 threads does one (sequence, plane, block of 32): the block's new rows stay in registers between the maximum and the
 // codes, so each value is read once. Bound by memory for a prompt, by one chain of latencies (row, maximum, store) for a single token:
-// then 16 threads hold the row and the rest look after the older codes.
+// then a few threads hold the row and the rest look after the older codes.
 #include "kv8.cuh"
 #include "../../include/straydog_gpu_b200.h"
 
@@ -53,9 +53,12 @@ template<> struct Load8<__nv_bfloat16> {
     }
 };
 
+// threads of a block: at most 32 values each
+template<int D> constexpr int kWriteThreads = D == 256 ? 256 : 128;
+
 template<int D, typename T, int CODE>
-__global__ void __launch_bounds__(128) kv8_write_kernel(const __grid_constant__ WriteArgs a) {
-    constexpr int kColumns = D / 8, kRows = 128 / kColumns, kPasses = int(kBlock) / kRows;   // threads a row, rows a pass
+__global__ void __launch_bounds__(kWriteThreads<D>) kv8_write_kernel(const __grid_constant__ WriteArgs a) {
+    constexpr int kThreads = kWriteThreads<D>, kColumns = D / 8, kRows = kThreads / kColumns, kPasses = int(kBlock) / kRows;   // threads a row, rows a pass
     uint32_t s = 0;
     {
         uint32_t high = a.sequences;   // the last sequence whose first unit is not behind this block
@@ -90,24 +93,27 @@ __global__ void __launch_bounds__(128) kv8_write_kernel(const __grid_constant__ 
     }
     #pragma unroll
     for (int offset = 16; offset; offset /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, offset));
-    __shared__ float tops[4];
+    __shared__ float tops[kThreads / 32];
     if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = top;
     __syncthreads();   // (also: every thread has read the old scale before one writes the new)
-    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    #pragma unroll
+    for (int i = 0; i < kThreads / 32; ++i) top = fmaxf(top, tops[i]);
     const float scale = fmaxf(old, __fdiv_rn(top, top_code<CODE>()));
+    const Reciprocal reciprocal(scale);
     #pragma unroll
     for (int p = 0; p < kPasses; ++p) {
         const uint32_t at = begin + p * kRows + row;
         if (at < low || at >= high) continue;
-        uint32_t w[2] = {0, 0};
+        uint32_t w[2];
         #pragma unroll
-        for (int i = 0; i < 8; ++i) w[i / 4] |= encode<CODE>(x[p][i], scale) << (8 * (i % 4));
+        for (int i = 0; i < 2; ++i)
+            w[i] = encode2<CODE>(x[p][4 * i], x[p][4 * i + 1], scale, reciprocal) | encode2<CODE>(x[p][4 * i + 2], x[p][4 * i + 3], scale, reciprocal) << 16;
         *reinterpret_cast<uint2*>(codes + size_t(p * kRows + row) * D + column) = make_uint2(w[0], w[1]);
     }
     if (begun && scale > old) {
         const float ratio = __fdiv_rn(old, scale);
         const uint32_t pieces = (low - begin) * (D / 16);   // the older rows, 16 codes a piece
-        for (uint32_t i = threadIdx.x; i < pieces; i += 128) {
+        for (uint32_t i = threadIdx.x; i < pieces; i += kThreads) {
             uint4* at = reinterpret_cast<uint4*>(codes) + i;
             *at = recode16<CODE>(*at, ratio);
         }
@@ -116,8 +122,8 @@ __global__ void __launch_bounds__(128) kv8_write_kernel(const __grid_constant__ 
 }
 
 template<int D, typename T> static void launch_code(int code, const WriteArgs& args, uint32_t units, cudaStream_t stream) {
-    if (code == kInt8) kv8_write_kernel<D, T, kInt8><<<units, 128, 0, stream>>>(args);
-    else kv8_write_kernel<D, T, kE4m3><<<units, 128, 0, stream>>>(args);
+    if (code == kInt8) kv8_write_kernel<D, T, kInt8><<<units, kWriteThreads<D>, 0, stream>>>(args);
+    else kv8_write_kernel<D, T, kE4m3><<<units, kWriteThreads<D>, 0, stream>>>(args);
 }
 template<int D> static void launch_type(int code, int type, const WriteArgs& args, uint32_t units, cudaStream_t stream) {
     if (type == kF32) launch_code<D, float>(code, args, units, stream);
