@@ -95,9 +95,8 @@ template<int CODE> __device__ __forceinline__ uint32_t encode2(float x, float y,
 }
 
 // Sixteen codes of a row whose block takes a larger scale: their values in the old scale, rounded again in the new one (ratio = old / new
-// <= 1). Code times ratio in F32, then one rounding to the code: what encode(decode(c) * ratio, 1) gives, without the conversion unit where
-// it can be done without (its 16 results a clock an SM would bound an eviction). int8: a byte becomes 2^23 + 128 + c by a byte permute, and a
-// sum with 1.5 * 2^23 rounds to nearest even and leaves the code in the low byte. E4M3: the code's bits placed in an F32 are its value times 2^-120.
+// <= 1): code times ratio in F32, then one rounding to the code. int8: a byte becomes 2^23 + 128 + c by a byte permute, and a sum with
+// 1.5 * 2^23 rounds to nearest even and leaves the code in the low byte. E4M3: two codes a conversion on the way in and out.
 template<int CODE> __device__ __forceinline__ uint4 recode16(uint4 v, float ratio) {
     if (ratio == 1.0f) return v;
     uint32_t w[4] = {v.x, v.y, v.z, v.w};
@@ -113,15 +112,11 @@ template<int CODE> __device__ __forceinline__ uint4 recode16(uint4 v, float rati
             }
             w[i] = prmt(prmt(q[0], q[1], 0x0040u), prmt(q[2], q[3], 0x0040u), 0x5410u);
         } else {
-            const float up = ratio * 1.329227995784916e36f;   // 2^120
-            float f[4];
-            #pragma unroll
-            for (int b = 0; b < 4; ++b) {
-                const uint32_t byte = w[i] >> (8 * b);
-                f[b] = __fmul_rn(__uint_as_float((byte & 0x80u) << 24 | (byte & 0x7fu) << 20), up);
-            }
-            w[i] = uint32_t(__nv_cvt_float2_to_fp8x2(make_float2(f[0], f[1]), __NV_SATFINITE, __NV_E4M3)) |
-                   uint32_t(__nv_cvt_float2_to_fp8x2(make_float2(f[2], f[3]), __NV_SATFINITE, __NV_E4M3)) << 16;
+            uint32_t low, high;
+            asm("{\n\t.reg .b16 lo, hi;\n\tmov.b32 {lo, hi}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, lo;\n\tcvt.rn.f16x2.e4m3x2 %1, hi;\n\t}" : "=r"(low), "=r"(high) : "r"(w[i]));
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&low)), g = __half22float2(*reinterpret_cast<const __half2*>(&high));
+            asm("{\n\t.reg .b16 lo, hi;\n\tcvt.rn.satfinite.e4m3x2.f32 lo, %2, %1;\n\tcvt.rn.satfinite.e4m3x2.f32 hi, %4, %3;\n\tmov.b32 %0, {lo, hi};\n\t}"
+                : "=r"(w[i]) : "f"(__fmul_rn(f.x, ratio)), "f"(__fmul_rn(f.y, ratio)), "f"(__fmul_rn(g.x, ratio)), "f"(__fmul_rn(g.y, ratio)));
         }
     }
     return make_uint4(w[0], w[1], w[2], w[3]);

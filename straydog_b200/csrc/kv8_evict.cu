@@ -10,7 +10,9 @@
 // and the bin where the places run out. A warp whose weights are all in one bin (weights of never-attended rows are all 0) adds them with one
 // atomic. (Sixteen steps of two bits by compares, without atomics, took 65 us for 16 sequences x 8 heads x 16384: eight issue slots a weight and
 // step.) Then ballots give every kept position its place in order.
-// kv8_evict_move_kernel: a block of 128 threads a (sequence, plane, target block of 32 rows): bound by memory, rows of `dim` bytes gathered.
+// kv8_evict_move_kernel: 128 threads a (sequence, plane, one or four target blocks of 32 rows), rows of `dim` bytes gathered: bound by memory as long as the
+// codes' rounding stays under its issue slots (eleven instructions a code with bit masks for E4M3 and a block a target block: 87 % of all issue slots, 101 us
+// for 16 x 16384 positions).
 #include "kv8.cuh"
 #include "../../include/straydog_gpu_b200.h"
 
@@ -30,7 +32,11 @@ struct EvictArgs {
     EvictSequence sequence[kSequences];
     int32_t* kept;      // [sequences of this launch][kv_heads][keep]
     uint32_t sequences, kv_heads, keep, sinks, recent;
+    uint32_t each;      // target blocks a thread block moves, one behind the other
 };
+
+// and back, but for NaN and -0
+__device__ __forceinline__ float weight_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); }
 
 constexpr int kSelectThreads = 1024, kSelectWarps = 32, kHeld = 32, kMostCluster = 8;   // weights a thread holds; blocks a head
 constexpr int kBins = 2048, kCopies = 4;   // a histogram's bins; copies that a block's warps share out, so that they meet less
@@ -94,12 +100,8 @@ __global__ void __launch_bounds__(kSelectThreads, 1) kv8_evict_select_kernel(con
         each_key([&](uint32_t j, uint32_t k) {
             const bool counts = first + j * 32 + lane < between && (step == 0 || (k >> (shift + bits)) == (last >> (shift + bits)));
             const uint32_t bin = counts ? (k >> shift) & ((1u << bits) - 1u) : 0xffffffffu;
-            const uint32_t live = __ballot_sync(0xffffffffu, counts);
-            if (!live) return;
-            const uint32_t leader = uint32_t(__ffs(int(live)) - 1), common = __shfl_sync(0xffffffffu, bin, int(leader));
-            const uint32_t same = __ballot_sync(0xffffffffu, bin == common);
-            if (lane == leader) atomicAdd(&mine_counts[common], uint32_t(__popc(same)));
-            if (counts && bin != common) atomicAdd(&mine_counts[bin], 1u);
+            const bool same = __all_sync(0xffffffffu, bin == __shfl_sync(0xffffffffu, bin, 0));
+            if (counts && (!same || lane == 0)) atomicAdd(&mine_counts[bin], same ? 32u : 1u);
         });
         __syncthreads();
         for (int i = threadIdx.x; i < kBins; i += kSelectThreads) {
@@ -120,7 +122,7 @@ __global__ void __launch_bounds__(kSelectThreads, 1) kv8_evict_select_kernel(con
         for (int offset = 1; offset < 32; offset *= 2) { const uint32_t other = __shfl_up_sync(0xffffffffu, above, offset); if (lane >= uint32_t(offset)) above += other; }
         if (lane == 31) warp_counts[warp][0] = above;
         __syncthreads();
-        for (uint32_t w = 0; w < warp; ++w) above += warp_counts[w][0];
+        above += __reduce_add_sync(0xffffffffu, lane < warp ? warp_counts[lane][0] : 0u);   // the warps before
         const uint32_t before_high = above - high - low, before_low = above - low;
         if (before_high < missing && missing <= above) {   // one thread: the places run out in one of its bins
             const bool in_high = missing <= before_low;
@@ -152,7 +154,8 @@ __global__ void __launch_bounds__(kSelectThreads, 1) kv8_evict_select_kernel(con
             const uint32_t* counts = cluster.map_shared_rank(&block_counts[0], r);
             reach += counts[0]; above += counts[1];
         }
-        for (uint32_t w = 0; w < warp; ++w) { reach += warp_counts[w][0]; above += warp_counts[w][1]; }
+        reach += __reduce_add_sync(0xffffffffu, lane < warp ? warp_counts[lane][0] : 0u);
+        above += __reduce_add_sync(0xffffffffu, lane < warp ? warp_counts[lane][1] : 0u);
         const uint32_t ties = want ? missing : 0;
         uint32_t equal = reach - above;
         uint32_t place = sinks + above + min(equal, ties);
@@ -165,7 +168,7 @@ __global__ void __launch_bounds__(kSelectThreads, 1) kv8_evict_select_kernel(con
             if (stays) {
                 const uint32_t i = first + j * 32 + lane, at = place + __popc(staying & below);
                 kept[at] = int32_t(sinks + i);
-                target_weights[at] = mine[i];
+                target_weights[at] = k && k != 0x80000000u ? weight_of(k) : mine[i];   // (a NaN and a zero's sign are not in the key)
             }
             equal += __popc(ties_here);
             place += __popc(staying);
@@ -183,41 +186,55 @@ __global__ void __launch_bounds__(128) kv8_evict_move_kernel(const __grid_consta
         while (high - s > 1) { const uint32_t mid = (s + high) / 2; if (a.sequence[mid].first_unit <= blockIdx.x) s = mid; else high = mid; }
     }
     const EvictSequence& sequence = a.sequence[s];
-    const uint32_t planes = 2 * a.kv_heads, unit = blockIdx.x - sequence.first_unit, plane = unit % planes, block = unit / planes;
-    const uint32_t rows = min(min(sequence.length, a.keep) - block * kBlock, kBlock);
+    const uint32_t planes = 2 * a.kv_heads, unit = blockIdx.x - sequence.first_unit, plane = unit % planes, first = unit / planes * a.each;
+    const uint32_t kept_rows = min(sequence.length, a.keep), end = min(first + a.each, (kept_rows + kBlock - 1) / kBlock);
     const uint32_t row = threadIdx.x / kPieces, piece = threadIdx.x % kPieces;
-    const int32_t* kept = a.kept + (size_t(s) * a.kv_heads + plane % a.kv_heads) * a.keep + block * kBlock;
-    const uint8_t* codes = sequence.state + size_t(plane) * sequence.context * D;
+    const int32_t* kept = a.kept + (size_t(s) * a.kv_heads + plane % a.kv_heads) * a.keep;
+    const uint8_t* codes = sequence.state + size_t(plane) * sequence.context * D + piece * 16;
     const float* scales = reinterpret_cast<const float*>(sequence.state + size_t(planes) * sequence.context * D) + size_t(plane) * (sequence.context / kBlock);
+    uint8_t* target = sequence.target + size_t(plane) * sequence.target_context * D + piece * 16;
+    float* target_scales = reinterpret_cast<float*>(sequence.target + size_t(planes) * sequence.target_context * D) + size_t(plane) * (sequence.target_context / kBlock);
+    __shared__ float tops[2][4];
     asm volatile("griddepcontrol.wait;" ::: "memory");   // the positions are the kernel's before
-    uint4 v[kPasses];
-    float old[kPasses];
-    #pragma unroll
-    for (int p = 0; p < kPasses; ++p) {
-        const uint32_t r = p * kRows + row;
-        const uint32_t from = r < rows ? uint32_t(kept[r]) : 0u;
-        old[p] = r < rows ? scales[from / kBlock] : 0.0f;
-        v[p] = r < rows ? *reinterpret_cast<const uint4*>(codes + size_t(from) * D + piece * 16) : make_uint4(0, 0, 0, 0);
+    uint32_t from[kPasses];
+    auto positions = [&](uint32_t block) {
+        #pragma unroll
+        for (int p = 0; p < kPasses; ++p) {
+            const uint32_t r = block * kBlock + p * kRows + row;
+            from[p] = block < end && r < kept_rows ? uint32_t(kept[r]) : 0xffffffffu;
+        }
+    };
+    positions(first);
+    #pragma unroll 1
+    for (uint32_t block = first; block < end; ++block) {
+        uint4 v[kPasses];
+        float old[kPasses];
+        #pragma unroll
+        for (int p = 0; p < kPasses; ++p) {
+            const bool there = from[p] != 0xffffffffu;
+            old[p] = there ? scales[from[p] / kBlock] : 0.0f;
+            v[p] = there ? *reinterpret_cast<const uint4*>(codes + size_t(from[p]) * D) : make_uint4(0, 0, 0, 0);
+        }
+        bool there[kPasses];
+        #pragma unroll
+        for (int p = 0; p < kPasses; ++p) there[p] = from[p] != 0xffffffffu;
+        positions(block + 1);   // (asked for while this block's rows are on their way)
+        float top = 0.0f;
+        #pragma unroll
+        for (int p = 0; p < kPasses; ++p) top = fmaxf(top, old[p]);
+        #pragma unroll
+        for (int offset = 16; offset >= kPieces; offset /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, offset));   // (a row's threads have one scale)
+        if (threadIdx.x % 32 == 0) tops[block & 1][threadIdx.x / 32] = top;
+        __syncthreads();
+        const float scale = fmaxf(fmaxf(tops[block & 1][0], tops[block & 1][1]), fmaxf(tops[block & 1][2], tops[block & 1][3]));
+        #pragma unroll
+        for (int p = 0; p < kPasses; ++p) {
+            if (!there[p]) continue;
+            const float ratio = scale > 0.0f ? __fdiv_rn(old[p], scale) : 0.0f;
+            *reinterpret_cast<uint4*>(target + size_t(block * kBlock + p * kRows + row) * D) = recode16<CODE>(v[p], ratio);
+        }
+        if (threadIdx.x == 0) target_scales[block] = scale;
     }
-    float top = 0.0f;
-    #pragma unroll
-    for (int p = 0; p < kPasses; ++p) top = fmaxf(top, old[p]);
-    #pragma unroll
-    for (int offset = 16; offset; offset /= 2) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, offset));
-    __shared__ float tops[4];
-    if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = top;
-    __syncthreads();
-    const float scale = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-    uint8_t* to = sequence.target + (size_t(plane) * sequence.target_context + block * kBlock) * D + piece * 16;
-    #pragma unroll
-    for (int p = 0; p < kPasses; ++p) {
-        const uint32_t r = p * kRows + row;
-        if (r >= rows) continue;
-        const float ratio = scale > 0.0f ? __fdiv_rn(old[p], scale) : 0.0f;
-        *reinterpret_cast<uint4*>(to + size_t(r) * D) = recode16<CODE>(v[p], ratio);
-    }
-    if (threadIdx.x == 0)
-        reinterpret_cast<float*>(sequence.target + size_t(planes) * sequence.target_context * D)[size_t(plane) * (sequence.target_context / kBlock) + block] = scale;
 }
 
 static void launch_move(Device& d, uint64_t dim, int code, const EvictArgs& args, uint32_t units) {
@@ -285,8 +302,12 @@ static void evict(Device& d, const void* const* states, const uint64_t* contexts
         args.kv_heads = uint32_t(kv_heads); args.keep = uint32_t(keep); args.sinks = uint32_t(sinks); args.recent = uint32_t(recent);
         args.kept = kept + at * kv_heads * keep;
         uint64_t units = 0, longest = 0;
+        // Four target blocks a thread block where there are enough of them to fill the SMs all the same (sixteen an SM run at once), else one
+        uint64_t blocks = 0;
+        for (uint64_t s = at; s < sequences && s < at + kSequences; ++s) blocks += (std::min(lengths[s], keep) + kBlock - 1) / kBlock * 2 * kv_heads;
+        args.each = blocks >= uint64_t(d.sms) * 16 * 4 ? 4 : 1;
         for (; at < sequences && args.sequences < kSequences; ++at) {
-            const uint64_t more = (std::min(lengths[at], keep) + kBlock - 1) / kBlock * 2 * kv_heads;
+            const uint64_t more = (std::min(lengths[at], keep) + args.each * kBlock - 1) / (args.each * kBlock) * 2 * kv_heads;
             if (units + more >= uint64_t(1) << 31) break;
             args.sequence[args.sequences++] = EvictSequence{static_cast<const uint8_t*>(states[at]), static_cast<uint8_t*>(targets[at]), weights[at],
                                                             target_weights[at], uint32_t(contexts[at]), uint32_t(lengths[at]),
