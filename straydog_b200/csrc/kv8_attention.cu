@@ -9,10 +9,10 @@
 // crosses. No warp waits for another: each has a ring of tiles in shared memory filled by its own 16-byte asynchronous copies, two or more tiles
 // ahead, pieces' borders not minded. (With the pieces cut a block and the eight warps' sums joined in shared memory, every piece cost its block
 // about 5 us of barriers and first loads: 78 us for 16 sequences of 4 rows and 167 MB.) The arithmetic is on mma.sync (16 keys x 8 queries x
-// 16 columns): int8 and E4M3 codes become FP16 exactly by byte permutes; the blocks' scales multiply scores and weighted sums in FP32. Softmax is
+// 16 columns): int8 and E4M3 codes become FP16 exactly by byte permutes; the keys' scales multiply the scores in FP32, the values' scales join the weights' exponent. Softmax is
 // online, in the exp2 domain. Queries enter as FP16: BF16 rows are multiplied by a power of two that brings their largest value to 2^14 (exact),
-// undone on the scores. Weights enter the value product as FP16 at 2^10 times their size (the running maximum has 2^10): 11 bits down to 2^-24 of
-// the largest. A piece that is all of its (sequence, K/V head) writes the output, the others leave FP32 partials that a second kernel joins in
+// undone on the scores. Weights (times their value scale) enter the value product as FP16 at 2^10 times their size (the running maximum has 2^10):
+// 11 bits down to 2^-24 of the largest. A piece that is all of its (sequence, K/V head) writes the output, the others leave FP32 partials that a second kernel joins in
 // order. Where a piece is cut depends on the batch, the order of the sums inside it does not.
 #include "kv8.cuh"
 #include "masked_attention.cuh"
@@ -250,6 +250,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
             const uint8_t* kt = ring + slot * S::kSlot;
             const uint32_t vt = ring_address + slot * S::kSlot + S::kPlane;
             const float k_scale = ring_scales[slot * 2], v_scale = ring_scales[slot * 2 + 1];
+            // The values' scale joins the weights' exponent: the products with the codes then need no scaling of their own, and the sum of the plain
+            // weights is the tile's sum over the scale (a scale of 0 stands over zero codes: any other serves).
+            const float v_log = v_scale > 0.0f ? __log2f(v_scale) : 0.0f, v_inverse = v_scale > 0.0f ? 1.0f / v_scale : 1.0f;
 
             // ---- scores ----
             float x[S::kTile / 16][NT][4];
@@ -285,7 +288,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
                 #pragma unroll
                 for (int h = 0; h < S::kTile / 16; ++h)
                     #pragma unroll
-                    for (int c = 0; c < 4; ++c) x[h][n][c] *= factor[c & 1];
+                    for (int c = 0; c < 4; ++c) x[h][n][c] = fmaf(x[h][n][c], factor[c & 1], a.cap > 0.0f ? 0.0f : v_log);
             }
             if (a.cap > 0.0f) {   // (the cap is in the exp2 domain too)
                 bool small = true;
@@ -301,7 +304,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
                     #pragma unroll
                     for (int n = 0; n < NT; ++n)
                         #pragma unroll
-                        for (int c = 0; c < 4; ++c) x[h][n][c] = a.cap * (all_small ? small_tanh(x[h][n][c]) : any_tanh(x[h][n][c]));
+                        for (int c = 0; c < 4; ++c) x[h][n][c] = fmaf(a.cap, all_small ? small_tanh(x[h][n][c]) : any_tanh(x[h][n][c]), v_log);
             }
             if (a.slopes) {
                 #pragma unroll
@@ -334,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
                         #pragma unroll
                         for (int i = 0; i < 2; ++i)
                             if (8 * n + 2 * t < int(queries_kept))
-                                *reinterpret_cast<float2*>(to + (16 * h + g + 8 * i) * queries_kept + 8 * n + 2 * t) = make_float2(x[h][n][2 * i], x[h][n][2 * i + 1]);
+                                *reinterpret_cast<float2*>(to + (16 * h + g + 8 * i) * queries_kept + 8 * n + 2 * t) = make_float2(x[h][n][2 * i] - v_log, x[h][n][2 * i + 1] - v_log);
             }
             // ---- the running maximum (lifted) and the weights ----
             bool grew = false;
@@ -364,22 +367,19 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
             #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const float u0 = m[n][0] == -INFINITY ? 0.0f : m[n][0], u1 = m[n][1] == -INFINITY ? 0.0f : m[n][1];   // (nothing seen so far: every weight 0)
+                float sum0 = 0.0f, sum1 = 0.0f;
                 #pragma unroll
                 for (int h = 0; h < S::kTile / 16; ++h) {
                     const float p0 = fast_exp2(x[h][n][0] - u0), p1 = fast_exp2(x[h][n][1] - u1), p2 = fast_exp2(x[h][n][2] - u0), p3 = fast_exp2(x[h][n][3] - u1);
-                    l[n][0] += p0 + p2; l[n][1] += p1 + p3;
+                    sum0 += p0 + p2; sum1 += p1 + p3;
                     pf[h][n][0] = movmatrix_trans(pack_half2(p0, p1));
                     pf[h][n][1] = movmatrix_trans(pack_half2(p2, p3));
                 }
+                l[n][0] = fmaf(sum0, v_inverse, l[n][0]); l[n][1] = fmaf(sum1, v_inverse, l[n][1]);
             }
-            // ---- O^T += value scale * V^T P^T: per 32 columns the tile's keys into fresh accumulators, then the scale in FP32 ----
+            // ---- O^T += V^T P^T ----
             #pragma unroll
-            for (int b = 0; b < D / 32; ++b) {
-                float acc[2][NT][4];
-                #pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    #pragma unroll
-                    for (int n = 0; n < NT; ++n) acc[i][n][0] = acc[i][n][1] = acc[i][n][2] = acc[i][n][3] = 0.0f;
+            for (int b = 0; b < D / 32; ++b)
                 #pragma unroll
                 for (int h = 0; h < S::kTile / 16; ++h) {
                     const uint32_t row = v_lane + 16 * h, piece = (2 * b + lane / 16) ^ (D == 64 ? (row >> 1) & 3 : row & 7);
@@ -392,17 +392,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
                     pairs_of<CODE, false>(w[3], ag[2], ag[3]);
                     #pragma unroll
                     for (int n = 0; n < NT; ++n) {
-                        mma_f16(acc[0][n], af, pf[h][n][0], pf[h][n][1]);
-                        mma_f16(acc[1][n], ag, pf[h][n][0], pf[h][n][1]);
+                        mma_f16(o[2 * b][n], af, pf[h][n][0], pf[h][n][1]);
+                        mma_f16(o[2 * b + 1][n], ag, pf[h][n][0], pf[h][n][1]);
                     }
                 }
-                #pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    #pragma unroll
-                    for (int n = 0; n < NT; ++n)
-                        #pragma unroll
-                        for (int c = 0; c < 4; ++c) o[2 * b + i][n][c] = fmaf(v_scale, acc[i][n][c], o[2 * b + i][n][c]);
-            }
             if (++slot == S::kStages) slot = 0;
         }
 
