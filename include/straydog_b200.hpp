@@ -7,6 +7,7 @@
 #include "straydog_gpu_b200.h"
 
 #include <cstdint>
+#include <initializer_list>
 #include <optional>
 #include <stdexcept>
 #include <string>
@@ -119,10 +120,63 @@ class Backend {
     }
     int decode_status() { return check(sdx_decode_status(handle_)); }
 
+    // ---- additions: 8-bit K/V rows with block scales, masked attention, eviction (straydog_gpu_b200.h has the definitions) ----
+    // How scores become weights: a cap (0: none), slopes (device, [heads], or null), a window (0: none), prefixes (empty, or one a sequence).
+    struct Rule {
+        float scale = 1.0f, cap = 0.0f;
+        const float* slopes = nullptr;
+        uint64_t window = 0;
+        std::vector<uint64_t> prefixes;
+    };
+    // Heads of a call and its element type (0 F32, 1 F16, 30 BF16); code: 0 int8, 1 E4M3.
+    struct Shape { uint64_t heads, kv_heads, dim; int code, type; };
+    static uint64_t kv8_bytes(uint64_t context, uint64_t kv_heads, uint64_t dim) {
+        const uint64_t bytes = sdx_kv8_bytes(context, kv_heads, dim);
+        if (!bytes) throw Error(sd_error());
+        return bytes;
+    }
+    void kv8_write(const std::vector<void*>& states, const std::vector<uint64_t>& contexts, const std::vector<uint64_t>& bases,
+                   const std::vector<uint64_t>& steps, const Shape& shape, const void* keys, const void* values, uint64_t stride = 0) {
+        same(states.size(), {contexts.size(), bases.size(), steps.size()});
+        check(sdx_kv8_write(handle_, states.data(), contexts.data(), bases.data(), steps.data(), states.size(), shape.kv_heads, shape.dim, shape.code,
+                            keys, values, stride, shape.type));
+    }
+    void kv8_attention(const std::vector<const void*>& states, const std::vector<uint64_t>& contexts, const std::vector<uint64_t>& lengths,
+                       const std::vector<uint64_t>& rows, const Shape& shape, const Rule& rule, const void* q, void* out,
+                       const std::vector<float*>& weights = {}, uint64_t q_stride = 0, uint64_t out_stride = 0) {
+        same(states.size(), {contexts.size(), lengths.size(), rows.size()});
+        if (!weights.empty()) same(states.size(), {weights.size()});
+        if (!rule.prefixes.empty()) same(states.size(), {rule.prefixes.size()});
+        check(sdx_kv8_attention(handle_, states.data(), contexts.data(), lengths.data(), rows.data(), states.size(), shape.heads, shape.kv_heads,
+                                shape.dim, shape.code, rule.scale, rule.cap, rule.slopes, rule.window, rule.prefixes.empty() ? nullptr : rule.prefixes.data(),
+                                q, q_stride, weights.empty() ? nullptr : weights.data(), out, out_stride, shape.type));
+    }
+    void masked_attention(const void* q, const void* k, const void* v, void* out, const std::vector<uint64_t>& rows, const std::vector<uint64_t>& lengths,
+                          const Shape& shape, const Rule& rule, uint64_t q_stride = 0, uint64_t k_stride = 0, uint64_t v_stride = 0,
+                          uint64_t out_stride = 0) {
+        same(rows.size(), {lengths.size()});
+        if (!rule.prefixes.empty()) same(rows.size(), {rule.prefixes.size()});
+        check(sdx_masked_attention(handle_, q, q_stride, k, k_stride, v, v_stride, rows.data(), lengths.data(), rows.size(), shape.heads, shape.kv_heads,
+                                   shape.dim, shape.type, rule.scale, rule.cap, rule.slopes, rule.window,
+                                   rule.prefixes.empty() ? nullptr : rule.prefixes.data(), out, out_stride));
+    }
+    void kv8_evict(const std::vector<const void*>& states, const std::vector<uint64_t>& contexts, const std::vector<uint64_t>& lengths,
+                   const std::vector<const float*>& weights, uint64_t keep, uint64_t sinks, uint64_t recent, const Shape& shape,
+                   const std::vector<void*>& targets, const std::vector<uint64_t>& target_contexts, const std::vector<float*>& target_weights,
+                   int32_t* kept = nullptr) {
+        same(states.size(), {contexts.size(), lengths.size(), weights.size(), targets.size(), target_contexts.size(), target_weights.size()});
+        check(sdx_kv8_evict(handle_, states.data(), contexts.data(), lengths.data(), weights.data(), states.size(), keep, sinks, recent, shape.kv_heads,
+                            shape.dim, shape.code, targets.data(), target_contexts.data(), target_weights.data(), kept));
+    }
+
   private:
     static int check(int result) {
         if (result < 0) throw Error(sd_error());
         return result;
+    }
+    static void same(size_t count, std::initializer_list<size_t> others) {
+        for (const size_t other : others)
+            if (other != count) throw Error("one entry for each sequence in every list");
     }
     static Buffer made(void* pointer, uint64_t bytes) {
         if (!pointer) throw Error(sd_error());

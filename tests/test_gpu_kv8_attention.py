@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from kv8_util import attention, from_bits, random_state, rounded, state_bytes, to_bits, tolerance
+from kv8_util import State, attention, from_bits, random_state, rounded, state_bytes, to_bits, tolerance
 
 pytestmark = pytest.mark.gpu
 GUARD = 64
@@ -138,8 +138,25 @@ def test_large_and_small_queries(gpu):
         assert np.all(np.abs(got - want) <= tolerance(30, want, size) + (0.5 * size if factor > 1 else 0))
 
 
+@pytest.mark.parametrize("kind", [1, 30])
+@pytest.mark.parametrize("dim,rows", [(64, 1), (128, 3), (256, 1), (64, 200), (128, 90), (256, 150)])
+def test_blocks_whose_scales_are_far_apart(gpu, kind, dim, rows):
+    # values of 2^-8 .. 2^8 from block to block, some blocks zero: the values' scales ride on the weights' exponents
+    rng = np.random.default_rng(dim + rows)
+    n = 400
+    x = rng.normal(size=(2, n, 2, dim)).astype(np.float32)
+    x[1] *= np.exp2(rng.integers(-8, 9, size=(13, 2, 1))).astype(np.float32).repeat(32, 0)[:n]
+    x[:, 64:128] = 0
+    state = State(416, 2, dim, 0).write(0, x[0], x[1])
+    q = rng.normal(size=(rows, 4, dim)).astype(np.float32)
+    got, _, held = attend(gpu, [state], [n], [rows], 4, q, kind)
+    want, _, size = attention(held, *state.values(n), dim ** -0.5)
+    # (a weight times its block's scale, over the largest such product, may lie below what FP16 holds as a normal number: half of 2^-24 a key)
+    floor = 2.0 ** -25 * n * np.abs(state.values(n)[1]).max() if kind == 1 else 0.0
+    assert np.all(np.abs(got - want) <= tolerance(kind, want, size) + floor)
+
+
 def test_zero_states(gpu):
-    from kv8_util import State
     for rows in (1, 100):
         got, _, _ = attend(gpu, [State(128, 1, 64, 0)], [100], [rows], 1, np.ones((rows, 1, 64), np.float32), 1)
         assert np.all(got == 0)
