@@ -438,7 +438,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
 }
 
 // Block = (unit, query): joins the partials of a unit that several warps worked on, and zeroes the rows of a sequence without keys.
-// Few partials (a batch of many sequences): 128 threads, so that all blocks run at once; many (one long sequence): 512.
+// Few partials (a batch of many sequences): 128 threads, so that all blocks run at once (4 verification rows of 16 sequences: 55.0 us against 65.2 with
+// 512; 64 sequences of up to 32768 keys: 197 against 203); many (one long sequence): 512.
 constexpr int kMostWarps = 2048, kFewPieces = 32;   // warps of a launch (eight an SM)
 template<int D, int kJoinThreads>
 __global__ void __launch_bounds__(kJoinThreads) kv8_decode_join_kernel(const __grid_constant__ AttentionArgs a, uint32_t queries_a_unit) {
@@ -660,7 +661,11 @@ template<int D> static void launch_queries(Device& d, AttentionArgs& args, int c
     else launch_decode<D, 1, kE4m3>(d, args, weights);
 }
 
-constexpr uint64_t kFewQueries = 64;   // query rows a K/V head up to which the decode kernel takes a sequence
+// Query rows a K/V head up to which the decode kernel takes a sequence. It reads the codes again for every sixteen (eight) query rows, the prompt kernel
+// unpacks them once to 16 bits. Decode / prompt kernel, int8: 8 heads of 128, 8192 keys, 32 rows 16.6 / 34.0 us, 64 27.3 / 36.1, 128 36.9 / 37.7, 256 59.4 / 40.5;
+// 16 sequences of 4096 keys, 32 rows 65 / 156, 64 119 / 158, 96 166 / 159, 128 216 / 161; 4 heads of 64 alike (64 rows 48 / 67, 96 68 / 68), 2 of 256: 48 rows
+// 67 / 76, 64 86 / 79. One sequence of 1024 keys stays ahead to 256 rows (17.5 / 24.0 us), which a second rule would gain.
+constexpr uint64_t kFewQueries = 64;
 
 static void attention(Device& d, const void* const* states, const uint64_t* contexts, const uint64_t* lengths, const uint64_t* rows,
                       uint64_t sequences, uint64_t heads, uint64_t kv_heads, uint64_t dim, int code, float scale, float cap, const float* slopes,

@@ -302,7 +302,8 @@ static void evict(Device& d, const void* const* states, const uint64_t* contexts
         args.kv_heads = uint32_t(kv_heads); args.keep = uint32_t(keep); args.sinks = uint32_t(sinks); args.recent = uint32_t(recent);
         args.kept = kept + at * kv_heads * keep;
         uint64_t units = 0, longest = 0;
-        // Four target blocks a thread block where there are enough of them to fill the SMs all the same (sixteen an SM run at once), else one
+        // Four target blocks a thread block where there are enough of them to fill the SMs all the same (sixteen an SM run at once), else one: 1024 kept of
+        // 2047 positions 10.8 us by ones, 12.3 by fours; 8192 kept of 16384 of 16 sequences 118.7 by ones, 114.6 by fours
         uint64_t blocks = 0;
         for (uint64_t s = at; s < sequences && s < at + kSequences; ++s) blocks += (std::min(lengths[s], keep) + kBlock - 1) / kBlock * 2 * kv_heads;
         args.each = blocks >= uint64_t(d.sms) * 16 * 4 ? 4 : 1;
@@ -316,7 +317,8 @@ static void evict(Device& d, const void* const* states, const uint64_t* contexts
             longest = std::max(longest, lengths[at]);
         }
         if (!units) continue;   // (every sequence of the group is empty)
-        // Blocks a head: enough for the weights to fit the registers, and twice as many again while the heads leave SMs idle
+        // Blocks a head: enough for the weights to fit the registers, and twice as many again while the heads leave SMs idle (8 heads of 16384 positions
+        // 22.2 us against 25.3 without, four such sequences 42.6 against 49.7, 131072 positions 66 against 77)
         uint32_t ctas = 1;
         const uint64_t heads = args.sequences * kv_heads;
         while (ctas < kMostCluster && longest > uint64_t(ctas) * kSelectThreads * kHeld) ctas *= 2;

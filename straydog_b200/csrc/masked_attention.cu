@@ -5,12 +5,16 @@
 //   s = scale * q . k;  s = cap * tanh(s / cap);  s -= slope[head] * |p - j|;  out = softmax over the seen keys . v, zeros where none is seen
 //
 // A unit is 256 M-rows of one K/V head as two tiles of 128 (one tile for 256 columns): 128 / group consecutive rows times the `group` query heads, so
-// K and V are fetched once for all of them and the diagonal is thin. Its work is the union of its rows' keys in tiles of 128:
-//   S[128 x 128] = Q . K^T    D / 16 tcgen05.mma, Q and K in shared memory (TMA, 128-byte swizzle), FP32 in TMEM
-//   O[128 x D]  += P . V      8 tcgen05.mma, P in TMEM over the columns of its S, V in shared memory
-// Two tiles a unit: while one tile's softmax runs, the tensor pipe works on the other's products. With 256 columns TMEM holds one O and two S,
-// the softmax of one key tile runs beside the products of the next.
-// Persistent blocks, one an SM: the units' tiles laid end to end are cut into equal runs (a unit counts two tiles more, for its first products, its masked
+// K and V are fetched once for all of them and the diagonal is thin. Its work is the union of its rows' keys in tiles of 128, in steps of 64 keys:
+//   S[128 x 64]  = Q . K^T    D / 16 tcgen05.mma, K in shared memory (TMA, 128-byte swizzle), Q there too (256 columns: in TMEM), S FP32 in TMEM
+//   O[128 x D]  += P . V      4 tcgen05.mma, P in TMEM over the columns of its S, V in shared memory
+// S has two buffers a query tile: while the softmax works on one, the next S and the last value product are under way, of the other query tile too.
+// What bounds it: the softmax's issue slots and the tensor pipe, almost evenly. 128 columns: 64 keys of two tiles take 1830 cycles, of which the
+// products fill about 1000 (half the rate: a product of 64 keys reads Q from shared memory twice as often for its flops as one of 128) and
+// a softmax warp 1480 (64 scores a thread: load, maximum, exponential, sum, rounding, store), the rest is hand-over. Steps of 128 keys with
+// one buffer a tile left softmax and products in turn: 285 us for a chunk of 2048 rows over 8192 keys (32 / 8 heads of 128), 238 us now (1.01
+// PFLOP/s); 4096 rows over 16384 keys of 16 / 2 heads of 256 under a cap 824 us (1.17 PFLOP/s), 7 documents of up to 2100 rows 141 us.
+// Persistent blocks, one an SM: the units' tiles laid end to end are cut into equal runs (a unit counts four tiles more, for its first products, its masked
 // tiles and its output). A block walks its run without stopping: the next unit's first products are issued while the last one's output is written. A unit that
 // two or more blocks share leaves FP32 partials for a second kernel. (A block a unit left the last of 1.7 waves a third empty for a chunk of 2048
 // rows, 285 us, and spent half of 184 us on first loads and outputs for packed documents of 8 tiles a unit.)
