@@ -72,7 +72,6 @@ struct Args {
     Shared share[kMostBlocks];
     void* out;
     size_t out_stride;
-    int wide_out;                // output rows on 32-byte boundaries
     const float* slopes;
     const float* block_table;    // 8-bit states: [kv_heads][tiles of four blocks of 32 keys][12]: four key scales, then log2 and inverse of four value scales over the head's largest
     const float* value_top;      // 8-bit states: [sequence][kv_heads] the largest value scale
@@ -178,13 +177,6 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
     return d;
 }
 __device__ __forceinline__ uint64_t both(float x) { return pair(x, x); }
-// small_tanh of two numbers
-__device__ __forceinline__ uint64_t small_tanh2(uint64_t y) {
-    const uint64_t z = mul2(y, y);
-    uint64_t p = fma2(z, both(-17.0f / 315.0f), both(2.0f / 15.0f));
-    p = fma2(p, z, both(-1.0f / 3.0f));
-    return fma2(mul2(p, z), y, y);
-}
 // of two pairs of 16-bit floats, the larger magnitudes; a NaN if either is
 template<bool BF16> __device__ __forceinline__ uint32_t largest(uint32_t a, uint32_t b) {
     uint32_t d;
@@ -192,6 +184,12 @@ template<bool BF16> __device__ __forceinline__ uint32_t largest(uint32_t a, uint
     if (BF16) asm("max.NaN.bf16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
     else asm("max.NaN.f16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
     return d;
+}
+// lanes whose bit BIT is 0 give y for the other's x, the others x for the other's y: a transposition in steps
+template<int BIT> __device__ __forceinline__ void trade(uint32_t& x, uint32_t& y, int lane) {
+    const bool high = lane & BIT;
+    const uint32_t other = __shfl_xor_sync(0xffffffffu, high ? x : y, BIT);
+    if (high) x = other; else y = other;
 }
 // the low `count` bits set (none below 0, all from 32 on)
 __device__ __forceinline__ uint32_t first_bits(int count) { return count <= 0 ? 0u : count >= 32 ? 0xffffffffu : (1u << count) - 1u; }
@@ -236,7 +234,12 @@ struct Unit {
         jump = body - head_tiles;
         tiles = all - jump;
     }
-    __device__ __forceinline__ uint32_t key(uint32_t tile) const { return (tile < head_tiles ? tile : tile + jump) * kStep; }
+    // The last keys come first: where scores fall off with the distance, the maximum then stands after the first tiles. (From the first key on, slopes of
+    // 0.001 to 0.01 made most steps of 4096 rows over 8192 keys move the maximum.)
+    __device__ __forceinline__ uint32_t key(uint32_t tile) const {
+        const uint32_t at = tiles - 1 - tile;
+        return (at < head_tiles ? at : at + jump) * kStep;
+    }
     // whether every row of the unit sees every key of the tile at key0
     __device__ __forceinline__ bool open(const Args& a, uint32_t key0) const {
         const int end_key = int(key0) + kStep - 1;
@@ -410,56 +413,81 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
                 // more than 2^8, where there is none yet, and in tiles with a mask, a cap or a bias, the scores are finished and the maximum found
                 // first, O is multiplied, and the pass runs over what went back to TMEM.
                 bool first = i == 0 || !open;
+                // all keys on one side of all rows: the distance is linear in the key, and its bias starts in the exponent's offset
+                float lean = 0.0f;
+                if (RULE && a.slopes && open) {
+                    if (int(key0) + kStep - 1 <= u.first) lean = slope;
+                    else if (int(key0) >= u.last) lean = -slope;
+                    else first = true;
+                }
                 if (!first) {
                     const float under = top_run == -INFINITY ? 0.0f : top_run - kLift;
-                    uint32_t packed[16 * kGroups];
-                    float top = -INFINITY, sum = 0.0f, steep = 0.0f;
+                    uint32_t loaded[kGroups][32], packed[16 * kGroups];
+                    float top = -INFINITY, sum = 0.0f;
+                    bool steep = false;
+                    #pragma unroll
+                    for (int g = 0; g < kGroups; ++g) tmem_load32(s_base + 32 * g, loaded[g]);
+                    #pragma unroll
+                    for (int g = 0; g < kGroups; ++g) tmem_load_wait(loaded[g]);
                     #pragma unroll
                     for (int g = 0; g < kGroups; ++g) {
-                        uint32_t bits[32];
-                        tmem_load32(s_base + 32 * g, bits);
-                        const float d = shift[g] - under;
-                        float c = a.scale_log2 * to_score[g];
-                        tmem_load_wait(bits);
-                        if (RULE && a.cap > 0.0f) {   // cap * tanh(s / cap), the cap (in the exp2 domain) kept for the exponent's argument
-                            const float inner = a.scale_over_cap * to_score[g];
-                            const uint64_t inner2 = pair(inner, inner);
+                        uint32_t (&bits)[32] = loaded[g];
+                        float most = -INFINITY;
+                        uint64_t sums = both(0.0f);
+                        auto pass = [&](auto cap_too, auto bias_too) {
+                            constexpr bool kCap = decltype(cap_too)::value, kBias = decltype(bias_too)::value;
+                            float d = shift[g] - under;
+                            if (kBias) d = fmaf(-lean, float(position - int(key0) - half * 32 - 32 * g), d);
+                            uint64_t d2 = kBias ? pair(d, d + lean) : both(d);
+                            const float c = a.scale_log2 * to_score[g], inner = kCap ? a.scale_over_cap * to_score[g] : 0.0f;
+                            const uint64_t c1 = both(kCap ? c * kTanh1 : c), c3 = both(c * inner * inner * kTanh3), c5 = both(c * inner * inner * (inner * inner) * kTanh5);
+                            const uint64_t step = both(2.0f * lean);
+                            float farthest = 0.0f;
+                            auto exponents = [&](int n) -> uint64_t {
+                                const uint64_t score = pair(__uint_as_float(bits[2 * n]), __uint_as_float(bits[2 * n + 1]));
+                                uint64_t x;
+                                if (kCap) {   // (the cap and the scale are in the series' coefficients)
+                                    farthest = max3(farthest, fabsf(__uint_as_float(bits[2 * n])), fabsf(__uint_as_float(bits[2 * n + 1])));
+                                    const uint64_t z = mul2(score, score);
+                                    x = fma2(score, fma2(fma2(z, c5, c3), z, c1), d2);
+                                } else {
+                                    x = fma2(score, c1, d2);
+                                }
+                                if (kBias) d2 = add2(d2, step);
+                                return x;
+                            };
+                            auto weights = [&](int n, float x0, float x1) {
+                                x0 = fast_exp2(x0); x1 = fast_exp2(x1);
+                                sums = add2(sums, pair(x0, x1));
+                                packed[16 * g + n] = BF16 ? pack_bf16x2(x0, x1) : pack_half2(x0, x1);
+                            };
+                            // (exponents first and weights then, where the exponents are chains: 428 us against 495 with a bias; plain ones are 2 % faster in one go)
                             #pragma unroll
                             for (int n = 0; n < 16; ++n) {
-                                const uint64_t y = mul2(pair(__uint_as_float(bits[2 * n]), __uint_as_float(bits[2 * n + 1])), inner2);
-                                float y0, y1;
-                                unpair(y, y0, y1);
-                                steep = max3(steep, fabsf(y0), fabsf(y1));
-                                unpair(small_tanh2(y), y0, y1);
-                                bits[2 * n] = __float_as_uint(y0); bits[2 * n + 1] = __float_as_uint(y1);
+                                float x0, x1;
+                                unpair(exponents(n), x0, x1);
+                                most = max3(most, x0, x1);
+                                if (kCap || kBias) { bits[2 * n] = __float_as_uint(x0); bits[2 * n + 1] = __float_as_uint(x1); }
+                                else weights(n, x0, x1);
                             }
-                            c = a.cap;
-                        }
-                        if (RULE && a.slopes) {
-                            const float from = float(position - int(key0) - half * 32 - 32 * g);
-                            #pragma unroll
-                            for (int n = 0; n < 32; ++n) bits[n] = __float_as_uint(fmaf(-slope, fabsf(from - float(n)), __uint_as_float(bits[n]) * c));
-                            c = 1.0f;
-                        }
-                        const uint64_t c2 = pair(c, c), d2 = pair(d, d);
-                        uint64_t sums = pair(0.0f, 0.0f);
-                        float most = -INFINITY;
-                        #pragma unroll
-                        for (int n = 0; n < 16; ++n) {
-                            const uint64_t x = fma2(pair(__uint_as_float(bits[2 * n]), __uint_as_float(bits[2 * n + 1])), c2, d2);
-                            float x0, x1;
-                            unpair(x, x0, x1);
-                            most = max3(most, x0, x1);
-                            x0 = fast_exp2(x0); x1 = fast_exp2(x1);
-                            sums = add2(sums, pair(x0, x1));
-                            packed[16 * g + n] = BF16 ? pack_bf16x2(x0, x1) : pack_half2(x0, x1);
-                        }
+                            if (kCap || kBias) {
+                                #pragma unroll
+                                for (int n = 0; n < 16; ++n) weights(n, __uint_as_float(bits[2 * n]), __uint_as_float(bits[2 * n + 1]));
+                            }
+                            // scores past the series, or so large that its coefficients may have left the normal numbers
+                            if (kCap) steep |= !(fabsf(inner) < 1e4f && farthest <= 1e6f && farthest * fabsf(inner) <= kSmallTanh);
+                        };
+                        using No = std::false_type;
+                        if (!RULE) pass(No{}, No{});
+                        else if (a.cap > 0.0f && a.slopes) pass(std::bool_constant<RULE>{}, std::bool_constant<RULE>{});
+                        else if (a.cap > 0.0f) pass(std::bool_constant<RULE>{}, No{});
+                        else pass(No{}, std::bool_constant<RULE>{});
                         float sum0, sum1;
                         unpair(sums, sum0, sum1);
                         top = fmaxf(top, most - shift[g]);
                         sum = fmaf(sum0 + sum1, to_sum[g], sum);
                     }
-                    first = any_of_rows(top > (top_run == -INFINITY ? -INFINITY : kLift + kRescale) || (RULE && steep > kSmallTanh));
+                    first = any_of_rows(top > (top_run == -INFINITY ? -INFINITY : kLift + kRescale) || (RULE && steep));
                     if (!first) {
                         sum_run += sum;
                         // (over scores that have been read)
@@ -581,7 +609,15 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
             if (T == 1) sum_run += other_half(sum_run, turn++);
             const float lift = a.value_top ? a.value_top[u.s * a.kv_heads + u.kv] : 1.0f;
             const float inverse = !run.whole ? lift : sum_run > 0.0f ? lift / sum_run : sum_run == 0.0f ? 0.0f : sum_run;
-            const size_t slot = ((2 * size_t(blockIdx.x) + (run.begin ? 0 : 1)) * T + tile_of) * kM + m;
+            const size_t slot = (2 * size_t(blockIdx.x) + (run.begin ? 0 : 1)) * T + tile_of;
+            // A thread has a row: four threads trade 16-byte pieces and store four rows' runs of 64 bytes, a lane of theirs a piece. (A row a thread, 32
+            // lines a store, took 5000 cycles a unit, and its partials, written the same way, 12000.)
+            uint16_t* row_at[4];
+            {
+                const uint64_t mine = run.whole && valid ? reinterpret_cast<uint64_t>(static_cast<uint16_t*>(a.out) + (size_t(sequence.first_row) + token) * a.out_stride + size_t(head) * D) : 0;
+                #pragma unroll
+                for (int r = 0; r < 4; ++r) row_at[r] = reinterpret_cast<uint16_t*>(__shfl_sync(0xffffffffu, mine, (lane & 28) + r));
+            }
             const bool patches = tiles && *flagged_piece == piece + 1;
             auto leave = [&] {   // O (and `flagged`) may be written again
                 fence_before();
@@ -617,24 +653,31 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
                         }
                     }
                 }
-                if (!valid) continue;
                 if (!run.whole) {
-                    float4* to = reinterpret_cast<float4*>(a.partial + slot * D + column);
+                    // [eight columns][row][column]: a warp's stores lie one behind the other
+                    float* to = a.partial + (slot * (D / 8) + column / 8) * (kM * 8) + m * 8;
                     #pragma unroll
-                    for (int n = 0; n < 8; ++n) to[n] = make_float4(o[4 * n] * inverse, o[4 * n + 1] * inverse, o[4 * n + 2] * inverse, o[4 * n + 3] * inverse);
+                    for (int n = 0; n < 4; ++n) {
+                        uint32_t w[8];
+                        #pragma unroll
+                        for (int x = 0; x < 8; ++x) w[x] = __float_as_uint(o[8 * n + x] * inverse);
+                        store32(to + n * (kM * 8), w);
+                    }
                 } else {
-                    uint16_t* to = static_cast<uint16_t*>(a.out) + (size_t(sequence.first_row) + token) * a.out_stride + size_t(head) * D + column;
                     uint32_t w[16];
                     #pragma unroll
                     for (int n = 0; n < 16; ++n) w[n] = BF16 ? pack_bf16x2(o[2 * n] * inverse, o[2 * n + 1] * inverse) : pack_half2(o[2 * n] * inverse, o[2 * n + 1] * inverse);
-                    if (a.wide_out) { store32(to, w); store32(to + 16, w + 8); }   // (whole sectors)
-                    else {
-                        #pragma unroll
-                        for (int n = 0; n < 4; ++n) reinterpret_cast<uint4*>(to)[n] = make_uint4(w[4 * n], w[4 * n + 1], w[4 * n + 2], w[4 * n + 3]);
+                    #pragma unroll
+                    for (int x = 0; x < 4; ++x) {
+                        trade<1>(w[x], w[4 + x], lane); trade<1>(w[8 + x], w[12 + x], lane);
+                        trade<2>(w[x], w[8 + x], lane); trade<2>(w[4 + x], w[12 + x], lane);
                     }
+                    #pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (row_at[r]) *reinterpret_cast<uint4*>(row_at[r] + column + (lane & 3) * 8) = make_uint4(w[4 * r], w[4 * r + 1], w[4 * r + 2], w[4 * r + 3]);
                 }
             }
-            if (!run.whole && valid && half == 0) *reinterpret_cast<float2*>(a.sums + slot * 2) = make_float2(top_run, sum_run);
+            if (!run.whole && valid && half == 0) *reinterpret_cast<float2*>(a.sums + (slot * kM + m) * 2) = make_float2(top_run, sum_run);
             if (patches) leave();
             if (tiles) {
                 ++piece;
@@ -809,11 +852,11 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
     }
 }
 
-// Warp = M-row of a shared unit: joins its pieces, in the order of the keys.
+// Joins the pieces of the shared units, in the order the blocks took them: four threads an M-row, eight columns at a time each.
 template<int D, bool BF16>
 __global__ void __launch_bounds__(256) masked_attention_join_kernel(const __grid_constant__ Args a) {
-    constexpr int T = Shape<D>::kTiles, kEach = D / 32;
-    const uint32_t lane = threadIdx.x % 32, index = blockIdx.x * 8 + threadIdx.x / 32, tile = index / kM % T, m = index % kM;
+    constexpr int T = Shape<D>::kTiles, kRuns = D / 32;
+    const uint32_t index = (blockIdx.x * 256 + threadIdx.x) / 4, quarter = threadIdx.x % 4, tile = index / kM % T, m = index % kM;
     const Shared share = a.share[index / (T * kM)];
     Unit u;
     u.find(a, share.unit, T * a.tokens);
@@ -821,28 +864,43 @@ __global__ void __launch_bounds__(256) masked_attention_join_kernel(const __grid
     const uint32_t token = u.row + tile * a.tokens + m / a.group, head = u.kv * a.group + m % a.group;
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (token >= sequence.rows || m >= a.tokens * a.group) return;
-    auto slot = [&](uint32_t p) -> size_t { return ((2 * (size_t(share.first) + p) + (p == 0 ? 1 : 0)) * T + tile) * kM + m; };
-    float top = -INFINITY, weight = 0.0f, total[kEach];
-    #pragma unroll
-    for (int e = 0; e < kEach; ++e) total[e] = 0.0f;
-    for (uint32_t p = 0; p < share.pieces; ++p) top = fmaxf(top, a.sums[slot(p) * 2]);
-    #pragma unroll 2
-    for (uint32_t p = 0; p < share.pieces; ++p) {
-        const float2 v = *reinterpret_cast<const float2*>(a.sums + slot(p) * 2);
-        const float factor = v.x == -INFINITY ? (v.y == 0.0f ? 0.0f : 1.0f) : fast_exp2(v.x - top);   // (scores that are all NaN leave a NaN sum)
-        weight = fmaf(factor, v.y, weight);
-        const float* from = a.partial + slot(p) * D;
+    auto slot = [&](uint32_t p) -> size_t { return (2 * (size_t(share.first) + p) + (p == 0 ? 1 : 0)) * T + tile; };
+    auto sums_of = [&](uint32_t p) -> float2 { return *reinterpret_cast<const float2*>(a.sums + (slot(p) * kM + m) * 2); };
+    auto load = [&](uint32_t p, float4 (&o)[2 * kRuns]) {
+        const float4* from = reinterpret_cast<const float4*>(a.partial + (slot(p) * (D / 8) + quarter) * (kM * 8) + m * 8);
         #pragma unroll
-        for (int e = 0; e < kEach; e += 2) {
-            const float2 o = *reinterpret_cast<const float2*>(from + (e / 2 * 32 + lane) * 2);
-            total[e] = fmaf(factor, o.x, total[e]); total[e + 1] = fmaf(factor, o.y, total[e + 1]);
-        }
-    }
-    const float inverse = weight > 0.0f ? 1.0f / weight : weight == 0.0f ? 0.0f : weight;
-    uint16_t* out = static_cast<uint16_t*>(a.out) + (size_t(sequence.first_row) + token) * a.out_stride + size_t(head) * D;
+        for (int e = 0; e < kRuns; ++e) { o[2 * e] = from[e * kM * 8]; o[2 * e + 1] = from[e * kM * 8 + 1]; }
+    };
+    // (two pieces at least, most often just two: both are asked for before the maximum is known)
+    const float2 first = sums_of(0), second = sums_of(1);
+    float4 total[2 * kRuns], other[2 * kRuns];
+    load(0, total);
+    load(1, other);
+    float top = fmaxf(first.x, second.x);
+    for (uint32_t p = 2; p < share.pieces; ++p) top = fmaxf(top, sums_of(p).x);
+    auto factor_of = [&](float2 v) -> float { return v.x == -INFINITY ? (v.y == 0.0f ? 0.0f : 1.0f) : fast_exp2(v.x - top); };   // (scores that are all NaN leave a NaN sum)
+    const float factor = factor_of(first);
+    float weight = factor * first.y;
     #pragma unroll
-    for (int e = 0; e < kEach; e += 2)
-        *reinterpret_cast<uint32_t*>(out + (e / 2 * 32 + lane) * 2) = BF16 ? pack_bf16x2(total[e] * inverse, total[e + 1] * inverse) : pack_half2(total[e] * inverse, total[e + 1] * inverse);
+    for (int e = 0; e < 2 * kRuns; ++e) { total[e].x *= factor; total[e].y *= factor; total[e].z *= factor; total[e].w *= factor; }
+    auto add = [&](float2 v) {
+        const float f = factor_of(v);
+        weight = fmaf(f, v.y, weight);
+        #pragma unroll
+        for (int e = 0; e < 2 * kRuns; ++e) {
+            total[e].x = fmaf(f, other[e].x, total[e].x); total[e].y = fmaf(f, other[e].y, total[e].y);
+            total[e].z = fmaf(f, other[e].z, total[e].z); total[e].w = fmaf(f, other[e].w, total[e].w);
+        }
+    };
+    add(second);
+    for (uint32_t p = 2; p < share.pieces; ++p) { load(p, other); add(sums_of(p)); }
+    const float inverse = weight > 0.0f ? 1.0f / weight : weight == 0.0f ? 0.0f : weight;
+    uint16_t* out = static_cast<uint16_t*>(a.out) + (size_t(sequence.first_row) + token) * a.out_stride + size_t(head) * D + quarter * 8;
+    auto both_of = [&](float x, float y) -> uint32_t { return BF16 ? pack_bf16x2(x * inverse, y * inverse) : pack_half2(x * inverse, y * inverse); };
+    #pragma unroll
+    for (int e = 0; e < kRuns; ++e)
+        *reinterpret_cast<uint4*>(out + 32 * e) = make_uint4(both_of(total[2 * e].x, total[2 * e].y), both_of(total[2 * e].z, total[2 * e].w),
+                                                            both_of(total[2 * e + 1].x, total[2 * e + 1].y), both_of(total[2 * e + 1].z, total[2 * e + 1].w));
 }
 
 // ---- 8-bit states: codes to 16 bits, exactly, and the blocks' scales in the form the kernel uses ----
@@ -979,7 +1037,7 @@ template<int D, bool BF16> static void launch(Device& d, Args& args, bool behind
         if (uint64_t(units) + uint64_t(q.blocks) * args.kv_heads >= uint64_t(1) << 30) throw std::runtime_error("too many attention rows in one call");
         units += q.blocks * args.kv_heads;
     }
-    // The runs: a unit weighs its tiles and two more. The units of a block of rows, one a K/V head, are alike.
+    // The runs: a unit weighs its tiles and kUnitTiles more. The units of a block of rows, one a K/V head, are alike.
     constexpr uint32_t kUnitTiles = 4;   // what a unit's first products, masked steps and output cost more, in steps
     uint64_t weight = 0;
     auto each_block = [&](auto&& act) {   // act(first unit, tiles of each of its kv_heads units); false ends
@@ -1035,7 +1093,7 @@ template<int D, bool BF16> static void launch(Device& d, Args& args, bool behind
     SDB_CHECK(cudaLaunchKernelEx(&config, args.slopes || args.cap > 0.0f ? masked_attention_kernel<D, BF16, true> : masked_attention_kernel<D, BF16, false>, args));
     ++d.launches;
     if (args.shares) {
-        config.gridDim = dim3(args.shares * S::kTiles * kM / 8);
+        config.gridDim = dim3(args.shares * S::kTiles * kM / 64);
         config.blockDim = dim3(256);
         config.dynamicSmemBytes = 0;
         config.numAttrs = 1;
@@ -1058,7 +1116,6 @@ static Args rule_args(uint64_t heads, uint64_t kv_heads, uint64_t dim, float sca
     args.window = uint32_t(std::min<uint64_t>(window, uint64_t(1) << 30));
     args.out = out; args.out_stride = out_stride; args.slopes = slopes;
     args.queries = static_cast<const uint16_t*>(q); args.query_stride = q_stride;
-    args.wide_out = reinterpret_cast<uintptr_t>(out) % 32 == 0 && out_stride % 16 == 0;
     args.scale_log2 = scale * 1.4426950408889634f;
     args.cap = cap * 1.4426950408889634f;
     args.scale_over_cap = cap > 0.0f ? scale / cap : 0.0f;

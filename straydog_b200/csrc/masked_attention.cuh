@@ -27,6 +27,8 @@ void attend_kv8(Device& d, const std::vector<Sequence>& sequences, uint64_t head
 // tanh(y) in two forms. Up to |y| = 1/4 the odd series to y^9: the next term is below 2^-28 of y, and it runs on the FMA pipe alone. For any y
 // 1 - 2 / (1 + e^(2y)): off by 2^-22 at most (an exponential and a reciprocal of 2^-22 and 2^-23 each).
 constexpr float kSmallTanh = 0.25f;
+// tanh(y) = y (kTanh1 + kTanh3 y^2 + kTanh5 y^4) up to |y| = 1/4, off by 2^-21.1 of it at most: the polynomial of least relative error (by Remez' exchange)
+constexpr float kTanh1 = 0.99999958f, kTanh3 = -0.33321908f, kTanh5 = 0.12841614f;
 __device__ __forceinline__ float small_tanh(float y) {
     const float z = y * y;
     float p = fmaf(z, 62.0f / 2835.0f, -17.0f / 315.0f);
