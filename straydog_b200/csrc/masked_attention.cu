@@ -14,7 +14,7 @@
 // a softmax warp 1480 (64 scores a thread: load, maximum, exponential, sum, rounding, store), the rest is hand-over. Steps of 128 keys with
 // one buffer a tile left softmax and products in turn: 285 us for a chunk of 2048 rows over 8192 keys (32 / 8 heads of 128), 238 us now (1.01
 // PFLOP/s); 4096 rows over 16384 keys of 16 / 2 heads of 256 under a cap 824 us (1.17 PFLOP/s), 7 documents of up to 2100 rows 141 us.
-// Persistent blocks, one an SM: the units' tiles laid end to end are cut into equal runs (a unit counts four tiles more, for its first products, its masked
+// Persistent blocks, one an SM: the units' tiles laid end to end are cut into equal runs (a unit counts three steps more, for its first products, its masked
 // tiles and its output). A block walks its run without stopping: the next unit's first products are issued while the last one's output is written. A unit that
 // two or more blocks share leaves FP32 partials for a second kernel. (A block a unit left the last of 1.7 waves a third empty for a chunk of 2048
 // rows, 285 us, and spent half of 184 us on first loads and outputs for packed documents of 8 tiles a unit.)
@@ -619,24 +619,18 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
                 for (int r = 0; r < 4; ++r) row_at[r] = reinterpret_cast<uint16_t*>(__shfl_sync(0xffffffffu, mine, (lane & 28) + r));
             }
             const bool patches = tiles && *flagged_piece == piece + 1;
-            auto leave = [&] {   // O (and `flagged`) may be written again
-                fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&bars[kOFree + tile_of]);
-            };
-            #pragma unroll 1
-            for (int b = 0; b < kOColumns / 32; ++b) {
-                uint32_t bits[32];
-                float o[32];
-                if (tiles) { tmem_load32(o_base + 32 * b, bits); tmem_load_wait(bits); }
-                #pragma unroll
-                for (int n = 0; n < 32; ++n) o[n] = tiles ? __uint_as_float(bits[n]) : 0.0f;
-                if (b + 1 == kOColumns / 32 && tiles && !patches) leave();
-                const int column = half * kOColumns + 32 * b;
-                if (patches && valid) {
-                    // values that were taken out of a tile: back for the rows that see them (rare: nothing here is fast)
-                    for (int p = 0; p < kFlagged; ++p) {
+            if (patches) {
+                // values that were taken out of a tile: back for the rows that see them (rare: nothing here is fast)
+                #pragma unroll 1
+                for (int b = 0; b < kOColumns / 32; ++b) {
+                    uint32_t bits[32];
+                    tmem_load32(o_base + 32 * b, bits);
+                    tmem_load_wait(bits);
+                    const int column = half * kOColumns + 32 * b;
+                    #pragma unroll 1
+                    for (int p = 0; valid && p < kFlagged; ++p) {
                         const int base = int(flagged[8 * p]);
+                        #pragma unroll 1
                         for (int n = 0; n < kStep; ++n) {
                             if (!(flagged[8 * p + 1 + n / 32] >> (n % 32) & 1)) continue;
                             const int key = base + n;
@@ -648,11 +642,31 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
                                 const float f = BF16 ? __uint_as_float(uint32_t(v[x]) << 16) : __half2float(__ushort_as_half(v[x]));
                                 if (fabsf(f) <= FLT_MAX) continue;
                                 #pragma unroll
-                                for (int y = 0; y < 32; ++y) if (y == x) o[y] += f;   // (no register is addressed by a variable)
+                                for (int y = 0; y < 32; ++y) if (y == x) bits[y] = __float_as_uint(__uint_as_float(bits[y]) + f);   // (no register is addressed by a variable)
                             }
                         }
                     }
+                    __syncwarp();
+                    tmem_store32(o_base + 32 * b, bits);
+                    tmem_store_wait();
                 }
+            }
+            #pragma unroll 1
+            for (int b = 0; b < kOColumns / 32; ++b) {
+                uint32_t bits[32];
+                if (tiles) {
+                    tmem_load32(o_base + 32 * b, bits);
+                    tmem_load_wait(bits);
+                    if (b + 1 == kOColumns / 32) {   // O (and `flagged`) may be written again
+                        fence_before();
+                        __syncwarp();
+                        if (lane == 0) mbar_arrive(&bars[kOFree + tile_of]);
+                    }
+                }
+                float o[32];
+                #pragma unroll
+                for (int n = 0; n < 32; ++n) o[n] = tiles ? __uint_as_float(bits[n]) * inverse : 0.0f;
+                const int column = half * kOColumns + 32 * b;
                 if (!run.whole) {
                     // [eight columns][row][column]: a warp's stores lie one behind the other
                     float* to = a.partial + (slot * (D / 8) + column / 8) * (kM * 8) + m * 8;
@@ -660,13 +674,13 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
                     for (int n = 0; n < 4; ++n) {
                         uint32_t w[8];
                         #pragma unroll
-                        for (int x = 0; x < 8; ++x) w[x] = __float_as_uint(o[8 * n + x] * inverse);
+                        for (int x = 0; x < 8; ++x) w[x] = __float_as_uint(o[8 * n + x]);
                         store32(to + n * (kM * 8), w);
                     }
                 } else {
                     uint32_t w[16];
                     #pragma unroll
-                    for (int n = 0; n < 16; ++n) w[n] = BF16 ? pack_bf16x2(o[2 * n] * inverse, o[2 * n + 1] * inverse) : pack_half2(o[2 * n] * inverse, o[2 * n + 1] * inverse);
+                    for (int n = 0; n < 16; ++n) w[n] = BF16 ? pack_bf16x2(o[2 * n], o[2 * n + 1]) : pack_half2(o[2 * n], o[2 * n + 1]);
                     #pragma unroll
                     for (int x = 0; x < 4; ++x) {
                         trade<1>(w[x], w[4 + x], lane); trade<1>(w[8 + x], w[12 + x], lane);
@@ -678,7 +692,6 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
                 }
             }
             if (!run.whole && valid && half == 0) *reinterpret_cast<float2*>(a.sums + (slot * kM + m) * 2) = make_float2(top_run, sum_run);
-            if (patches) leave();
             if (tiles) {
                 ++piece;
                 used[0] += (tiles + 1) / 2; used[1] += tiles / 2;
@@ -1038,7 +1051,8 @@ template<int D, bool BF16> static void launch(Device& d, Args& args, bool behind
         units += q.blocks * args.kv_heads;
     }
     // The runs: a unit weighs its tiles and kUnitTiles more. The units of a block of rows, one a K/V head, are alike.
-    constexpr uint32_t kUnitTiles = 4;   // what a unit's first products, masked steps and output cost more, in steps
+    // (7 documents of up to 2100 rows: 2 steps 147.6 us, 3 132.9, 4 134.7, 6 139.0)
+    constexpr uint32_t kUnitTiles = 3;   // what a unit's first products, masked steps and output cost more, in steps
     uint64_t weight = 0;
     auto each_block = [&](auto&& act) {   // act(first unit, tiles of each of its kv_heads units); false ends
         for (uint32_t s = 0; s < args.sequences; ++s)
