@@ -28,6 +28,12 @@ using attn::small_tanh;
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
 constexpr float kLift = 10.0f;   // log2 of what weights are multiplied by on their way to FP16
 
+// Query rows a K/V head up to which the decode kernel takes a sequence. It reads the codes again for every sixteen (eight) query rows, the prompt kernel
+// unpacks them once to 16 bits. Decode / prompt kernel, int8: 8 heads of 128, 8192 keys, 32 rows 16.6 / 34.0 us, 64 27.3 / 36.1, 128 36.9 / 37.7, 256 59.4 / 40.5;
+// 16 sequences of 4096 keys, 32 rows 65 / 156, 64 119 / 158, 96 166 / 159, 128 216 / 161; 4 heads of 64 alike (64 rows 48 / 67, 96 68 / 68), 2 of 256: 48 rows
+// 67 / 76, 64 86 / 79. One sequence of 1024 keys stays ahead to 256 rows (17.5 / 24.0 us), which a second rule would gain.
+constexpr uint64_t kFewQueries = 64;
+
 struct AttentionSequence {
     const uint8_t* state;
     float* weights;          // [kv_heads][context] or null
@@ -448,6 +454,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_decode_join_kernel(const __g
     __shared__ float factors[kMost];
     __shared__ float tops[kJoinThreads / 32], weights[kJoinThreads / 32];
     __shared__ float4 totals[kGroups][kColumns];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t unit = blockIdx.x, query = blockIdx.y;
     uint32_t s = 0;
     {
@@ -539,26 +546,28 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_decode_join_kernel(const __g
                                                        : make_uint2(pack_half2(total.x * inverse, total.y * inverse), pack_half2(total.z * inverse, total.w * inverse));
 }
 
-// Thread = (K/V head, seen key): the key's weights over a K/V head's query rows, from the scores the attention left, added to the running sums.
+// Thread = a seen key of the block's (sequence, K/V head): its weights over the K/V head's query rows, from the scores the attention left, added to the
+// running sums. Launched behind the join as its programmatic dependent.
 template<int TILE, int QUERIES>
 __global__ void __launch_bounds__(256) kv8_weights_kernel(const __grid_constant__ AttentionArgs a) {
-    const uint32_t s = blockIdx.y;
-    const AttentionSequence& sequence = a.sequence[s];
-    const uint32_t keys = sequence.tiles * TILE;
-    const uint64_t index = uint64_t(blockIdx.x) * 256 + threadIdx.x;
-    if (index >= uint64_t(keys) * a.kv_heads) return;
-    const uint32_t kv = uint32_t(index / keys), at = uint32_t(index % keys);
+    const AttentionSequence& sequence = a.sequence[blockIdx.y];
+    const uint32_t kv = blockIdx.z, at = blockIdx.x * 256 + threadIdx.x, keys = sequence.tiles * TILE;
     uint32_t tile = at / TILE;
     if (tile >= sequence.head_tiles) tile += sequence.jump;
-    const uint32_t key = tile * TILE + at % TILE;
-    if (key >= sequence.length) return;
+    const uint32_t key = tile * TILE + at % TILE, kept = sequence.score_queries;
+    const bool there = at < keys && key < sequence.length;
+    __shared__ float2 stat[kFewQueries];
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // (in every block, as in the join)
+    if (blockIdx.x * 256 >= keys) return;
+    const uint32_t all = sequence.rows * a.group;
+    if (threadIdx.x < all)
+        stat[threadIdx.x] = reinterpret_cast<const float2*>(a.stats)[size_t(sequence.first_unit + kv * sequence.parts + threadIdx.x / QUERIES) * QUERIES + threadIdx.x % QUERIES];
+    __syncthreads();
+    if (!there) return;
     float total = 0.0f;
-    const uint32_t kept = sequence.score_queries;
     for (uint32_t part = 0; part < sequence.parts; ++part) {
-        const uint32_t inside = kv * sequence.parts + part;
-        const uint32_t queries = min(uint32_t(QUERIES), sequence.rows * a.group - part * QUERIES);
-        const float4* scores = reinterpret_cast<const float4*>(a.scores + sequence.first_score + (uint64_t(inside) * sequence.tiles * TILE + at) * kept);
-        const float2* stats = reinterpret_cast<const float2*>(a.stats) + size_t(sequence.first_unit + inside) * QUERIES;
+        const uint32_t queries = min(uint32_t(QUERIES), all - part * QUERIES);
+        const float4* scores = reinterpret_cast<const float4*>(a.scores + sequence.first_score + (uint64_t(kv * sequence.parts + part) * sequence.tiles * TILE + at) * kept);
         #pragma unroll
         for (int i = 0; i < QUERIES / 4; ++i) {
             if (uint32_t(4 * i) >= queries) break;
@@ -567,13 +576,12 @@ __global__ void __launch_bounds__(256) kv8_weights_kernel(const __grid_constant_
             #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 if (uint32_t(4 * i + c) >= queries) continue;
-                const float2 stat = stats[4 * i + c];
-                if (x[c] != -INFINITY) total = fmaf(fast_exp2(x[c] - stat.x), stat.y, total);
+                const float2 of = stat[part * QUERIES + 4 * i + c];
+                if (x[c] != -INFINITY) total = fmaf(fast_exp2(x[c] - of.x), of.y, total);
             }
         }
     }
-    float* to = sequence.weights + size_t(kv) * sequence.context + key;
-    *to += total;
+    sequence.weights[size_t(kv) * sequence.context + key] += total;
 }
 
 template<int D, int NT, int CODE> static void launch_decode(Device& d, AttentionArgs& args, bool weights) {
@@ -597,7 +605,7 @@ template<int D, int NT, int CODE> static void launch_decode(Device& d, Attention
         score_floats += uint64_t(args.kv_heads) * q.parts * q.tiles * S::kTile * q.score_queries;
         args.units += args.kv_heads * q.parts;
         args.tiles += uint64_t(args.kv_heads) * q.parts * q.tiles;
-        most_keys = std::max(most_keys, uint64_t(q.tiles) * S::kTile * args.kv_heads);
+        most_keys = std::max(most_keys, uint64_t(q.tiles) * S::kTile);
         empty |= !q.tiles;
     }
     // One block an SM; a warp takes a tile at least
@@ -648,7 +656,13 @@ template<int D, int NT, int CODE> static void launch_decode(Device& d, Attention
         ++d.launches;
     }
     if (args.scores) {
-        kv8_weights_kernel<S::kTile, S::kQueries><<<dim3(unsigned((most_keys + 255) / 256), args.sequences), 256, 0, d.stream>>>(args);
+        cudaLaunchConfig_t config{};
+        config.gridDim = dim3(unsigned((most_keys + 255) / 256), args.sequences, args.kv_heads);
+        config.blockDim = dim3(256);
+        config.stream = d.stream;
+        config.attrs = &attribute;
+        config.numAttrs = 1;
+        SDB_CHECK(cudaLaunchKernelEx(&config, kv8_weights_kernel<S::kTile, S::kQueries>, args));
         ++d.launches;
     }
 }
@@ -660,12 +674,6 @@ template<int D> static void launch_queries(Device& d, AttentionArgs& args, int c
     else if (code == kInt8) launch_decode<D, 1, kInt8>(d, args, weights);
     else launch_decode<D, 1, kE4m3>(d, args, weights);
 }
-
-// Query rows a K/V head up to which the decode kernel takes a sequence. It reads the codes again for every sixteen (eight) query rows, the prompt kernel
-// unpacks them once to 16 bits. Decode / prompt kernel, int8: 8 heads of 128, 8192 keys, 32 rows 16.6 / 34.0 us, 64 27.3 / 36.1, 128 36.9 / 37.7, 256 59.4 / 40.5;
-// 16 sequences of 4096 keys, 32 rows 65 / 156, 64 119 / 158, 96 166 / 159, 128 216 / 161; 4 heads of 64 alike (64 rows 48 / 67, 96 68 / 68), 2 of 256: 48 rows
-// 67 / 76, 64 86 / 79. One sequence of 1024 keys stays ahead to 256 rows (17.5 / 24.0 us), which a second rule would gain.
-constexpr uint64_t kFewQueries = 64;
 
 static void attention(Device& d, const void* const* states, const uint64_t* contexts, const uint64_t* lengths, const uint64_t* rows,
                       uint64_t sequences, uint64_t heads, uint64_t kv_heads, uint64_t dim, int code, float scale, float cap, const float* slopes,
