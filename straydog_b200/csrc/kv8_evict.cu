@@ -9,7 +9,7 @@
 // bits, with the weights in registers: a histogram in shared memory of the weights that agree with the bits found so far, summed over the cluster,
 // and the bin where the places run out. A warp whose weights are all in one bin (weights of never-attended rows are all 0) adds them with one
 // atomic. (Sixteen steps of two bits by compares, without atomics, took 65 us for 16 sequences x 8 heads x 16384: eight issue slots a weight and
-// step.) Then ballots give every kept position its place in order.
+// step.) Then ballots give every kept position its place in order. 8192 of 16384 positions of 16 sequences of 8 heads: 23 us, of one sequence 12.
 // kv8_evict_move_kernel: 128 threads a (sequence, plane, one or four target blocks of 32 rows), rows of `dim` bytes gathered: bound by memory as long as the
 // codes' rounding stays under its issue slots (eleven instructions a code with bit masks for E4M3 and a block a target block: 87 % of all issue slots, 101 us
 // for 16 x 16384 positions).
@@ -38,7 +38,7 @@ struct EvictArgs {
 // and back, but for NaN and -0
 __device__ __forceinline__ float weight_of(uint32_t key) { return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key); }
 
-constexpr int kSelectThreads = 1024, kSelectWarps = 32, kHeld = 32, kMostCluster = 8;   // weights a thread holds; blocks a head
+constexpr int kSelectThreads = 1024, kSelectWarps = 32, kHeld = 16, kFewHeld = 4, kMostCluster = 8;   // weights a thread holds; blocks a head
 constexpr int kBins = 2048, kCopies = 4;   // a histogram's bins; copies that a block's warps share out, so that they meet less
 
 // weights in an order of unsigned integers: NaN 0, then -inf .. +inf; the two zeros are equal
@@ -48,11 +48,12 @@ __device__ __forceinline__ uint32_t order_of(float w) {
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-template<bool HELD>
+template<int HELD>   // weights a thread holds in registers; 0: read again in every step
 __global__ void __launch_bounds__(kSelectThreads, 1) kv8_evict_select_kernel(const __grid_constant__ EvictArgs a, uint32_t ctas) {
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
-    __shared__ uint32_t histogram[kCopies][kBins];
+    __shared__ __align__(8) uint32_t histogram[kCopies][kBins];
+    __shared__ __align__(8) uint32_t groups[kSelectWarps];
     __shared__ uint32_t warp_counts[kSelectWarps][2], block_counts[2], found[2];
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t unit = blockIdx.x / ctas, rank = blockIdx.x % ctas, s = unit / a.kv_heads, head = unit % a.kv_heads;
@@ -73,20 +74,28 @@ __global__ void __launch_bounds__(kSelectThreads, 1) kv8_evict_select_kernel(con
     const uint32_t each = (between + ctas * kSelectThreads - 1) / (ctas * kSelectThreads);
     const uint32_t first = (rank * kSelectWarps + warp) * each * 32;
     const float* mine = weights + sinks;
-    uint32_t key[HELD ? kHeld : 1];
-    auto load = [&](uint32_t j) -> uint32_t { const uint32_t i = first + j * 32 + lane; return i < between ? order_of(mine[i]) : 0u; };
+    uint32_t key[HELD ? HELD : 1];
+    auto load = [&](uint32_t j) -> uint32_t { const uint32_t i = first + j * 32 + lane; return i < between ? order_of(__ldg(mine + i)) : 0u; };
     if (HELD) {
+        // (one bound for all, so that the loads go out together: 22000 cycles for 16 weights a thread when each waited for the one before)
+        const uint32_t end = min(between, first + each * 32);
         #pragma unroll
-        for (int j = 0; j < kHeld; ++j) key[j] = uint32_t(j) < each ? load(j) : 0u;
+        for (int j = 0; j < HELD; ++j) {
+            const uint32_t i = first + j * 32 + lane;
+            key[j] = i < end ? __float_as_uint(__ldg(mine + i)) : 0u;
+        }
+        #pragma unroll
+        for (int j = 0; j < HELD; ++j) key[j] = order_of(__uint_as_float(key[j]));
     }
     auto each_key = [&](auto&& act) {
         if (HELD) {
             #pragma unroll
-            for (int j = 0; j < kHeld; ++j) {
+            for (int j = 0; j < HELD; ++j) {
                 if (uint32_t(j) >= each) break;
                 act(uint32_t(j), key[j]);
             }
         } else {
+            #pragma unroll 4
             for (uint32_t j = 0; j < each; ++j) act(j, load(j));
         }
     };
@@ -99,35 +108,52 @@ __global__ void __launch_bounds__(kSelectThreads, 1) kv8_evict_select_kernel(con
         uint32_t* mine_counts = histogram[warp % kCopies];
         each_key([&](uint32_t j, uint32_t k) {
             const bool counts = first + j * 32 + lane < between && (step == 0 || (k >> (shift + bits)) == (last >> (shift + bits)));
+            if (step && !__any_sync(0xffffffffu, counts)) return;   // (most steps of 32, once the upper bits are known)
             const uint32_t bin = counts ? (k >> shift) & ((1u << bits) - 1u) : 0xffffffffu;
             const bool same = __all_sync(0xffffffffu, bin == __shfl_sync(0xffffffffu, bin, 0));
             if (counts && (!same || lane == 0)) atomicAdd(&mine_counts[bin], same ? 32u : 1u);
         });
         __syncthreads();
-        for (int i = threadIdx.x; i < kBins; i += kSelectThreads) {
-            uint32_t sum = 0;
-            #pragma unroll
-            for (int c = 0; c < kCopies; ++c) sum += histogram[c][i];
-            histogram[0][i] = sum;
-        }
-        if (ctas > 1) cluster.sync(); else __syncthreads();
-        // thread t: the bins 2047 - 2t and 2046 - 2t (from the greatest down), over the cluster
-        uint32_t high = 0, low = 0;
-        for (uint32_t r = 0; r < ctas; ++r) {
-            const uint32_t* counts = ctas > 1 ? cluster.map_shared_rank(&histogram[0][0], r) : &histogram[0][0];
-            high += counts[kBins - 1 - 2 * threadIdx.x]; low += counts[kBins - 2 - 2 * threadIdx.x];
-        }
-        uint32_t above = high + low;   // inclusive sums over the threads
+        // the copies' sum, two bins a thread, and the sums of a warp's 64
+        uint2 sum = make_uint2(0, 0);
         #pragma unroll
-        for (int offset = 1; offset < 32; offset *= 2) { const uint32_t other = __shfl_up_sync(0xffffffffu, above, offset); if (lane >= uint32_t(offset)) above += other; }
-        if (lane == 31) warp_counts[warp][0] = above;
-        __syncthreads();
-        above += __reduce_add_sync(0xffffffffu, lane < warp ? warp_counts[lane][0] : 0u);   // the warps before
-        const uint32_t before_high = above - high - low, before_low = above - low;
-        if (before_high < missing && missing <= above) {   // one thread: the places run out in one of its bins
-            const bool in_high = missing <= before_low;
-            found[0] = in_high ? kBins - 1 - 2 * threadIdx.x : kBins - 2 - 2 * threadIdx.x;
-            found[1] = missing - (in_high ? before_high : before_low);
+        for (int c = 0; c < kCopies; ++c) {
+            const uint2 counts = reinterpret_cast<const uint2*>(histogram[c])[threadIdx.x];
+            sum.x += counts.x; sum.y += counts.y;
+        }
+        reinterpret_cast<uint2*>(histogram[0])[threadIdx.x] = sum;
+        const uint32_t group = __reduce_add_sync(0xffffffffu, sum.x + sum.y);
+        if (lane == 0) groups[warp] = group;
+        if (ctas > 1) cluster.sync(); else __syncthreads();
+        if (warp == 0) {
+            // the group where the places run out, then its bin, each over the cluster from the greatest down. (Every bin of every block read by all threads:
+            // 6200 cycles a step with eight blocks.)
+            auto over_cluster = [&](uint2* at) -> uint2 {
+                if (ctas == 1) return *at;
+                uint2 total = make_uint2(0, 0);
+                #pragma unroll
+                for (uint32_t r = 0; r < kMostCluster; ++r) {
+                    const uint2 counts = r < ctas ? *cluster.map_shared_rank(at, r) : make_uint2(0, 0);
+                    total.x += counts.x; total.y += counts.y;
+                }
+                return total;
+            };
+            auto up_to = [&](uint32_t count) -> uint32_t {   // inclusive sums over the lanes
+                #pragma unroll
+                for (int offset = 1; offset < 32; offset *= 2) { const uint32_t other = __shfl_up_sync(0xffffffffu, count, offset); if (lane >= uint32_t(offset)) count += other; }
+                return count;
+            };
+            const uint2 two = over_cluster(reinterpret_cast<uint2*>(groups) + (15 - lane / 2));
+            const uint32_t mine_group = lane & 1 ? two.x : two.y, above_group = up_to(mine_group);
+            const int place = __ffs(__ballot_sync(0xffffffffu, above_group >= missing)) - 1;
+            const uint32_t before = __shfl_sync(0xffffffffu, above_group - mine_group, place), base = (31 - place) * 64;
+            const uint2 bins = over_cluster(reinterpret_cast<uint2*>(&histogram[0][base + 62 - 2 * lane]));
+            const uint32_t above = before + up_to(bins.x + bins.y), before_low = above - bins.x, before_high = before_low - bins.y;
+            if (before_high < missing && missing <= above) {   // one lane
+                const bool in_high = missing <= before_low;
+                found[0] = in_high ? base + 63 - 2 * lane : base + 62 - 2 * lane;
+                found[1] = missing - (in_high ? before_high : before_low);
+            }
         }
         if (ctas > 1) cluster.sync(); else __syncthreads();   // (also: every block has read the others' counts before they are zeroed)
         last |= found[0] << shift;
@@ -149,13 +175,10 @@ __global__ void __launch_bounds__(kSelectThreads, 1) kv8_evict_select_kernel(con
             if (lane == 0) { block_counts[0] = all_reach; block_counts[1] = all_above; }
         }
         if (ctas > 1) cluster.sync();
-        reach = above = 0;
-        for (uint32_t r = 0; r < rank; ++r) {
-            const uint32_t* counts = cluster.map_shared_rank(&block_counts[0], r);
-            reach += counts[0]; above += counts[1];
-        }
-        reach += __reduce_add_sync(0xffffffffu, lane < warp ? warp_counts[lane][0] : 0u);
-        above += __reduce_add_sync(0xffffffffu, lane < warp ? warp_counts[lane][1] : 0u);
+        // (a lane a block before this one, and a lane a warp)
+        const uint32_t* others = lane < rank ? cluster.map_shared_rank(&block_counts[0], lane) : nullptr;
+        reach = __reduce_add_sync(0xffffffffu, (others ? others[0] : 0u) + (lane < warp ? warp_counts[lane][0] : 0u));
+        above = __reduce_add_sync(0xffffffffu, (others ? others[1] : 0u) + (lane < warp ? warp_counts[lane][1] : 0u));
         const uint32_t ties = want ? missing : 0;
         uint32_t equal = reach - above;
         uint32_t place = sinks + above + min(equal, ties);
@@ -318,12 +341,13 @@ static void evict(Device& d, const void* const* states, const uint64_t* contexts
         }
         if (!units) continue;   // (every sequence of the group is empty)
         // Blocks a head: enough for the weights to fit the registers, and twice as many again while the heads leave SMs idle (8 heads of 16384 positions
-        // 22.2 us against 25.3 without, four such sequences 42.6 against 49.7, 131072 positions 66 against 77)
+        // 22.2 us against 25.3 without, four such sequences 42.6 against 49.7, before the clusters' sums got faster: 16.9 and 36.8 now)
         uint32_t ctas = 1;
         const uint64_t heads = args.sequences * kv_heads;
         while (ctas < kMostCluster && longest > uint64_t(ctas) * kSelectThreads * kHeld) ctas *= 2;
         while (ctas < kMostCluster && heads * ctas * 2 <= uint64_t(d.sms) && longest > uint64_t(ctas) * kSelectThreads * 4) ctas *= 2;
-        const bool held = longest <= uint64_t(ctas) * kSelectThreads * kHeld;
+        // Few weights a thread have a kernel of their own, a quarter of the unrolled code: 1024 kept of 2047 positions 9.6 us against 10.8, 4096 of 16384 16.9 against 18.3
+        const uint64_t each = (longest + ctas * kSelectThreads - 1) / (ctas * kSelectThreads);
         cudaLaunchConfig_t config{};
         config.gridDim = dim3(unsigned(heads * ctas));
         config.blockDim = dim3(kSelectThreads);
@@ -333,7 +357,7 @@ static void evict(Device& d, const void* const* states, const uint64_t* contexts
         attribute.val.clusterDim.x = ctas; attribute.val.clusterDim.y = 1; attribute.val.clusterDim.z = 1;
         config.attrs = &attribute;
         config.numAttrs = 1;
-        SDB_CHECK(cudaLaunchKernelEx(&config, held ? kv8_evict_select_kernel<true> : kv8_evict_select_kernel<false>, args, ctas));
+        SDB_CHECK(cudaLaunchKernelEx(&config, each <= kFewHeld ? kv8_evict_select_kernel<kFewHeld> : each <= kHeld ? kv8_evict_select_kernel<kHeld> : kv8_evict_select_kernel<0>, args, ctas));
         ++d.launches;
         launch_move(d, dim, code, args, uint32_t(units));
     }
