@@ -258,7 +258,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
             const float k_scale = ring_scales[slot * 2], v_scale = ring_scales[slot * 2 + 1];
             // The values' scale joins the weights' exponent: the products with the codes then need no scaling of their own, and the sum of the plain
             // weights is the tile's sum over the scale (a scale of 0 stands over zero codes: any other serves).
-            const float v_log = v_scale > 0.0f ? __log2f(v_scale) : 0.0f, v_inverse = v_scale > 0.0f ? 1.0f / v_scale : 1.0f;
+            // Below 2^-96 it counts as that: the sum of plain weights, at 2^10 over the scale each, stays finite, and blocks of almost nothing keep their weight in it.
+            const float v_held = v_scale > 0.0f ? fmaxf(v_scale, 1.262177448e-29f) : 1.0f, v_log = __log2f(v_held), v_inverse = 1.0f / v_held;
 
             // ---- scores ----
             float x[S::kTile / 16][NT][4];

@@ -156,6 +156,24 @@ def test_blocks_whose_scales_are_far_apart(gpu, kind, dim, rows):
     assert np.all(np.abs(got - want) <= tolerance(kind, want, size) + floor)
 
 
+@pytest.mark.parametrize("magnitude", [1e-37, 1e-20, 1e30])
+@pytest.mark.parametrize("dim,rows", [(128, 1), (64, 3), (256, 2), (128, 100), (256, 70)])
+def test_values_near_the_ends_of_fp32(gpu, dim, rows, magnitude):
+    # scales down to subnormal ones, all of a head's or one block's: the sums of weights must not notice
+    rng = np.random.default_rng(dim + rows)
+    n = 200
+    x = rng.normal(size=(2, n, 2, dim)).astype(np.float32)
+    x[1, 64:96, 0] *= np.float32(magnitude)
+    x[1, :, 1] *= np.float32(magnitude)
+    state = State(224, 2, dim, 0).write(0, x[0], x[1])
+    q = rng.normal(size=(rows, 4, dim)).astype(np.float32)
+    got, _, held = attend(gpu, [state], [n], [rows], 4, q, 30)
+    want, _, size = attention(held, *state.values(n), dim ** -0.5)
+    # (without the absolute part of the tolerance, but scales below 2^-96, or 2^-64 of the head's largest, count as that: 127 times it a value)
+    top = np.abs(x[1]).max(axis=(0, 2)).repeat(2)[None, :, None]
+    assert np.all(np.abs(got - want) <= tolerance(30, want, size) - 1e-7 + 127 * 2.0 ** -96 + 2.0 ** -64 * top)
+
+
 def test_zero_states(gpu):
     for rows in (1, 100):
         got, _, _ = attend(gpu, [State(128, 1, 64, 0)], [100], [rows], 1, np.ones((rows, 1, 64), np.float32), 1)
