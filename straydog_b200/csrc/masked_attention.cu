@@ -9,12 +9,13 @@
 //   S[128 x 64]  = Q . K^T    D / 16 tcgen05.mma, K in shared memory (TMA, 128-byte swizzle), Q there too (256 columns: in TMEM), S FP32 in TMEM
 //   O[128 x D]  += P . V      4 tcgen05.mma, P in TMEM over the columns of its S, V in shared memory
 // S has two buffers a query tile: while the softmax works on one, the next S and the last value product are under way, of the other query tile too.
-// What bounds it: the softmax's issue slots and the tensor pipe, almost evenly. 128 columns: 64 keys of two tiles take 1830 cycles, of which the
+// What bounds it: the softmax's issue slots and the tensor pipe, almost evenly. 128 columns: 64 keys of two tiles take 1780 cycles, of which the
 // products fill about 1000 (half the rate: a product of 64 keys reads Q from shared memory twice as often for its flops as one of 128) and
 // a softmax warp 1480 (64 scores a thread: load, maximum, exponential, sum, rounding, store), the rest is hand-over. Steps of 128 keys with
-// one buffer a tile left softmax and products in turn: 285 us for a chunk of 2048 rows over 8192 keys (32 / 8 heads of 128), 238 us now (1.01
-// PFLOP/s); 4096 rows over 16384 keys of 16 / 2 heads of 256 under a cap 824 us (1.17 PFLOP/s), 7 documents of up to 2100 rows 141 us.
-// Persistent blocks, one an SM: the units' tiles laid end to end are cut into equal runs (a unit counts three steps more, for its first products, its masked
+// one buffer a tile left softmax and products in turn: 285 us for a chunk of 2048 rows over 8192 keys (32 / 8 heads of 128), 233 us now (1.03
+// PFLOP/s); 4096 rows over 16384 keys of 16 / 2 heads of 256 under a cap 830 us (1.16 PFLOP/s), 7 documents of up to 2100 rows 132 us. A distance
+// bias or a cap adds FMA work to the softmax: 4096 rows over 8192 keys of 32 / 8 heads of 128 take 385 us, 447 with a bias, 498 with a cap.
+// Persistent blocks, one an SM: the units' steps laid end to end are cut into equal runs (a unit counts three steps more, for its first products, its masked
 // tiles and its output). A block walks its run without stopping: the next unit's first products are issued while the last one's output is written. A unit that
 // two or more blocks share leaves FP32 partials for a second kernel. (A block a unit left the last of 1.7 waves a third empty for a chunk of 2048
 // rows, 285 us, and spent half of 184 us on first loads and outputs for packed documents of 8 tiles a unit.)
