@@ -352,8 +352,8 @@ uint64_t sdx_kv8_bytes(uint64_t context, uint64_t kv_heads, uint64_t dim);
 /* Rows bases[s] .. bases[s] + steps[s] - 1 of every state written from packed rows: keys and values hold the sequences' rows one behind the
    other, [kv_heads][dim] elements of `type` each, `stride` elements apart (0: kv_heads * dim; rows on 16-byte boundaries). Scales: a block whose
    first position is written takes max |x| / top of the call's rows in it; a begun block keeps its scale unless the new rows need a larger
-   one, and then its older codes are rounded again in it (code * old / new, to nearest even). What lies behind the last row is not touched. No
-   state may be listed twice. */
+   one, and then its older codes are rounded again in it (code * old / new, to nearest even). What lies behind the last row is not touched. The
+   states lie apart from one another and from the rows. */
 int sdx_kv8_write(void* handle, void* const* states, const uint64_t* contexts, const uint64_t* bases, const uint64_t* steps,
                   uint64_t sequences, uint64_t kv_heads, uint64_t dim, int code, const void* keys, const void* values, uint64_t stride, int type);
 /* Attention of rows[s] query rows of every sequence over its first lengths[s] positions (the rows' own keys written before). Row i of
@@ -361,7 +361,8 @@ int sdx_kv8_write(void* handle, void* const* states, const uint64_t* contexts, c
    and, with a window, j > p - window, or when j < prefixes[s] (prefixes null: none). Score: x = scale * q . k, then cap * tanh(x / cap) when
    cap > 0, then x - slopes[head] * |p - j| (slopes: [heads] F32 in device memory, or null). out = softmax over the seen positions times the
    values; a row that sees none is 0. q and out: [heads][dim] F16 or BF16 rows, packed in sequence order, q_stride and out_stride elements
-   apart (0: heads * dim), on 16-byte boundaries; out apart from q. heads / kv_heads <= 128. weights (or null): per sequence [kv_heads]
+   apart (0: heads * dim), on 16-byte boundaries; out apart from q, the states and the weights, those apart
+   from one another. heads / kv_heads <= 128. weights (or null): per sequence [kv_heads]
    [contexts[s]] F32, to which every seen position's softmax weight is added, summed over the rows and the heads of its K/V head, for at
    most 64 query rows (rows * heads / kv_heads) a K/V head. Up to 64 such query rows a K/V head run on the decode kernel, more on the prompt
    kernel. A position's codes and scale must have been written. A value scale below 2^-96 (decode) or

@@ -39,12 +39,13 @@ inline void check_state(Device& d, const void* state, uint64_t context, uint64_t
     if (reinterpret_cast<uintptr_t>(state) % 16) throw std::runtime_error("an 8-bit K/V state must be 16-byte aligned");
 }
 
-// A state listed twice would be written by two blocks of one launch.
-inline void check_distinct(const void* const* states, uint64_t sequences) {
-    std::vector<const void*> sorted(states, states + sequences);
-    std::sort(sorted.begin(), sorted.end());
-    if (std::adjacent_find(sorted.begin(), sorted.end()) != sorted.end())
-        throw std::runtime_error("an 8-bit K/V state is listed twice in one batch: its rows would be written twice");
+// What a launch writes lies apart: blocks run in any order.
+using Range = std::pair<uintptr_t, uintptr_t>;
+inline Range range(const void* p, size_t bytes) { return {reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + bytes}; }
+inline void check_apart(std::vector<Range>& written, const char* message) {
+    std::sort(written.begin(), written.end());
+    for (size_t i = 1; i < written.size(); ++i)
+        if (written[i].first < written[i - 1].second) throw std::runtime_error(message);
 }
 
 inline bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {

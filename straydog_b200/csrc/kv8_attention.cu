@@ -697,13 +697,21 @@ static void attention(Device& d, const void* const* states, const uint64_t* cont
         }
         total += rows[s];
     }
-    if (weights) check_distinct(reinterpret_cast<const void* const*>(weights), sequences);
+    if (weights) {
+        std::vector<Range> written;
+        for (uint64_t s = 0; s < sequences; ++s) written.push_back(range(weights[s], kv_heads * contexts[s] * 4));
+        check_apart(written, "attention weights of one call overlap, or are listed twice");
+    }
     if (!total) return;
     attn::check_rows(d, q, total, q_stride, heads * dim, "attention queries");
     attn::check_rows(d, out, total, out_stride, heads * dim, "an attention output");
     if (slopes) span(d, slopes, checked_product({heads, 4}), "attention slopes");
     if (overlap(q, ((total - 1) * q_stride + heads * dim) * 2, out, ((total - 1) * out_stride + heads * dim) * 2))
         throw std::runtime_error("an attention output lies over its queries");
+    const size_t out_bytes = ((total - 1) * out_stride + heads * dim) * 2;
+    for (uint64_t s = 0; s < sequences; ++s)
+        if (overlap(out, out_bytes, states[s], state_bytes(contexts[s], kv_heads, dim)) || (weights && overlap(out, out_bytes, weights[s], kv_heads * contexts[s] * 4)))
+            throw std::runtime_error("an attention output lies over a state or over attention weights");
 
     AttentionArgs args{};
     args.heads = uint32_t(heads); args.kv_heads = uint32_t(kv_heads); args.group = uint32_t(group);

@@ -285,10 +285,7 @@ static void evict(Device& d, const void* const* states, const uint64_t* contexts
         throw std::runtime_error("invalid Straydog eviction");
     if (!keep || keep > (uint64_t(1) << 24) || sinks > keep || recent > keep - sinks)
         throw std::runtime_error("an eviction keeps at least its sinks and its recent positions, at most 2^24");
-    std::vector<std::pair<uintptr_t, uintptr_t>> written, read;
-    auto range = [](std::vector<std::pair<uintptr_t, uintptr_t>>& list, const void* p, size_t bytes) {
-        list.emplace_back(reinterpret_cast<uintptr_t>(p), reinterpret_cast<uintptr_t>(p) + bytes);
-    };
+    std::vector<Range> written, read;
     for (uint64_t s = 0; s < sequences; ++s) {
         check_state(d, states[s], contexts[s], kv_heads, dim);
         check_state(d, targets[s], target_contexts[s], kv_heads, dim);
@@ -299,22 +296,20 @@ static void evict(Device& d, const void* const* states, const uint64_t* contexts
         span(d, target_weights[s], to, "an eviction's target weights");
         if (reinterpret_cast<uintptr_t>(weights[s]) % 4 || reinterpret_cast<uintptr_t>(target_weights[s]) % 4)
             throw std::runtime_error("attention weights must be 4-byte aligned");
-        range(read, states[s], state_bytes(contexts[s], kv_heads, dim));
-        range(read, weights[s], from);
-        range(written, targets[s], state_bytes(target_contexts[s], kv_heads, dim));
-        range(written, target_weights[s], to);
+        read.push_back(range(states[s], state_bytes(contexts[s], kv_heads, dim)));
+        read.push_back(range(weights[s], from));
+        written.push_back(range(targets[s], state_bytes(target_contexts[s], kv_heads, dim)));
+        written.push_back(range(target_weights[s], to));
     }
     if (kept) {
         const size_t bytes = checked_product({sequences, kv_heads, keep, 4});
         span(d, kept, bytes, "an eviction's positions");
         if (reinterpret_cast<uintptr_t>(kept) % 4) throw std::runtime_error("an eviction's positions must be 4-byte aligned");
-        range(written, kept, bytes);
+        written.push_back(range(kept, bytes));
     }
     // what is written lies apart from everything else: rows move between blocks that run in any order
-    std::sort(written.begin(), written.end());
+    check_apart(written, "an eviction's targets overlap");
     std::sort(read.begin(), read.end());
-    for (size_t i = 1; i < written.size(); ++i)
-        if (written[i].first < written[i - 1].second) throw std::runtime_error("an eviction's targets overlap");
     for (size_t i = 0, j = 0; i < read.size(); ++i) {
         while (j < written.size() && written[j].second <= read[i].first) ++j;
         if (j < written.size() && written[j].first < read[i].second) throw std::runtime_error("an eviction's target overlaps what it reads");

@@ -149,7 +149,9 @@ static void write(Device& d, void* const* states, const uint64_t* contexts, cons
     }
     if (!rows) return;
     if (rows >= uint64_t(1) << 31) throw std::runtime_error("too many 8-bit K/V rows in one write");
-    check_distinct(const_cast<const void* const*>(states), sequences);
+    std::vector<Range> written;
+    for (uint64_t s = 0; s < sequences; ++s) written.push_back(range(states[s], state_bytes(contexts[s], kv_heads, dim)));
+    check_apart(written, "8-bit K/V states of one write overlap, or one is listed twice");
     for (const void* from : {keys, values}) {
         span(d, from, (checked_product({rows - 1, stride}) + kv_heads * dim) * size, "8-bit K/V rows to write");
         for (uint64_t s = 0; s < sequences; ++s)

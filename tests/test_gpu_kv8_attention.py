@@ -211,3 +211,23 @@ def test_refusals(gpu):
     assert np.all(gpu.read(out, np.int16, (4 * 8 * 128,)) == 0x5a5a)
     for b in (state, q, out, w, big):
         gpu.release(b)
+
+
+def test_what_is_written_lies_apart(gpu):
+    from straydog_b200.backend import StraydogError
+    size = state_bytes(64, 1, 64)
+    pool = gpu.upload(np.zeros(4 * size, np.uint8))
+    q = gpu.buffer(2 * 64 * 2)
+    one = dict(lengths=[9], rows=[1], heads=1, kv_heads=1, dim=64, code=0, scale=0.1, q=q.pointer, type=1)
+    with pytest.raises(StraydogError, match="over a state"):
+        gpu.kv8_attention([pool], [64], out=pool.at(size - 128), **one)
+    with pytest.raises(StraydogError, match="over attention weights|over a state or"):
+        gpu.kv8_attention([pool], [64], out=pool.at(2 * size), weights=[pool.at(2 * size + 64)], **one)
+    with pytest.raises(StraydogError, match="overlap"):
+        gpu.kv8_attention([pool] * 2, [64] * 2, [9] * 2, [1] * 2, 1, 1, 64, 0, 0.1, q.pointer, pool.at(3 * size), 1, weights=[pool.at(size), pool.at(size + 128)])
+    with pytest.raises(StraydogError, match="overlap"):
+        gpu.kv8_write([pool, pool.at(size - 16)], [64] * 2, [0] * 2, [1] * 2, 1, 64, 0, q.pointer, q.pointer, 1)
+    assert not np.any(gpu.read(pool, np.uint8, (4 * size,)))
+    gpu.kv8_attention([pool], [64], out=pool.at(size), weights=[pool.at(2 * size)], **one)   # (side by side is apart)
+    for b in (pool, q):
+        gpu.release(b)
