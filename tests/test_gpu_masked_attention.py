@@ -145,3 +145,18 @@ def test_refusals(gpu):
     assert np.all(gpu.read(out, np.int16, (8 * 4 * 64,)) == 0x5a5a)
     for b in (q, k, v, out):
         gpu.release(b)
+
+
+@pytest.mark.parametrize("kind", [1, 30])
+@pytest.mark.parametrize("dim,heads,kv_heads", [(64, 8, 1), (128, 4, 2), (256, 4, 1)])
+@pytest.mark.parametrize("cap,size", [(0.0, 1.0), (5.0, 0.5), (50.0, 1.0), (50.0, 20.0)])
+def test_caps_and_biases_over_many_tiles(gpu, kind, dim, heads, kv_heads, cap, size):
+    # slopes of either sign from flat to steep, keys behind, across and ahead of the rows (a prefix past them), scores within and far past the cap's series
+    def spoil(q, k, v):
+        q *= np.float32(size)
+
+    slopes = np.asarray([0.0, 0.004, 0.06, 0.7, -0.003, 0.02, 0.25, -0.0001], np.float32)[:heads]
+    check(gpu, [260, 700, 130], [900, 700, 1100], heads, kv_heads, dim, kind, dim + heads, cap=cap, slopes=slopes, spoil=spoil)
+    check(gpu, [300, 200], [700, 900], heads, kv_heads, dim, kind, dim, prefixes=[640, 900], cap=cap, slopes=slopes, spoil=spoil)
+    check(gpu, [300], [800], heads, kv_heads, dim, kind, dim + 1, cap=cap, window=333, slopes=-slopes, spoil=spoil)
+    check(gpu, [600], [600], heads, kv_heads, dim, kind, dim + 2, cap=cap, spoil=spoil)
