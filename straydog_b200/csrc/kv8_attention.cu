@@ -446,11 +446,13 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
 
 // Block = (unit, query): joins the partials of a unit that several warps worked on, and zeroes the rows of a sequence without keys.
 // Few partials (a batch of many sequences): 128 threads, so that all blocks run at once (4 verification rows of 16 sequences: 55.0 us against 65.2 with
-// 512; 64 sequences of up to 32768 keys: 197 against 203); many (one long sequence): 512.
+// 512; 64 sequences of up to 32768 keys: 197 against 203); many (one long sequence): 512. Where those are few blocks with long sums, four (two) of them share a row's columns: one
+// row of 8192 keys, 16/2 heads of 256 11.5 us against 17.5, 32768 keys 16.0 against 22.0; with 64 partials (1024 keys) 9.0 against 8.1, with 64 query rows
+// 22.8 against 20.8, so from more than 64 partials on, and up to two blocks an SM.
 constexpr int kMostWarps = 2048, kFewPieces = 32;   // warps of a launch (eight an SM)
-template<int D, int kJoinThreads>
+template<int D, int kJoinThreads, int kColumns>   // kColumns: how many of a row's D / 4 pieces a block joins
 __global__ void __launch_bounds__(kJoinThreads) kv8_decode_join_kernel(const __grid_constant__ AttentionArgs a, uint32_t queries_a_unit) {
-    constexpr int kColumns = D / 4, kGroups = kJoinThreads / kColumns;   // threads a partial row, partials at a time
+    constexpr int kRow = D / 4, kGroups = kJoinThreads / kColumns;   // partials at a time
     constexpr int kMost = kJoinThreads == 128 ? kFewPieces : kMostWarps, kSums = (kMost + kJoinThreads - 1) / kJoinThreads;
     __shared__ float factors[kMost];
     __shared__ float tops[kJoinThreads / 32], weights[kJoinThreads / 32];
@@ -468,22 +470,22 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_decode_join_kernel(const __g
     if (global >= sequence.rows * a.group) return;
     uint16_t* out = static_cast<uint16_t*>(a.out) + size_t(sequence.first_row + global / a.group) * a.out_stride + size_t(kv * a.group + global % a.group) * D;
     if (!sequence.tiles) {
-        if (threadIdx.x < kColumns) *reinterpret_cast<uint2*>(out + 4 * threadIdx.x) = make_uint2(0, 0);
+        if (threadIdx.x < kColumns) *reinterpret_cast<uint2*>(out + 4 * (blockIdx.z * kColumns + threadIdx.x)) = make_uint2(0, 0);
         return;
     }
     const uint64_t begin = sequence.first_tile + uint64_t(inside) * sequence.tiles, end = begin + sequence.tiles;
     const uint32_t first = uint32_t(begin / a.tiles_a_warp), pieces = uint32_t((end - 1) / a.tiles_a_warp) - first + 1;
     if (pieces == 1) return;
     const float2* sums = reinterpret_cast<const float2*>(a.sums) + (size_t(first) + unit) * queries_a_unit + query;
-    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, column = threadIdx.x % kColumns, group = threadIdx.x / kColumns;
-    const float4* partial = reinterpret_cast<const float4*>(a.partial + ((size_t(first) + unit) * queries_a_unit + query) * D) + column;
+    const int lane = threadIdx.x % 32, warp = threadIdx.x / 32, column = threadIdx.x % kColumns, group = threadIdx.x / kColumns, from_column = blockIdx.z * kColumns;
+    const float4* partial = reinterpret_cast<const float4*>(a.partial + ((size_t(first) + unit) * queries_a_unit + query) * D) + from_column + column;
     // the first partials are asked for before the maximum is known
     constexpr int kAhead = 4;
     float4 v[kAhead];
     #pragma unroll
     for (int i = 0; i < kAhead; ++i) {
         const uint32_t p = group + i * kGroups;
-        v[i] = p < pieces ? partial[size_t(p) * queries_a_unit * kColumns] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        v[i] = p < pieces ? partial[size_t(p) * queries_a_unit * kRow] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
     float2 mine[kSums];
     float top = -INFINITY;
@@ -522,7 +524,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_decode_join_kernel(const __g
         #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
             const uint32_t p = from + (kAhead + i) * kGroups;
-            next[i] = p < pieces ? partial[size_t(p) * queries_a_unit * kColumns] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            next[i] = p < pieces ? partial[size_t(p) * queries_a_unit * kRow] : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
         }
         #pragma unroll
         for (int i = 0; i < kAhead; ++i) {
@@ -536,14 +538,14 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_decode_join_kernel(const __g
     totals[group][column] = total;
     __syncthreads();
     const float inverse = inverse_of(weight);
-    if (a.scores && threadIdx.x == 0) *reinterpret_cast<float2*>(a.stats + (size_t(unit) * queries_a_unit + query) * 2) = make_float2(top, inverse);
+    if (a.scores && threadIdx.x == 0 && blockIdx.z == 0) *reinterpret_cast<float2*>(a.stats + (size_t(unit) * queries_a_unit + query) * 2) = make_float2(top, inverse);
     if (threadIdx.x >= kColumns) return;
     #pragma unroll
     for (int i = 1; i < kGroups; ++i) {
         const float4 other = totals[i][column];
         total.x += other.x; total.y += other.y; total.z += other.z; total.w += other.w;
     }
-    *reinterpret_cast<uint2*>(out + 4 * column) = a.bf16 ? make_uint2(pack_bf16x2(total.x * inverse, total.y * inverse), pack_bf16x2(total.z * inverse, total.w * inverse))
+    *reinterpret_cast<uint2*>(out + 4 * (from_column + column)) = a.bf16 ? make_uint2(pack_bf16x2(total.x * inverse, total.y * inverse), pack_bf16x2(total.z * inverse, total.w * inverse))
                                                        : make_uint2(pack_half2(total.x * inverse, total.y * inverse), pack_half2(total.z * inverse, total.w * inverse));
 }
 
@@ -588,7 +590,7 @@ __global__ void __launch_bounds__(256) kv8_weights_kernel(const __grid_constant_
 template<int D, int NT, int CODE> static void launch_decode(Device& d, AttentionArgs& args, bool weights) {
     using S = Shape<D, NT>;
     args.units = 0; args.tiles = 0;
-    uint64_t most_keys = 0, score_floats = 0;
+    uint64_t most_keys = 0, score_floats = 0, joined = 0;   // joined: query rows a unit, over the units
     bool empty = false;
     for (uint32_t s = 0; s < args.sequences; ++s) {
         AttentionSequence& q = args.sequence[s];
@@ -605,6 +607,7 @@ template<int D, int NT, int CODE> static void launch_decode(Device& d, Attention
         q.first_score = score_floats;
         score_floats += uint64_t(args.kv_heads) * q.parts * q.tiles * S::kTile * q.score_queries;
         args.units += args.kv_heads * q.parts;
+        joined += uint64_t(args.kv_heads) * q.rows * args.group;
         args.tiles += uint64_t(args.kv_heads) * q.parts * q.tiles;
         most_keys = std::max(most_keys, uint64_t(q.tiles) * S::kTile);
         empty |= !q.tiles;
@@ -647,13 +650,15 @@ template<int D, int NT, int CODE> static void launch_decode(Device& d, Attention
         behind = true;
     }
     if (cut || empty) {
+        const bool few = pieces <= kFewPieces, share = pieces > 64 && joined * (D / 64) <= uint64_t(d.sms) * 2;
         cudaLaunchConfig_t config{};
-        config.gridDim = dim3(args.units, S::kQueries);
-        config.blockDim = dim3(pieces <= kFewPieces ? 128 : 512);
+        config.gridDim = dim3(args.units, S::kQueries, share ? D / 64 : 1);
+        config.blockDim = dim3(few ? 128 : 512);
         config.stream = d.stream;
         config.attrs = &attribute;
         config.numAttrs = behind ? 1 : 0;
-        SDB_CHECK(cudaLaunchKernelEx(&config, pieces <= kFewPieces ? kv8_decode_join_kernel<D, 128> : kv8_decode_join_kernel<D, 512>, args, uint32_t(S::kQueries)));
+        SDB_CHECK(cudaLaunchKernelEx(&config, few ? kv8_decode_join_kernel<D, 128, D / 4> : share ? kv8_decode_join_kernel<D, 512, 16> : kv8_decode_join_kernel<D, 512, D / 4>,
+                                     args, uint32_t(S::kQueries)));
         ++d.launches;
     }
     if (args.scores) {

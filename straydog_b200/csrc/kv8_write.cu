@@ -8,6 +8,8 @@
 // One block of 128 or 256 threads does one (sequence, plane, block of 32): the block's new rows stay in registers between the maximum and the
 // codes, so each value is read once. Bound by memory for a prompt, by one chain of latencies (row, maximum, store) for a single token:
 // then a few threads hold the row and the rest look after the older codes.
+// One row each of 32 sequences of 8 heads of 128 (BF16): 3.5 us; 8191 rows of 2 heads of 256 (F16 to E4M3, 25 MB): 11.1 us, of which the copy rate would
+// take 3.8: the encoding's issue slots and a tail of one wave are the rest.
 #include "kv8.cuh"
 #include "../../include/straydog_gpu_b200.h"
 

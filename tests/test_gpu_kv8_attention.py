@@ -231,3 +231,14 @@ def test_what_is_written_lies_apart(gpu):
     gpu.kv8_attention([pool], [64], out=pool.at(size), weights=[pool.at(2 * size)], **one)   # (side by side is apart)
     for b in (pool, q):
         gpu.release(b)
+
+
+@pytest.mark.parametrize("dim,heads,kv_heads", [(64, 4, 2), (128, 8, 2), (256, 4, 1)])
+@pytest.mark.parametrize("rows", [1, 5])
+def test_one_long_sequence(gpu, dim, heads, kv_heads, rows):
+    # a few rows over many partial sums, and an empty sequence beside it
+    rng = np.random.default_rng(dim + rows)
+    n = 9000
+    states = [random_state(rng, rounded(n), kv_heads, dim, 0, n), random_state(rng, 32, kv_heads, dim, 0, 0)]
+    check(gpu, states, [n, 0], [rows, 2], heads, 30, rng, weights=True)
+    check(gpu, states, [n, 0], [rows, 2], heads, 1, rng, window=5000, cap=20.0)
