@@ -66,6 +66,10 @@ struct AttentionArgs {
 __device__ __forceinline__ void copy16(uint32_t to, const void* from) {
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
+// the first `bytes` (16 or 0) of them, zeros in place of the rest
+__device__ __forceinline__ void copy16_or_zeros(uint32_t to, const void* from, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(bytes) : "memory");
+}
 // 1 / a row's sum of weights; 0 for a row that has seen nothing, NaN for one of NaN scores
 __device__ __forceinline__ float inverse_of(float sum) { return sum > 0.0f ? 1.0f / sum : sum == 0.0f ? 0.0f : sum; }
 __device__ __forceinline__ void copy4(uint32_t to, const void* from) {
@@ -162,7 +166,9 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
             for (int i = 0; i < S::kTile / kStepRows; ++i) {
                 const int row = row0 + i * kStepRows;
                 const int v_piece = D == 64 ? piece0 ^ ((row >> 1) & 3) : piece0 ^ (row & 7);
-                copy16(v_to + row * D + v_piece * 16, v_from + i * 512);
+                // Rows behind the last one hold whatever was there: a weight of 0 times a code that is a NaN in E4M3 (0x7f, 0xff) would be a NaN
+                if (CODE == kE4m3) copy16_or_zeros(v_to + row * D + v_piece * 16, v_from + i * 512, key + row < q.length ? 16u : 0u);
+                else copy16(v_to + row * D + v_piece * 16, v_from + i * 512);
             }
             if (lane < 2) {
                 const float* scales = reinterpret_cast<const float*>(q.state + size_t(2 * a.kv_heads) * q.context * D);
