@@ -402,9 +402,10 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
                 #pragma unroll
                 for (int g = 0; g < kGroups; ++g) { to_score[g] = 1.0f; shift[g] = 0.0f; to_sum[g] = 1.0f; }
                 if (table_at) {
-                    const float* table = table_at + key0 / 128 * 12 + key0 / 64 % 2 * 2;
+                    // (plain loads: the kernel before this one, whose programmatic dependent it is, may still have been writing the table when it was launched)
+                    const volatile float* table = table_at + key0 / 128 * 12 + key0 / 64 % 2 * 2;
                     #pragma unroll
-                    for (int g = 0; g < kGroups; ++g) { to_score[g] = __ldg(table + g); shift[g] = __ldg(table + 4 + g); to_sum[g] = __ldg(table + 8 + g); }
+                    for (int g = 0; g < kGroups; ++g) { to_score[g] = table[g]; shift[g] = table[4 + g]; to_sum[g] = table[8 + g]; }
                 }
                 if (!wait(kSFull + ready, (used[buffer] + (i >> 1)) & 1)) { alive = false; break; }
                 fence_after();
