@@ -24,7 +24,9 @@
 //
 // Roundings: scores, maxima, sums and O are FP32. P is rounded to the operands' type once (FP16 or BF16), at 2^7 times its size so that FP16 keeps
 // 11 bits down to 2^-21 of the largest weight. O is multiplied in TMEM only when a row's maximum grew by more than 2^8. The keys' scales of an 8-bit
-// state multiply the scores, a block of 32 a factor; the values' scales, relative to the largest of the K/V head, join the exponent of P.
+// state multiply the scores, a block of 32 a factor; the values' scales join the exponent of P, and the running maximum is that of a weight times its
+// value's scale, so that P has its bits for what the row sees, however large the values are that it does not see or gives no weight. (The maximum of the
+// weights alone, with scales relative to the head's largest: a block of values 2^23 times the others, behind a row's window, left the row's FP16 P nothing.)
 //
 // A weight of 0 times a value that is infinite or NaN is NaN. In tiles where some row does not see some key (the diagonal, a border), a warp
 // replaces such values by 0 before the product reads them; the rows that do see them get them back at the end. What no row sees does not reach it.
@@ -74,8 +76,7 @@ struct Args {
     void* out;
     size_t out_stride;
     const float* slopes;
-    const float* block_table;    // 8-bit states: [kv_heads][tiles of four blocks of 32 keys][12]: four key scales, then log2 and inverse of four value scales over the head's largest
-    const float* value_top;      // 8-bit states: [sequence][kv_heads] the largest value scale
+    const float* block_table;    // 8-bit states: [kv_heads][tiles of four blocks of 32 keys][12]: four key scales, log2 of four value scales (from a floor up), the rests below it
     uint32_t table_blocks;
     const uint16_t* queries;     // the query rows again, where they do not come through the map
     size_t query_stride;
@@ -146,6 +147,9 @@ __device__ __forceinline__ void tmem_store16(uint32_t address, const uint32_t* r
 }
 __device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// (plain loads: see where the table is read)
+__device__ __forceinline__ void load_factors(const float* from, float (&v)[1]) { asm volatile("ld.global.f32 %0, [%1];" : "=f"(v[0]) : "l"(from) : "memory"); }
+__device__ __forceinline__ void load_factors(const float* from, float (&v)[2]) { asm volatile("ld.global.v2.f32 {%0, %1}, [%2];" : "=f"(v[0]), "=f"(v[1]) : "l"(from) : "memory"); }
 __device__ __forceinline__ void store32(void* to, const uint32_t* w) {
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), SDB_I8(w, 0) : "memory");
 }
@@ -391,21 +395,28 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
             const bool valid = token < sequence.rows && uint32_t(m) < a.tokens * a.group;
             const int position = u.length - int(sequence.rows) + int(token);
             const float slope = RULE && a.slopes && valid ? a.slopes[head] * 1.4426950408889634f : 0.0f;
-            // 8-bit states: a tile's factors are 12 floats, [scores' | weights' log2 | sums'] x [four groups of 32 keys]
+            // 8-bit states: a tile's factors are 12 floats, [scores' | weights' log2 | rests] x [four groups of 32 keys]
             const float* table_at = a.block_table ? a.block_table + (size_t(u.kv) * a.table_blocks + sequence.first_block) * 3 + half : nullptr;
             float top_run = -INFINITY, sum_run = 0.0f;
             #pragma unroll 1
             for (uint32_t i = 0; i < tiles; ++i) {
                 const uint32_t key0 = u.key(run.begin + i);
                 const int buffer = int(i & 1), ready = 2 * tile_of + buffer;
-                float to_score[kGroups], shift[kGroups], to_sum[kGroups];
+                float to_score[kGroups], shift[kGroups], to_sum[kGroups], rest[kGroups];
+                bool rests = false;
                 #pragma unroll
-                for (int g = 0; g < kGroups; ++g) { to_score[g] = 1.0f; shift[g] = 0.0f; to_sum[g] = 1.0f; }
+                for (int g = 0; g < kGroups; ++g) { to_score[g] = 1.0f; shift[g] = 0.0f; to_sum[g] = 1.0f; rest[g] = 1.0f; }
                 if (table_at) {
                     // (plain loads: the kernel before this one, whose programmatic dependent it is, may still have been writing the table when it was launched)
-                    const volatile float* table = table_at + key0 / 128 * 12 + key0 / 64 % 2 * 2;
+                    const float* table = table_at + key0 / 128 * 12 + key0 / 64 % 2 * 2;
+                    load_factors(table, to_score); load_factors(table + 4, shift); load_factors(table + 8, rest);
                     #pragma unroll
-                    for (int g = 0; g < kGroups; ++g) { to_score[g] = table[g]; shift[g] = table[4 + g]; to_sum[g] = table[8 + g]; }
+                    for (int g = 0; g < kGroups; ++g) { to_sum[g] = fast_exp2(-shift[g]); rests |= rest[g] != 1.0f; }
+                    if (T == 1) {   // (the two threads of a row go the same way: they meet at barriers)
+                        float other[1];
+                        load_factors(table + 8 + 1 - 2 * half, other);
+                        rests |= other[0] != 1.0f;
+                    }
                 }
                 if (!wait(kSFull + ready, (used[buffer] + (i >> 1)) & 1)) { alive = false; break; }
                 fence_after();
@@ -413,8 +424,8 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
                 const bool open = u.open(a, key0);
                 // Weights are computed from the maximum so far, in one pass over the scores that finds the tile's own on the way. Where that is above by
                 // more than 2^8, where there is none yet, and in tiles with a mask, a cap or a bias, the scores are finished and the maximum found
-                // first, O is multiplied, and the pass runs over what went back to TMEM.
-                bool first = i == 0 || !open;
+                // first, O is multiplied, and the pass runs over what went back to TMEM. (So it does where a value scale lies below the table's floor.)
+                bool first = i == 0 || !open || rests;
                 // all keys on one side of all rows: the distance is linear in the key, and its bias starts in the exponent's offset
                 float lean = 0.0f;
                 if (RULE && a.slopes && open) {
@@ -486,7 +497,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
                         else pass(No{}, std::bool_constant<RULE>{});
                         float sum0, sum1;
                         unpair(sums, sum0, sum1);
-                        top = fmaxf(top, most - shift[g]);
+                        top = fmaxf(top, most);
                         sum = fmaf(sum0 + sum1, to_sum[g], sum);
                     }
                     first = any_of_rows(top > (top_run == -INFINITY ? -INFINITY : kLift + kRescale) || (RULE && steep));
@@ -550,7 +561,8 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
                         float t = __uint_as_float(bits[0]);
                         #pragma unroll
                         for (int n = 1; n < 31; n += 2) t = max3(t, __uint_as_float(bits[n]), __uint_as_float(bits[n + 1]));
-                        top = max3(top, t * c, __uint_as_float(bits[31]) * c);
+                        const float d = of(shift, g);
+                        top = max3(top, fmaf(t, c, d), fmaf(__uint_as_float(bits[31]), c, d));
                     }
                     if (finish) tmem_store_wait();
                     top = fmaxf(top, other_half(top, turn++));
@@ -579,14 +591,23 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
                     for (int g = 0; g < kGroups; ++g) {
                         uint32_t bits[32];
                         tmem_load32(s_base + 32 * g, bits);
-                        const float c = RULE && a.slopes ? 1.0f : RULE && a.cap > 0.0f ? a.cap : a.scale_log2 * of(to_score, g), d = of(shift, g) - under;
+                        const float c = RULE && a.slopes ? 1.0f : RULE && a.cap > 0.0f ? a.cap : a.scale_log2 * of(to_score, g), d = of(shift, g) - under, down = of(rest, g);
                         tmem_load_wait(bits);
                         float sum0 = 0.0f, sum1 = 0.0f;
                         #pragma unroll
                         for (int n = 0; n < 16; ++n) {
                             const float p0 = fast_exp2(fmaf(__uint_as_float(bits[2 * n]), c, d)), p1 = fast_exp2(fmaf(__uint_as_float(bits[2 * n + 1]), c, d));
-                            bits[n] = BF16 ? pack_bf16x2(p0, p1) : pack_half2(p0, p1);
+                            bits[2 * n] = __float_as_uint(p0); bits[2 * n + 1] = __float_as_uint(p1);
                             sum0 += p0; sum1 += p1;
+                        }
+                        if (rests) {
+                            #pragma unroll
+                            for (int n = 0; n < 32; ++n) bits[n] = __float_as_uint(__uint_as_float(bits[n]) * down);
+                        }
+                        #pragma unroll
+                        for (int n = 0; n < 16; ++n) {
+                            const float p0 = __uint_as_float(bits[2 * n]), p1 = __uint_as_float(bits[2 * n + 1]);
+                            bits[n] = BF16 ? pack_bf16x2(p0, p1) : pack_half2(p0, p1);
                         }
                         sum_run = fmaf(sum0 + sum1, of(to_sum, g), sum_run);
                         tmem_store16(s_base + 16 * g, bits);
@@ -609,8 +630,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
             if (tiles && !wait(kPvDone + 2 * tile_of + int(tiles - 1 & 1), (used[tiles - 1 & 1] + ((tiles - 1) >> 1)) & 1)) { alive = false; break; }
             fence_after();
             if (T == 1) sum_run += other_half(sum_run, turn++);
-            const float lift = a.value_top ? a.value_top[u.s * a.kv_heads + u.kv] : 1.0f;
-            const float inverse = !run.whole ? lift : sum_run > 0.0f ? lift / sum_run : sum_run == 0.0f ? 0.0f : sum_run;
+            const float inverse = !run.whole ? 1.0f : sum_run > 0.0f ? 1.0f / sum_run : sum_run == 0.0f ? 0.0f : sum_run;
             const size_t slot = (2 * size_t(blockIdx.x) + (run.begin ? 0 : 1)) * T + tile_of;
             // A thread has a row: four threads trade 16-byte pieces and store four rows' runs of 64 bytes, a lane of theirs a piece. (A row a thread, 32
             // lines a store, took 5000 cycles a unit, and its partials, written the same way, 12000.)
@@ -929,8 +949,11 @@ struct UnpackArgs {
     uint32_t sequences, kv_heads, blocks;
     uint16_t* rows;       // [2 * kv_heads][blocks * 32][D]
     float* table;
-    float* top;
 };
+// Value scales count as 2^-88, or 2^-64 of their head's largest, where they are below: what is missing (`rest`) multiplies P then. So the sum of plain weights
+// (2^15 over the scale each, 2^24 of them) stays finite, and a weight beside a small scale, zero among them, stays in the sum: the exponential of weight times
+// scale is 2^-57 of the row's largest weight's or more.
+constexpr float kLowestScale = -88.0f, kScaleRange = 64.0f;
 
 template<int CODE, bool BF16> __device__ __forceinline__ void unpack4(uint32_t w, uint32_t (&out)[2]) {
     float f[4];
@@ -963,14 +986,12 @@ __global__ void __launch_bounds__(128) kv8_unpack_kernel(const __grid_constant__
         if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = top;
         __syncthreads();
         top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-        if (!(top > 0.0f)) top = 1.0f;
-        if (threadIdx.x == 0) a.top[size_t(blockIdx.x) * a.kv_heads + kv] = top;
+        const float floor = fmaxf(log2f(top) - kScaleRange, kLowestScale);
         float* to = a.table + (size_t(kv) * a.blocks + q.first_block) * 3;
         for (uint32_t i = threadIdx.x; i < q.blocks; i += 128) {
-            // (a block of zeros counts as one of scale `top`: its values add nothing. Below 2^-64 of the largest a value scale is taken as that.)
-            const float ratio = i < real && v[i] > 0.0f ? fmaxf(v[i] / top, 5.421010862427522e-20f) : 1.0f, down = log2f(ratio);
+            const float scale = i < real ? v[i] : 0.0f, exponent = log2f(scale);   // (-inf for a block of zeros: any rest serves)
             float* at = to + i / 4 * 12 + i % 4;
-            at[0] = i < real ? fmaxf(k[i], 1e-30f) : 1e-30f; at[4] = down; at[8] = 1.0f / fast_exp2(down);
+            at[0] = i < real ? fmaxf(k[i], 1e-30f) : 1e-30f; at[4] = fmaxf(exponent, floor); at[8] = scale > 0.0f && exponent < floor ? exp2f(exponent - floor) : 1.0f;
         }
         return;
     }
@@ -1160,13 +1181,12 @@ void attend_kv8(Device& d, const std::vector<Sequence>& sequences, uint64_t head
         }
         unpack.sequences = args.sequences;
         unpack.blocks = uint32_t(blocks);
-        args.block_table = nullptr; args.value_top = nullptr;
+        args.block_table = nullptr;
         if (blocks) {
             const size_t row_bytes = checked_product({2 * kv_heads, blocks, 32, dim, 2}), table_bytes = checked_product({kv_heads, blocks, 12});
-            auto* space = static_cast<uint8_t*>(workspace(d, d.kv8_rows, row_bytes + table_bytes + args.sequences * kv_heads * 4));
+            auto* space = static_cast<uint8_t*>(workspace(d, d.kv8_rows, row_bytes + table_bytes));
             unpack.rows = reinterpret_cast<uint16_t*>(space);
             unpack.table = reinterpret_cast<float*>(space + row_bytes);
-            unpack.top = reinterpret_cast<float*>(space + row_bytes + table_bytes);
             const dim3 grid{unsigned(std::max<uint64_t>(blocks, args.sequences)), unsigned(3 * kv_heads)};
             const bool bf16 = type == kv8::kBf16, int8 = code == kv8::kInt8;
             auto go = [&](auto* kernel) { kernel<<<grid, 128, 0, d.stream>>>(unpack); };
@@ -1178,7 +1198,6 @@ void attend_kv8(Device& d, const std::vector<Sequence>& sequences, uint64_t head
             args.k_map = tensor_map(unpack.rows, bf16, dim, kv_heads, keys, keys * dim, dim, 1, kStep);
             args.v_map = tensor_map(unpack.rows + kv_heads * keys * dim, bf16, dim, kv_heads, keys, keys * dim, dim, 1, kStep);
             args.block_table = unpack.table;
-            args.value_top = unpack.top;
             args.table_blocks = uint32_t(blocks);
         } else {
             args.k_map = args.v_map = args.q_map;   // (no keys: nothing is loaded through them)

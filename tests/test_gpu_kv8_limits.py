@@ -3,7 +3,7 @@ import numpy as np
 import pytest
 
 from kv8_util import EPS, State, attention, evict, from_bits, rounded, state_bytes, to_bits
-from test_gpu_kv8_attention import check
+from test_gpu_kv8_attention import attend, check
 
 pytestmark = pytest.mark.gpu
 
@@ -57,3 +57,38 @@ def test_attention_over_an_eviction_into_memory_of_another_use(gpu, fill, code, 
             gpu.release(b)
     for b in (source, w, target, moved):
         gpu.release(b)
+
+
+# ---- value scales far apart and far down ----
+
+def bound(kind, held, state, length, want, size, heads, lowest=0.0, **rule):
+    """What an output may be off, from what its own row sees: its rounding; the weights' (half a step of FP16 or BF16) and 2^-16 of the sum of |p v| for
+    the FP32 arithmetic, as in kv8_util.tolerance; and, since a weight times its block's scale enters the products at 2^7 times its share of the row's largest
+    or more, half of 2^-24 a key of that (codes of up to 127): 127 * 2^-32 * n of the largest product, which is at most their sum. `lowest`: what a
+    value scale may be off at the low end, 127 times it a value. Outputs below the normal numbers of F16: half of 2^-24."""
+    k, _ = state.values(length)
+    scales = np.repeat(state.scales[state.kv_heads:], 32, 1)[:, :length].T[:, :, None].astype(np.float64)
+    products, _, _ = attention(held, k, np.broadcast_to(scales, (length, state.kv_heads, held.shape[2])), held.shape[2] ** -0.5, **rule)
+    return (EPS[kind] * np.abs(want) + (EPS[kind] + 2.0 ** -16) * size + 127 * 2.0 ** -32 * length * products + 127 * lowest +
+            (2.0 ** -25 if kind == 1 else 0.0))
+
+
+@pytest.mark.parametrize("kind", [1, 30])
+@pytest.mark.parametrize("code", [0, 1])
+@pytest.mark.parametrize("dim,rows", [(64, 300), (128, 290), (256, 70), (128, 7), (64, 1), (256, 2)])
+@pytest.mark.parametrize("where", ["later", "left", "light"])
+def test_a_block_of_large_values_that_a_row_gives_no_weight(gpu, kind, code, dim, rows, where):
+    # one block 2^23 times the others, behind a row's position, left by its window, or at a distance that leaves it nothing
+    rng = np.random.default_rng(dim + rows + code)
+    n, heads, kv_heads = 512, 4, 2
+    x = rng.normal(size=(2, n, kv_heads, dim)).astype(np.float32)
+    x[1] *= 2.0 ** -9
+    large = slice(480, 512) if where == "later" else slice(0, 32)
+    x[1, large] *= 2.0 ** 23
+    state = State(n, kv_heads, dim, code).write(0, x[0], x[1])
+    rule = {"later": {}, "left": dict(window=100), "light": dict(slopes=np.full(heads, 0.6, np.float32))}[where]
+    q = rng.normal(size=(rows, heads, dim)).astype(np.float32)
+    got, _, held = attend(gpu, [state], [n], [rows], heads, q, kind, **rule)
+    want, _, size = attention(held, *state.values(n), dim ** -0.5, **rule)
+    limit = bound(kind, held, state, n, want, size, heads, **rule)
+    assert np.all(np.abs(got - want) <= limit), float((np.abs(got - want) / limit).max())
