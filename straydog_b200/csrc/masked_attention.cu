@@ -514,6 +514,8 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
                         for (int x = 1; x < kGroups; ++x) r = g == x ? v[x] : r;
                         return r;
                     };
+                    // (a block of zero keys has a scale of 0, which a masked score of -inf must not be multiplied by)
+                    auto score_factor = [&](float key_scale) -> float { return fmaxf(a.scale_log2 * key_scale, FLT_TRUE_MIN); };
                     const bool finish = !open || RULE;
                     float top = -INFINITY;
                     #pragma unroll 1
@@ -539,7 +541,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
                             }
                             c = a.cap;
                         } else {
-                            c *= a.scale_log2;
+                            c = score_factor(c);
                         }
                         if (RULE && a.slopes) {
                             const float from = float(position - int(key0) - half * 32 - 32 * g);
@@ -591,7 +593,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
                     for (int g = 0; g < kGroups; ++g) {
                         uint32_t bits[32];
                         tmem_load32(s_base + 32 * g, bits);
-                        const float c = RULE && a.slopes ? 1.0f : RULE && a.cap > 0.0f ? a.cap : a.scale_log2 * of(to_score, g), d = of(shift, g) - under, down = of(rest, g);
+                        const float c = RULE && a.slopes ? 1.0f : RULE && a.cap > 0.0f ? a.cap : score_factor(of(to_score, g)), d = of(shift, g) - under, down = of(rest, g);
                         tmem_load_wait(bits);
                         float sum0 = 0.0f, sum1 = 0.0f;
                         #pragma unroll
@@ -991,7 +993,7 @@ __global__ void __launch_bounds__(128) kv8_unpack_kernel(const __grid_constant__
         for (uint32_t i = threadIdx.x; i < q.blocks; i += 128) {
             const float scale = i < real ? v[i] : 0.0f, exponent = log2f(scale);   // (-inf for a block of zeros: any rest serves)
             float* at = to + i / 4 * 12 + i % 4;
-            at[0] = i < real ? fmaxf(k[i], 1e-30f) : 1e-30f; at[4] = fmaxf(exponent, floor); at[8] = scale > 0.0f && exponent < floor ? exp2f(exponent - floor) : 1.0f;
+            at[0] = i < real ? k[i] : 0.0f; at[4] = fmaxf(exponent, floor); at[8] = scale > 0.0f && exponent < floor ? exp2f(exponent - floor) : 1.0f;
         }
         return;
     }

@@ -92,3 +92,21 @@ def test_a_block_of_large_values_that_a_row_gives_no_weight(gpu, kind, code, dim
     want, _, size = attention(held, *state.values(n), dim ** -0.5, **rule)
     limit = bound(kind, held, state, n, want, size, heads, **rule)
     assert np.all(np.abs(got - want) <= limit), float((np.abs(got - want) / limit).max())
+
+
+# ---- key scales far down ----
+
+@pytest.mark.parametrize("dim,rows", [(64, 1), (128, 4), (256, 1), (64, 80), (128, 100), (256, 70)])
+@pytest.mark.parametrize("size", [1e-20, 1e-31, 1e-34])
+def test_small_keys_under_large_queries(gpu, dim, rows, size):
+    rng = np.random.default_rng(dim + rows)
+    n, heads, kv_heads = 300, 4, 2
+    x = rng.normal(size=(2, n, kv_heads, dim)).astype(np.float32)
+    x[0] *= np.float32(size)
+    state = State(320, kv_heads, dim, 0).write(0, x[0], x[1])
+    q = (rng.normal(size=(rows, heads, dim)) / size).astype(np.float32)
+    for rule in (dict(), dict(cap=3.0), dict(slopes=np.full(heads, 0.01, np.float32), window=150)):
+        got, _, held = attend(gpu, [state], [n], [rows], heads, q, 30, **rule)
+        want, _, total = attention(held, *state.values(n), dim ** -0.5, **rule)
+        limit = bound(30, held, state, n, want, total, heads, **rule)
+        assert np.all(np.abs(got - want) <= limit), float((np.abs(got - want) / limit).max())
