@@ -366,8 +366,8 @@ int sdx_kv8_write(void* handle, void* const* states, const uint64_t* contexts, c
    [contexts[s]] F32, to which every seen position's softmax weight is added, summed over the rows and the heads of its K/V head, for at
    most 64 query rows (rows * heads / kv_heads) a K/V head. Up to 64 such query rows a K/V head run on the decode kernel, more on the prompt
    kernel. A position's codes and scale must have been written. Weights enter the products
-   with the values in 16 bits, relative to the largest product of weight and value scale that the row sees. A value scale below 2^-96 counts as that on the
-   decode kernel; on the prompt kernel values may be off by 2^-113, or by 2^-96 of the largest of their K/V head. */
+   with the values in 16 bits, relative to the largest product of weight and value scale that the row sees: values of blocks whose scale is below 2^-88, or
+   below 2^-64 of their K/V head's largest, may be off by 2^-113, or by 2^-96 of that head's largest value. */
 int sdx_kv8_attention(void* handle, const void* const* states, const uint64_t* contexts, const uint64_t* lengths, const uint64_t* rows,
                       uint64_t sequences, uint64_t heads, uint64_t kv_heads, uint64_t dim, int code, float scale, float cap,
                       const float* slopes, uint64_t window, const uint64_t* prefixes, const void* q, uint64_t q_stride,

@@ -27,6 +27,7 @@ using attn::small_tanh;
 
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
 constexpr float kLift = 10.0f;   // log2 of what weights are multiplied by on their way to FP16
+constexpr float kLowestScale = -88.0f, kScaleRange = 64.0f;   // log2 of the lowest value scale, and below the largest, that weights' exponents take
 
 // Query rows a K/V head up to which the decode kernel takes a sequence. It reads the codes again for every sixteen (eight) query rows, the prompt kernel
 // unpacks them once to 16 bits. Decode / prompt kernel, int8: 8 heads of 128, 8192 keys, 32 rows 16.6 / 34.0 us, 64 27.3 / 36.1, 128 36.9 / 37.7, 256 59.4 / 40.5;
@@ -60,7 +61,7 @@ struct AttentionArgs {
     float* partial;          // [warp + unit][queries][D]: a run's next piece has the next unit, a unit's next piece the next warp
     float* sums;             // [warp + unit][queries][2]: maximum (exp2 domain, lifted), denominator
     float* scores;           // [tile][keys][score_queries] or null
-    float* stats;            // [unit][queries][2]: final maximum and inverse of the sum, for the weights
+    float* stats;            // [unit][queries]: final maximum and log2 of the sum, added, for the weights
 };
 
 __device__ __forceinline__ void copy16(uint32_t to, const void* from) {
@@ -240,7 +241,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
         const int first_position = int(sequence.length) - int(sequence.rows);
         const int open_to = min(first_position, int(sequence.length) - 1), open_from = a.window ? int(sequence.length) - 1 - int(a.window) : -1;
         const int open_prefix = int(sequence.prefix);
-        float o[D / 16][NT][4], m[NT][2], l[NT][2];
+        float o[D / 16][NT][4], m[NT][2], l[NT][2], v_most = -INFINITY;
         #pragma unroll
         for (int n = 0; n < NT; ++n) {
             m[n][0] = m[n][1] = -INFINITY; l[n][0] = l[n][1] = 0.0f;
@@ -264,8 +265,12 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
             const float k_scale = ring_scales[slot * 2], v_scale = ring_scales[slot * 2 + 1];
             // The values' scale joins the weights' exponent: the products with the codes then need no scaling of their own, and the sum of the plain
             // weights is the tile's sum over the scale (a scale of 0 stands over zero codes: any other serves).
-            // Below 2^-96 it counts as that: the sum of plain weights, at 2^10 over the scale each, stays finite, and blocks of almost nothing keep their weight in it.
-            const float v_held = v_scale > 0.0f ? fmaxf(v_scale, 1.262177448e-29f) : 1.0f, v_log = __log2f(v_held), v_inverse = 1.0f / v_held;
+            // Below 2^-88, or 2^-64 of the largest the piece has had, it counts as that, and what is missing comes off the weights' exponents on their way to FP16: the sum of
+            // plain weights, at 2^10 over the scale each, stays finite with 2^24 keys, and blocks of almost nothing keep their weight in it. So do blocks of
+            // zeros, whose maximum must not stand in the way of the others' weights (at a scale of 1 it took all bits of values of 1e-8).
+            const float v_true = __log2f(v_scale);
+            v_most = fmaxf(v_most, v_true);
+            const float v_log = fmaxf(v_true, fmaxf(v_most - kScaleRange, kLowestScale)), v_inverse = fast_exp2(-v_log);
 
             // ---- scores ----
             float x[S::kTile / 16][NT][4];
@@ -370,8 +375,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
             if (__any_sync(0xffffffffu, grew)) {
                 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    const float f0 = m[n][0] == -INFINITY ? 0.0f : fast_exp2(m[n][0] - now[n][0]), f1 = m[n][1] == -INFINITY ? 0.0f : fast_exp2(m[n][1] - now[n][1]);
-                    l[n][0] *= f0; l[n][1] *= f1; m[n][0] = now[n][0]; m[n][1] = now[n][1];
+                    // (the sum in two steps: from a block of zeros to one of large values the factor alone may be too small for FP32, the sum is not)
+                    const float h0 = m[n][0] == -INFINITY ? 0.0f : fast_exp2(0.5f * (m[n][0] - now[n][0])), h1 = m[n][1] == -INFINITY ? 0.0f : fast_exp2(0.5f * (m[n][1] - now[n][1]));
+                    const float f0 = h0 * h0, f1 = h1 * h1;
+                    l[n][0] = l[n][0] * h0 * h0; l[n][1] = l[n][1] * h1 * h1; m[n][0] = now[n][0]; m[n][1] = now[n][1];
                     #pragma unroll
                     for (int i = 0; i < D / 16; ++i) { o[i][n][0] *= f0; o[i][n][1] *= f1; o[i][n][2] *= f0; o[i][n][3] *= f1; }
                 }
@@ -389,6 +396,17 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
                     pf[h][n][1] = movmatrix_trans(pack_half2(p2, p3));
                 }
                 l[n][0] = fmaf(sum0, v_inverse, l[n][0]); l[n][1] = fmaf(sum1, v_inverse, l[n][1]);
+            }
+            if (v_true < v_log) {
+                #pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    const float u0 = (m[n][0] == -INFINITY ? 0.0f : m[n][0]) + (v_log - v_true), u1 = (m[n][1] == -INFINITY ? 0.0f : m[n][1]) + (v_log - v_true);
+                    #pragma unroll
+                    for (int h = 0; h < S::kTile / 16; ++h) {
+                        pf[h][n][0] = movmatrix_trans(pack_half2(fast_exp2(x[h][n][0] - u0), fast_exp2(x[h][n][1] - u1)));
+                        pf[h][n][1] = movmatrix_trans(pack_half2(fast_exp2(x[h][n][2] - u0), fast_exp2(x[h][n][3] - u1)));
+                    }
+                }
             }
             // ---- O^T += V^T P^T ----
             #pragma unroll
@@ -436,7 +454,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
                         const float v0 = o[b][n][i] * inverse, v1 = o[b][n][i + 2] * inverse;
                         *reinterpret_cast<uint32_t*>(to + 16 * b) = a.bf16 ? pack_bf16x2(v0, v1) : pack_half2(v0, v1);
                     }
-                    if (a.scores && g == 0) *reinterpret_cast<float2*>(a.stats + (size_t(at.unit) * S::kQueries + query) * 2) = make_float2(m[n][i], inverse);
+                    if (a.scores && g == 0) a.stats[size_t(at.unit) * S::kQueries + query] = m[n][i] + log2f(l[n][i]);
                 } else {
                     float* to = a.partial + (mine * S::kQueries + query) * D + 2 * g;
                     #pragma unroll
@@ -513,9 +531,9 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_decode_join_kernel(const __g
     for (int i = 0; i < kSums; ++i) {
         const uint32_t p = threadIdx.x + i * kJoinThreads;
         // (nothing seen in a piece: no weight; scores that are all NaN leave a NaN sum, which stays)
-        const float factor = mine[i].y == 0.0f ? 0.0f : mine[i].x == -INFINITY ? 1.0f : fast_exp2(mine[i].x - top);
-        if (p < pieces) factors[p] = factor;
-        weight = fmaf(factor, mine[i].y, weight);
+        const float root = mine[i].y == 0.0f ? 0.0f : mine[i].x == -INFINITY ? 1.0f : fast_exp2(0.5f * (mine[i].x - top));
+        if (p < pieces) factors[p] = root * root;
+        weight = fmaf(root * mine[i].y, root, weight);   // (in two steps, as in the decode kernel)
     }
     #pragma unroll
     for (int offset = 16; offset; offset /= 2) weight += __shfl_xor_sync(0xffffffffu, weight, offset);
@@ -544,7 +562,7 @@ __global__ void __launch_bounds__(kJoinThreads) kv8_decode_join_kernel(const __g
     totals[group][column] = total;
     __syncthreads();
     const float inverse = inverse_of(weight);
-    if (a.scores && threadIdx.x == 0 && blockIdx.z == 0) *reinterpret_cast<float2*>(a.stats + (size_t(unit) * queries_a_unit + query) * 2) = make_float2(top, inverse);
+    if (a.scores && threadIdx.x == 0 && blockIdx.z == 0) a.stats[size_t(unit) * queries_a_unit + query] = top + log2f(weight);
     if (threadIdx.x >= kColumns) return;
     #pragma unroll
     for (int i = 1; i < kGroups; ++i) {
@@ -565,12 +583,12 @@ __global__ void __launch_bounds__(256) kv8_weights_kernel(const __grid_constant_
     if (tile >= sequence.head_tiles) tile += sequence.jump;
     const uint32_t key = tile * TILE + at % TILE, kept = sequence.score_queries;
     const bool there = at < keys && key < sequence.length;
-    __shared__ float2 stat[kFewQueries];
+    __shared__ float stat[kFewQueries];
     asm volatile("griddepcontrol.wait;" ::: "memory");   // (in every block, as in the join)
     if (blockIdx.x * 256 >= keys) return;
     const uint32_t all = sequence.rows * a.group;
     if (threadIdx.x < all)
-        stat[threadIdx.x] = reinterpret_cast<const float2*>(a.stats)[size_t(sequence.first_unit + kv * sequence.parts + threadIdx.x / QUERIES) * QUERIES + threadIdx.x % QUERIES];
+        stat[threadIdx.x] = a.stats[size_t(sequence.first_unit + kv * sequence.parts + threadIdx.x / QUERIES) * QUERIES + threadIdx.x % QUERIES];
     __syncthreads();
     if (!there) return;
     float total = 0.0f;
@@ -585,8 +603,7 @@ __global__ void __launch_bounds__(256) kv8_weights_kernel(const __grid_constant_
             #pragma unroll
             for (int c = 0; c < 4; ++c) {
                 if (uint32_t(4 * i + c) >= queries) continue;
-                const float2 of = stat[part * QUERIES + 4 * i + c];
-                if (x[c] != -INFINITY) total = fmaf(fast_exp2(x[c] - of.x), of.y, total);
+                if (x[c] != -INFINITY) total += fast_exp2(x[c] - stat[part * QUERIES + 4 * i + c]);
             }
         }
     }
@@ -638,7 +655,7 @@ template<int D, int NT, int CODE> static void launch_decode(Device& d, Attention
     args.sums = partial + partial_floats;
     args.scores = args.stats = nullptr;
     if (weights && args.tiles) {
-        args.scores = static_cast<float*>(workspace(d, d.kv8_scores, checked_product({score_floats + uint64_t(args.units) * S::kQueries * 2, 4})));
+        args.scores = static_cast<float*>(workspace(d, d.kv8_scores, checked_product({score_floats + uint64_t(args.units) * S::kQueries, 4})));
         args.stats = args.scores + score_floats;
     }
     static bool configured[64] = {};

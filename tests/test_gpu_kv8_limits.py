@@ -110,3 +110,27 @@ def test_small_keys_under_large_queries(gpu, dim, rows, size):
         want, _, total = attention(held, *state.values(n), dim ** -0.5, **rule)
         limit = bound(30, held, state, n, want, total, heads, **rule)
         assert np.all(np.abs(got - want) <= limit), float((np.abs(got - want) / limit).max())
+
+
+# ---- small values ----
+
+@pytest.mark.parametrize("magnitude", [1e30, 1.0, 1e-8, 1e-20, 1e-30, 1e-34])
+@pytest.mark.parametrize("dim,rows", [(64, 1), (128, 3), (256, 2), (64, 80), (128, 100), (256, 70)])
+@pytest.mark.parametrize("zeros", [slice(0, 32), slice(96, 160), slice(0, 0)])
+def test_small_and_large_values_beside_blocks_of_zeros(gpu, magnitude, dim, rows, zeros):
+    # a block of zeros weighs like any other and takes nothing from the rest; head 1: a few blocks of ones beside the small or large ones
+    rng = np.random.default_rng(dim + rows)
+    n, heads, kv_heads, copies = 1000, 4, 2, 64 if rows < 10 else 1   # (copies: so many tiles that a warp has several)
+    x = rng.normal(size=(2, n, kv_heads, dim)).astype(np.float32)
+    x[1, :, 0] *= np.float32(magnitude)
+    x[1, 32:96, 1] *= np.float32(magnitude)
+    x[1, zeros] = 0
+    state = State(1024, kv_heads, dim, 0).write(0, x[0], x[1])
+    q = rng.normal(size=(copies * rows, heads, dim)).astype(np.float32)
+    got, _, held = attend(gpu, [state] * copies, [n] * copies, [rows] * copies, heads, q, 30)
+    for copy in range(0, copies, 21):
+        at = slice(copy * rows, copy * rows + rows)
+        want, _, size = attention(held[at], *state.values(n), dim ** -0.5)
+        # (half of 2^-24 a key under 2^7 times 2^-88: what a product with a smaller scale may lose of itself)
+        limit = bound(30, held[at], state, n, want, size, heads, lowest=n * 2.0 ** (-25 - 7 - 88))
+        assert np.all(np.abs(got[at] - want) <= limit), (copy, float((np.abs(got[at] - want) / limit).max()))
