@@ -112,6 +112,23 @@ def test_small_keys_under_large_queries(gpu, dim, rows, size):
         assert np.all(np.abs(got - want) <= limit), float((np.abs(got - want) / limit).max())
 
 
+@pytest.mark.parametrize("dim,rows", [(64, 1), (128, 4), (256, 1)])
+def test_the_largest_queries(gpu, dim, rows):
+    # BF16 rows of up to 2^127 over keys of 1e-36
+    rng = np.random.default_rng(dim + rows)
+    n, heads, kv_heads = 300, 4, 2
+    x = rng.uniform(-1, 1, size=(2, n, kv_heads, dim)).astype(np.float32)
+    x[0] *= np.float32(1e-36)
+    state = State(320, kv_heads, dim, 0).write(0, x[0], x[1])
+    q = (rng.uniform(-1, 1, size=(rows, heads, dim)) * 2.0 ** 119).astype(np.float32)
+    q[0, 0] *= 2.0 ** -8
+    q[0, 1, 3] = 1.7e38
+    got, _, held = attend(gpu, [state], [n], [rows], heads, q, 30)
+    want, _, total = attention(held, *state.values(n), dim ** -0.5)
+    limit = bound(30, held, state, n, want, total, heads)
+    assert np.all(np.abs(got - want) <= limit), float((np.abs(got - want) / limit).max())
+
+
 # ---- small values ----
 
 @pytest.mark.parametrize("magnitude", [1e30, 1.0, 1e-8, 1e-20, 1e-30, 1e-34])
