@@ -361,8 +361,8 @@ int sdx_kv8_write(void* handle, void* const* states, const uint64_t* contexts, c
    and, with a window, j > p - window, or when j < prefixes[s] (prefixes null: none). Score: x = scale * q . k, then cap * tanh(x / cap) when
    cap > 0, then x - slopes[head] * |p - j| (slopes: [heads] F32 in device memory, or null). out = softmax over the seen positions times the
    values; a row that sees none is 0. q and out: [heads][dim] F16 or BF16 rows, packed in sequence order, q_stride and out_stride elements
-   apart (0: heads * dim), on 16-byte boundaries; out apart from q, the states and the weights, those apart
-   from one another. heads / kv_heads <= 128. weights (or null): per sequence [kv_heads]
+   apart (0: heads * dim), on 16-byte boundaries; out and the weights apart from one another, q, the
+   slopes and the states. heads / kv_heads <= 128. weights (or null): per sequence [kv_heads]
    [contexts[s]] F32, to which every seen position's softmax weight is added, summed over the rows and the heads of its K/V head, for at
    most 64 query rows (rows * heads / kv_heads) a K/V head. Up to 64 such query rows a K/V head run on the decode kernel, more on the prompt
    kernel. A position's codes and scale must have been written. Weights enter the products

@@ -48,6 +48,15 @@ inline void check_apart(std::vector<Range>& written, const char* message) {
         if (written[i].first < written[i - 1].second) throw std::runtime_error(message);
 }
 
+// (written: sorted and apart, as check_apart leaves them)
+inline void check_apart_from(const std::vector<Range>& written, std::vector<Range>& read, const char* message) {
+    std::sort(read.begin(), read.end());
+    for (size_t i = 0, j = 0; i < read.size(); ++i) {
+        while (j < written.size() && written[j].second <= read[i].first) ++j;
+        if (j < written.size() && written[j].first < read[i].second) throw std::runtime_error(message);
+    }
+}
+
 inline bool overlap(const void* a, size_t a_bytes, const void* b, size_t b_bytes) {
     const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
     return x < y + b_bytes && y < x + a_bytes;

@@ -725,8 +725,8 @@ static void attention(Device& d, const void* const* states, const uint64_t* cont
         }
         total += rows[s];
     }
+    std::vector<Range> written;
     if (weights) {
-        std::vector<Range> written;
         for (uint64_t s = 0; s < sequences; ++s) written.push_back(range(weights[s], kv_heads * contexts[s] * 4));
         check_apart(written, "attention weights of one call overlap, or are listed twice");
     }
@@ -740,6 +740,13 @@ static void attention(Device& d, const void* const* states, const uint64_t* cont
     for (uint64_t s = 0; s < sequences; ++s)
         if (overlap(out, out_bytes, states[s], state_bytes(contexts[s], kv_heads, dim)) || (weights && overlap(out, out_bytes, weights[s], kv_heads * contexts[s] * 4)))
             throw std::runtime_error("an attention output lies over a state or over attention weights");
+    if (weights) {
+        std::vector<Range> read{range(q, ((total - 1) * q_stride + heads * dim) * 2)};
+        if (slopes) read.push_back(range(slopes, heads * 4));
+        for (uint64_t s = 0; s < sequences; ++s) read.push_back(range(states[s], state_bytes(contexts[s], kv_heads, dim)));
+        check_apart_from(written, read, "attention weights overlap a state, the queries or the slopes");
+    }
+    if (slopes && overlap(out, out_bytes, slopes, heads * 4)) throw std::runtime_error("an attention output lies over the slopes");
 
     AttentionArgs args{};
     args.heads = uint32_t(heads); args.kv_heads = uint32_t(kv_heads); args.group = uint32_t(group);

@@ -309,11 +309,7 @@ static void evict(Device& d, const void* const* states, const uint64_t* contexts
     }
     // what is written lies apart from everything else: rows move between blocks that run in any order
     check_apart(written, "an eviction's targets overlap");
-    std::sort(read.begin(), read.end());
-    for (size_t i = 0, j = 0; i < read.size(); ++i) {
-        while (j < written.size() && written[j].second <= read[i].first) ++j;
-        if (j < written.size() && written[j].first < read[i].second) throw std::runtime_error("an eviction's target overlaps what it reads");
-    }
+    check_apart_from(written, read, "an eviction's target overlaps what it reads");
     if (!kept) kept = static_cast<int32_t*>(workspace(d, d.kv8_kept, checked_product({sequences, kv_heads, keep, 4})));
     for (uint64_t at = 0; at < sequences;) {
         EvictArgs args{};

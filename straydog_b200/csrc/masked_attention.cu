@@ -1232,6 +1232,7 @@ static void masked(Device& d, const void* q, uint64_t q_stride, const void* k, u
     if (kv8::overlap(out, out_bytes, q, ((total - 1) * q_stride + heads * dim) * 2) ||
         (keys && (kv8::overlap(out, out_bytes, k, ((keys - 1) * k_stride + kv_heads * dim) * 2) || kv8::overlap(out, out_bytes, v, ((keys - 1) * v_stride + kv_heads * dim) * 2))))
         throw std::runtime_error("an attention output lies over its queries, keys or values");
+    if (slopes && kv8::overlap(out, out_bytes, slopes, heads * 4)) throw std::runtime_error("an attention output lies over the slopes");
     Args args = rule_args(heads, kv_heads, dim, scale, cap, slopes, window, q, total, q_stride, out, out_stride, type);
     args.k_map = keys ? tensor_map(k, type == kv8::kBf16, dim, kv_heads, keys, dim, k_stride, 1, kStep) : args.q_map;
     args.v_map = keys ? tensor_map(v, type == kv8::kBf16, dim, kv_heads, keys, dim, v_stride, 1, kStep) : args.q_map;

@@ -151,3 +151,27 @@ def test_small_and_large_values_beside_blocks_of_zeros(gpu, magnitude, dim, rows
         # (half of 2^-24 a key under 2^7 times 2^-88: what a product with a smaller scale may lose of itself)
         limit = bound(30, held[at], state, n, want, size, heads, lowest=n * 2.0 ** (-25 - 7 - 88))
         assert np.all(np.abs(got[at] - want) <= limit), (copy, float((np.abs(got[at] - want) / limit).max()))
+
+
+# ---- arrays that overlap or lie askew ----
+
+def test_nothing_written_lies_over_what_is_read(gpu):
+    from straydog_b200.backend import StraydogError
+    size = state_bytes(64, 1, 64)
+    pool = gpu.upload(np.zeros(8 * size, np.uint8))
+    one = dict(heads=1, kv_heads=1, dim=64, code=0, scale=0.1, type=1)
+    q, out, slopes, weights = pool.at(2 * size), pool.at(3 * size), pool.at(4 * size), pool.at(5 * size)
+    good = dict(states=[pool], contexts=[64], lengths=[9], rows=[1], q=q, out=out, slopes=slopes, weights=[weights], **one)
+    two = dict(states=[pool, pool.at(size)], contexts=[64] * 2, lengths=[9] * 2, rows=[1] * 2, weights=[weights, pool.at(6 * size)])
+    bad = [dict(weights=[pool.pointer]), dict(weights=[pool.at(2 * 64 * 64)]), dict(weights=[q]), dict(weights=[q + 124]), dict(weights=[slopes]), dict(slopes=out),
+           dict(slopes=out + 124), dict(two, weights=[weights, pool.at(2 * size - 256)]), dict(two, weights=[pool.at(size), weights]), dict(two, out=weights)]
+    for change in bad:
+        with pytest.raises(StraydogError, match="overlap|lies over"):
+            gpu.kv8_attention(**{**good, **change})
+    with pytest.raises(StraydogError, match="overlap|lies over"):
+        gpu.masked_attention(q, pool.pointer, pool.at(size), out, [1], [4], 1, 1, 64, 1, 0.1, slopes=out + 64)
+    assert not np.any(gpu.read(pool, np.uint8, (8 * size,)))
+    gpu.kv8_attention(**good)
+    gpu.kv8_attention(**{**good, **two})
+    gpu.kv8_attention(**{**good, "slopes": q})   # (what is read may be read twice)
+    gpu.release(pool)
