@@ -733,7 +733,7 @@ static void attention(Device& d, const void* const* states, const uint64_t* cont
     if (!total) return;
     attn::check_rows(d, q, total, q_stride, heads * dim, "attention queries");
     attn::check_rows(d, out, total, out_stride, heads * dim, "an attention output");
-    if (slopes) span(d, slopes, checked_product({heads, 4}), "attention slopes");
+    attn::check_slopes(d, slopes, heads);
     if (overlap(q, ((total - 1) * q_stride + heads * dim) * 2, out, ((total - 1) * out_stride + heads * dim) * 2))
         throw std::runtime_error("an attention output lies over its queries");
     const size_t out_bytes = ((total - 1) * out_stride + heads * dim) * 2;

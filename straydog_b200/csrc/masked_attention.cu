@@ -1037,6 +1037,12 @@ void check_rows(Device& d, const void* pointer, uint64_t rows, uint64_t stride, 
     if (rows) span(d, pointer, (checked_product({rows - 1, stride}) + width) * 2, what);
 }
 
+void check_slopes(Device& d, const float* slopes, uint64_t heads) {
+    if (!slopes) return;
+    if (reinterpret_cast<uintptr_t>(slopes) % 4) throw std::runtime_error("attention slopes must be 4-byte aligned");
+    span(d, slopes, checked_product({heads, 4}), "attention slopes");
+}
+
 static CUtensorMap tensor_map(const void* base, bool bf16, uint64_t dim, uint64_t heads, uint64_t rows, uint64_t head_stride, uint64_t row_stride,
                               uint32_t box_heads, uint32_t box_rows) {
     using Encode = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
@@ -1227,7 +1233,7 @@ static void masked(Device& d, const void* q, uint64_t q_stride, const void* k, u
     check_rows(d, out, total, out_stride, heads * dim, "an attention output");
     if (keys) check_rows(d, k, keys, k_stride, kv_heads * dim, "attention keys");
     if (keys) check_rows(d, v, keys, v_stride, kv_heads * dim, "attention values");
-    if (slopes) span(d, slopes, checked_product({heads, 4}), "attention slopes");
+    check_slopes(d, slopes, heads);
     const size_t out_bytes = ((total - 1) * out_stride + heads * dim) * 2;
     if (kv8::overlap(out, out_bytes, q, ((total - 1) * q_stride + heads * dim) * 2) ||
         (keys && (kv8::overlap(out, out_bytes, k, ((keys - 1) * k_stride + kv_heads * dim) * 2) || kv8::overlap(out, out_bytes, v, ((keys - 1) * v_stride + kv_heads * dim) * 2))))

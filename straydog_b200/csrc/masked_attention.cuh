@@ -17,6 +17,7 @@ struct Sequence {
 
 void check_rule(uint64_t heads, uint64_t kv_heads, uint64_t dim, float scale, float cap, int type);
 void check_rows(Device& d, const void* pointer, uint64_t rows, uint64_t stride, uint64_t width, const char* what);
+void check_slopes(Device& d, const float* slopes, uint64_t heads);
 
 // Sequences over 8-bit states whose query rows are too many for the decode kernel: their codes are unpacked to 16 bits (exactly), then the
 // prompt kernel runs over them with the blocks' scales beside.

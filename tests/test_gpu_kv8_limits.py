@@ -175,3 +175,16 @@ def test_nothing_written_lies_over_what_is_read(gpu):
     gpu.kv8_attention(**{**good, **two})
     gpu.kv8_attention(**{**good, "slopes": q})   # (what is read may be read twice)
     gpu.release(pool)
+
+
+def test_slopes_lie_on_four_byte_boundaries(gpu):
+    from straydog_b200.backend import StraydogError
+    state, q, out, slopes = gpu.buffer(state_bytes(64, 1, 64)), gpu.buffer(128), gpu.upload(np.full(64, 0x5a5a, np.int16)), gpu.buffer(64)
+    for off in (1, 2, 3, 6):
+        with pytest.raises(StraydogError, match="slopes"):
+            gpu.kv8_attention([state], [64], [9], [1], 1, 1, 64, 0, 0.1, q, out, 1, slopes=slopes.at(off))
+        with pytest.raises(StraydogError, match="slopes"):
+            gpu.masked_attention(q, state.pointer, state.pointer, out, [1], [4], 1, 1, 64, 1, 0.1, slopes=slopes.at(off))
+    assert np.all(gpu.read(out, np.int16, (64,)) == 0x5a5a)
+    for b in (state, q, out, slopes):
+        gpu.release(b)
