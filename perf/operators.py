@@ -265,15 +265,15 @@ def prepare(case, seed):
 # ---- the framework's calls ----
 
 @functools.lru_cache(maxsize=None)
-def _backend(stream):
+def _backend(device, stream):   # (the default stream is 0 on every device)
     from straydog_b200.backend import Backend
-    return Backend.adopt(torch.cuda.current_device(), stream)
+    return Backend.adopt(device, stream)
 
 
 def _own(st):
     from straydog_b200 import backend as b
     case = st["case"]
-    gpu = _backend(torch.cuda.current_stream().cuda_stream)
+    gpu = _backend(torch.cuda.current_device(), torch.cuda.current_stream().cuda_stream)
     kind = {"f32": b.F32, "f16": b.F16, "bf16": b.BF16}.get(case.get("dtype"))
     code = {"int8": b.INT8, "e4m3": b.E4M3}.get(case.get("code"))
     op, kv_heads, dim = case["op"], case["kv_heads"], case["dim"]
