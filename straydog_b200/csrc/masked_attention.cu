@@ -282,7 +282,7 @@ template<int ROWS> struct Run {
     }
 };
 
-template<int D, bool BF16, bool RULE>
+template<int D, bool BF16, bool RULE, bool KV8>   // KV8: keys and values are codes with scales beside (a path without them is 6 % faster than one that asks)
 __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __grid_constant__ Args a) {
     using S = Shape<D>;
     constexpr int T = S::kTiles, kGroups = T;   // a softmax thread's groups of 32 columns of S
@@ -396,7 +396,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
             const int position = u.length - int(sequence.rows) + int(token);
             const float slope = RULE && a.slopes && valid ? a.slopes[head] * 1.4426950408889634f : 0.0f;
             // 8-bit states: a tile's factors are 12 floats, [scores' | weights' log2 | rests] x [four groups of 32 keys]
-            const float* table_at = a.block_table ? a.block_table + (size_t(u.kv) * a.table_blocks + sequence.first_block) * 3 + half : nullptr;
+            const float* table_at = KV8 ? a.block_table + (size_t(u.kv) * a.table_blocks + sequence.first_block) * 3 + half : nullptr;
             float top_run = -INFINITY, sum_run = 0.0f;
             #pragma unroll 1
             for (uint32_t i = 0; i < tiles; ++i) {
@@ -406,7 +406,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
                 bool rests = false;
                 #pragma unroll
                 for (int g = 0; g < kGroups; ++g) { to_score[g] = 1.0f; shift[g] = 0.0f; to_sum[g] = 1.0f; rest[g] = 1.0f; }
-                if (table_at) {
+                if (KV8) {
                     // (plain loads: the kernel before this one, whose programmatic dependent it is, may still have been writing the table when it was launched)
                     const float* table = table_at + key0 / 128 * 12 + key0 / 64 % 2 * 2;
                     load_factors(table, to_score); load_factors(table + 4, shift); load_factors(table + 8, rest);
@@ -593,23 +593,24 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
                     for (int g = 0; g < kGroups; ++g) {
                         uint32_t bits[32];
                         tmem_load32(s_base + 32 * g, bits);
-                        const float c = RULE && a.slopes ? 1.0f : RULE && a.cap > 0.0f ? a.cap : score_factor(of(to_score, g)), d = of(shift, g) - under, down = of(rest, g);
+                        const float c = RULE && a.slopes ? 1.0f : RULE && a.cap > 0.0f ? a.cap : score_factor(of(to_score, g)), d = of(shift, g) - under;
                         tmem_load_wait(bits);
                         float sum0 = 0.0f, sum1 = 0.0f;
                         #pragma unroll
                         for (int n = 0; n < 16; ++n) {
                             const float p0 = fast_exp2(fmaf(__uint_as_float(bits[2 * n]), c, d)), p1 = fast_exp2(fmaf(__uint_as_float(bits[2 * n + 1]), c, d));
-                            bits[2 * n] = __float_as_uint(p0); bits[2 * n + 1] = __float_as_uint(p1);
+                            bits[n] = BF16 ? pack_bf16x2(p0, p1) : pack_half2(p0, p1);
                             sum0 += p0; sum1 += p1;
                         }
-                        if (rests) {
+                        if (KV8 && rests) {   // (rare: once more, for the products alone)
+                            const float down = of(rest, g);
+                            tmem_load32(s_base + 32 * g, bits);
+                            tmem_load_wait(bits);
                             #pragma unroll
-                            for (int n = 0; n < 32; ++n) bits[n] = __float_as_uint(__uint_as_float(bits[n]) * down);
-                        }
-                        #pragma unroll
-                        for (int n = 0; n < 16; ++n) {
-                            const float p0 = __uint_as_float(bits[2 * n]), p1 = __uint_as_float(bits[2 * n + 1]);
-                            bits[n] = BF16 ? pack_bf16x2(p0, p1) : pack_half2(p0, p1);
+                            for (int n = 0; n < 16; ++n) {
+                                const float p0 = fast_exp2(fmaf(__uint_as_float(bits[2 * n]), c, d)) * down, p1 = fast_exp2(fmaf(__uint_as_float(bits[2 * n + 1]), c, d)) * down;
+                                bits[n] = BF16 ? pack_bf16x2(p0, p1) : pack_half2(p0, p1);
+                            }
                         }
                         sum_run = fmaf(sum0 + sum1, of(to_sum, g), sum_run);
                         tmem_store16(s_base + 16 * g, bits);
@@ -642,7 +643,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
                 #pragma unroll
                 for (int r = 0; r < 4; ++r) row_at[r] = reinterpret_cast<uint16_t*>(__shfl_sync(0xffffffffu, mine, (lane & 28) + r));
             }
-            const bool patches = tiles && *flagged_piece == piece + 1;
+            const bool patches = !KV8 && tiles && *flagged_piece == piece + 1;
             if (patches) {
                 // values that were taken out of a tile: back for the rows that see them (rare: nothing here is fast)
                 #pragma unroll 1
@@ -762,7 +763,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
                 for (uint32_t f = 0; f < kAhead && f < tiles && alive; ++f) alive = score(f, tiles);
                 #pragma unroll 1
                 for (uint32_t i = 0; i < tiles && alive; ++i) {
-                    const bool look = a.values && !run.u.open(a, run.u.key(run.begin + i));
+                    const bool look = !KV8 && !run.u.open(a, run.u.key(run.begin + i));
                     const uint32_t at = done + i, slot = at % S::kVSlots;
                     const int buffer = int(i & 1);
                     // the outputs of the piece before have left O (and `flagged`)
@@ -824,7 +825,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
                     ++piece;
                 }
             }
-        } else if (warp == kLookWarp && a.values) {
+        } else if (warp == kLookWarp && !KV8) {
             // ================= masked values that are not finite =================
             uint32_t looked = 0;   // steps looked at (the next is not asked for before this one is done: the barriers' parities cannot be missed)
             for (bool more = run.start(a); more && alive; more = run.next(a)) {
@@ -1064,12 +1065,12 @@ static CUtensorMap tensor_map(const void* base, bool bf16, uint64_t dim, uint64_
     return map;
 }
 
-template<int D, bool BF16> static void launch(Device& d, Args& args, bool behind) {
+template<int D, bool BF16, bool KV8> static void launch(Device& d, Args& args, bool behind) {
     using S = Shape<D>;
     static bool configured[64] = {};
     if (!configured[d.ordinal & 63]) {
-        SDB_CHECK(cudaFuncSetAttribute(masked_attention_kernel<D, BF16, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(S::kSmem)));
-        SDB_CHECK(cudaFuncSetAttribute(masked_attention_kernel<D, BF16, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(S::kSmem)));
+        SDB_CHECK(cudaFuncSetAttribute(masked_attention_kernel<D, BF16, false, KV8>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(S::kSmem)));
+        SDB_CHECK(cudaFuncSetAttribute(masked_attention_kernel<D, BF16, true, KV8>, cudaFuncAttributeMaxDynamicSharedMemorySize, int(S::kSmem)));
         configured[d.ordinal & 63] = true;
     }
     uint32_t units = 0;
@@ -1135,7 +1136,7 @@ template<int D, bool BF16> static void launch(Device& d, Args& args, bool behind
     config.stream = d.stream;
     config.attrs = &attribute;
     config.numAttrs = behind ? 1 : 0;
-    SDB_CHECK(cudaLaunchKernelEx(&config, args.slopes || args.cap > 0.0f ? masked_attention_kernel<D, BF16, true> : masked_attention_kernel<D, BF16, false>, args));
+    SDB_CHECK(cudaLaunchKernelEx(&config, args.slopes || args.cap > 0.0f ? masked_attention_kernel<D, BF16, true, KV8> : masked_attention_kernel<D, BF16, false, KV8>, args));
     ++d.launches;
     if (args.shares) {
         config.gridDim = dim3(args.shares * S::kTiles * kM / 64);
@@ -1147,11 +1148,11 @@ template<int D, bool BF16> static void launch(Device& d, Args& args, bool behind
     }
 }
 
-static void launch_dim(Device& d, uint64_t dim, int type, Args& args, bool behind) {
+template<bool KV8> static void launch_dim(Device& d, uint64_t dim, int type, Args& args, bool behind) {
     const bool bf16 = type == kv8::kBf16;
-    if (dim == 64) bf16 ? launch<64, true>(d, args, behind) : launch<64, false>(d, args, behind);
-    else if (dim == 128) bf16 ? launch<128, true>(d, args, behind) : launch<128, false>(d, args, behind);
-    else bf16 ? launch<256, true>(d, args, behind) : launch<256, false>(d, args, behind);
+    if (dim == 64) bf16 ? launch<64, true, KV8>(d, args, behind) : launch<64, false, KV8>(d, args, behind);
+    else if (dim == 128) bf16 ? launch<128, true, KV8>(d, args, behind) : launch<128, false, KV8>(d, args, behind);
+    else bf16 ? launch<256, true, KV8>(d, args, behind) : launch<256, false, KV8>(d, args, behind);
 }
 
 static Args rule_args(uint64_t heads, uint64_t kv_heads, uint64_t dim, float scale, float cap, const float* slopes, uint64_t window, const void* q,
@@ -1210,7 +1211,7 @@ void attend_kv8(Device& d, const std::vector<Sequence>& sequences, uint64_t head
         } else {
             args.k_map = args.v_map = args.q_map;   // (no keys: nothing is loaded through them)
         }
-        launch_dim(d, dim, type, args, blocks != 0);
+        launch_dim<true>(d, dim, type, args, blocks != 0);
     }
 }
 
@@ -1253,7 +1254,7 @@ static void masked(Device& d, const void* q, uint64_t q_stride, const void* k, u
                                                                  uint32_t(prefixes ? std::min(prefixes[at], lengths[at]) : 0), uint32_t(row), uint32_t(key), 0, 0, 0};
             row += rows[at]; key += lengths[at];
         }
-        if (args.sequences) launch_dim(d, dim, type, args, false);
+        if (args.sequences) launch_dim<false>(d, dim, type, args, false);
     }
 }
 
