@@ -22,6 +22,8 @@ namespace sdb {
 namespace kv8 {
 
 using attn::any_tanh;
+using attn::either_tanh;
+using attn::kFineCap;
 using attn::kSmallTanh;
 using attn::small_tanh;
 
@@ -316,13 +318,17 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
                     for (int n = 0; n < NT; ++n)
                         #pragma unroll
                         for (int c = 0; c < 4; ++c) small &= fabsf(x[h][n][c]) <= kSmallTanh;
-                const bool all_small = __all_sync(0xffffffffu, small);   // (the usual case: scores well below the cap)
-                #pragma unroll
-                for (int h = 0; h < S::kTile / 16; ++h)
+                auto capped = [&](auto&& tanh_of) {
                     #pragma unroll
-                    for (int n = 0; n < NT; ++n)
+                    for (int h = 0; h < S::kTile / 16; ++h)
                         #pragma unroll
-                        for (int c = 0; c < 4; ++c) x[h][n][c] = fmaf(a.cap, all_small ? small_tanh(x[h][n][c]) : any_tanh(x[h][n][c]), v_log);
+                        for (int n = 0; n < NT; ++n)
+                            #pragma unroll
+                            for (int c = 0; c < 4; ++c) x[h][n][c] = fmaf(a.cap, tanh_of(x[h][n][c]), v_log);
+                };
+                if (__all_sync(0xffffffffu, small)) capped([](float y) { return small_tanh(y); });   // (the usual case: scores well below the cap)
+                else if (a.cap <= kFineCap) capped([](float y) { return any_tanh(y); });
+                else capped([](float y) { return either_tanh(y); });
             }
             if (a.slopes) {
                 #pragma unroll

@@ -535,9 +535,12 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
                                     const float y = __uint_as_float(bits[n]) * c, z = y * y;
                                     bits[n] = __float_as_uint(fmaf(fmaf(fmaf(z, -17.0f / 315.0f, 2.0f / 15.0f), z, -1.0f / 3.0f) * z, y, y));
                                 }
-                            } else {
+                            } else if (a.cap <= kFineCap) {
                                 #pragma unroll
                                 for (int n = 0; n < 32; ++n) bits[n] = __float_as_uint(any_tanh(__uint_as_float(bits[n]) * c));
+                            } else {
+                                #pragma unroll
+                                for (int n = 0; n < 32; ++n) bits[n] = __float_as_uint(either_tanh(__uint_as_float(bits[n]) * c));
                             }
                             c = a.cap;
                         } else {

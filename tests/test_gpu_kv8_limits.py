@@ -188,3 +188,37 @@ def test_slopes_lie_on_four_byte_boundaries(gpu):
     assert np.all(gpu.read(out, np.int16, (64,)) == 0x5a5a)
     for b in (state, q, out, slopes):
         gpu.release(b)
+
+
+# ---- scores far past a cap ----
+
+@pytest.mark.parametrize("kind", [1, 30])
+@pytest.mark.parametrize("dim,rows", [(64, 1), (128, 3), (256, 1), (64, 90), (128, 80), (256, 70)])
+@pytest.mark.parametrize("cap", [1e3, 1e5])
+def test_a_score_far_under_a_large_cap_leaves_the_others_theirs(gpu, kind, dim, rows, cap):
+    # keys with scores of -cap / 3: their weight is 0, and the others' scores, of a few units under the cap's curve, are as exact as without them
+    rng = np.random.default_rng(dim + rows)
+    n, heads, kv_heads = 256, 4, 2
+    k, v = (rng.normal(size=(n, kv_heads, dim)).astype(np.float32) for _ in range(2))
+    q = rng.normal(size=(rows, heads, dim)).astype(np.float32)
+    q[:, :, 0], k[:, :, 0] = 16.0, 0.0
+    k[3::64] = 0.0
+    k[3::64, :, 0] = -cap / 3 * dim ** 0.5 / 16
+    v[3::64] = 0.0
+    (qr, qh), (kr, kh), (vr, vh) = (to_bits(x, kind) for x in (q, k, v))
+    buffers = [gpu.upload(x) for x in (qr, kr, vr)]
+    out = gpu.buffer(rows * heads * dim * 2)
+    gpu.masked_attention(*(b.pointer for b in buffers), out, [rows], [n], heads, kv_heads, dim, kind, dim ** -0.5, cap=cap)
+    got = from_bits(gpu.read(out, np.int16, (rows, heads, dim)), kind)
+    want, _, size = attention(qh, kh, vh, dim ** -0.5, cap=cap)
+    limit = EPS[kind] * np.abs(want) + (EPS[kind] + 2.0 ** -16) * size + 1e-7
+    assert np.all(np.abs(got - want) <= limit), float((np.abs(got - want) / limit).max())
+    for b in buffers + [out]:
+        gpu.release(b)
+    # 8-bit rows: the same over the codes that the small keys keep (blocks of their own for the large ones)
+    k[:32], k[32:] = np.concatenate([k[3::64]] * 8), np.where(np.arange(224)[:, None, None] % 64 == 35, 0, k[32:])
+    state = State(n, kv_heads, dim, 0).write(0, k, v)
+    got, _, held = attend(gpu, [state], [n], [rows], heads, q, kind, cap=cap)
+    want, _, size = attention(held, *state.values(n), dim ** -0.5, cap=cap)
+    limit = EPS[kind] * np.abs(want) + (EPS[kind] + 2.0 ** -16) * size + 1e-7
+    assert np.all(np.abs(got - want) <= limit), float((np.abs(got - want) / limit).max())
