@@ -366,7 +366,7 @@ int sdx_kv8_write(void* handle, void* const* states, const uint64_t* contexts, c
    [contexts[s]] F32, to which every seen position's softmax weight is added, summed over the rows and the heads of its K/V head, for at
    most 64 query rows (rows * heads / kv_heads) a K/V head. Up to 64 such query rows a K/V head run on the decode kernel, more on the prompt
    kernel. A position's codes and scale must have been written. Weights enter the products
-   with the values in 16 bits, relative to the largest product of weight and value scale that the row sees: values of blocks whose scale is below 2^-88, or
+   with the values in FP16, relative to the largest product of weight and value scale that the row sees: values of blocks whose scale is below 2^-88, or
    below 2^-64 of their K/V head's largest, may be off by 2^-113, or by 2^-96 of that head's largest value. */
 int sdx_kv8_attention(void* handle, const void* const* states, const uint64_t* contexts, const uint64_t* lengths, const uint64_t* rows,
                       uint64_t sequences, uint64_t heads, uint64_t kv_heads, uint64_t dim, int code, float scale, float cap,
@@ -375,8 +375,8 @@ int sdx_kv8_attention(void* handle, const void* const* states, const uint64_t* c
 /* The same attention over 16-bit keys and values of packed documents: document d has rows[d] queries and lengths[d] keys, one behind the
    other in q, out ([heads][dim] rows) and k, v ([kv_heads][dim] rows), each with its own row stride in elements (0: packed), so that the parts
    of one projection's rows can be given as they are; rows on 16-byte boundaries. A row sees keys of its own document only, by the rule
-   above (a prefix of lengths[d]: every key). What a row does not see does not reach its output, infinities and NaN included. dim 64, 128
-   or 256, type 1 (F16) or 30 (BF16), heads / kv_heads <= 128. */
+   above (a prefix of lengths[d]: every key). What a row does not see does not reach its output, infinities and NaN included. Weights enter
+   the products with the values in the rows' type. dim 64, 128 or 256, type 1 (F16) or 30 (BF16), heads / kv_heads <= 128. */
 int sdx_masked_attention(void* handle, const void* q, uint64_t q_stride, const void* k, uint64_t k_stride, const void* v, uint64_t v_stride,
                          const uint64_t* rows, const uint64_t* lengths, uint64_t documents, uint64_t heads, uint64_t kv_heads, uint64_t dim,
                          int type, float scale, float cap, const float* slopes, uint64_t window, const uint64_t* prefixes, void* out,

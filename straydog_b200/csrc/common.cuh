@@ -75,7 +75,7 @@ struct Device {
     void* kv_stage = nullptr; uint64_t kv_stage_rows = 0;
     uint32_t* rope_rows = nullptr; size_t rope_first = 0, rope_count = 0;   // a sequence with images: three rotation positions a row (sd_rope_rows)
     uint64_t launches = 0;   // kernels launched through this handle (the benchmark's gpu_launches)
-    Workspace kv8_partial, kv8_scores, kv8_rows, kv8_kept;   // 8-bit rows: split partials, scores behind the weights, unpacked rows, an eviction's positions
+    Workspace kv8_partial, kv8_scores, kv8_rows, kv8_queries, kv8_kept;   // 8-bit rows: split partials, scores behind the weights, unpacked rows, a chunk's queries in FP16, an eviction's positions
     std::vector<void*> retired;                               // outgrown workspaces that a captured graph may still use (freed with the handle)
     bool adopted = false;    // made by sdx_adopt over another library's stream and allocations: no range checks, nothing owned but workspaces
     explicit Device(int o) : ordinal(o) {}

@@ -214,7 +214,7 @@ void sd_destroy(void* handle) {
         }
         if (value->pinned) cudaFreeHost(value->pinned);
         for (void* p : {value->work, value->partial, value->tables, value->unions, static_cast<void*>(value->turns), static_cast<void*>(value->rope_rows)}) if (p) cudaFree(p);
-        for (const Workspace& slot : {value->kv8_partial, value->kv8_scores, value->kv8_rows, value->kv8_kept}) if (slot.pointer) cudaFree(slot.pointer);
+        for (const Workspace& slot : {value->kv8_partial, value->kv8_scores, value->kv8_rows, value->kv8_queries, value->kv8_kept}) if (slot.pointer) cudaFree(slot.pointer);
         for (void* p : value->retired) cudaFree(p);
         if (value->side) { cudaStreamDestroy(value->side); cudaEventDestroy(value->side_fork); cudaEventDestroy(value->side_join); }
         if (!value->adopted) cudaStreamDestroy(value->stream);

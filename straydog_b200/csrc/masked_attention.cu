@@ -23,7 +23,8 @@
 // looks after values that some row may not see (below).
 //
 // Roundings: scores, maxima, sums and O are FP32. P is rounded to the operands' type once (FP16 or BF16), at 2^7 times its size so that FP16 keeps
-// 11 bits down to 2^-21 of the largest weight. O is multiplied in TMEM only when a row's maximum grew by more than 2^8. The keys' scales of an 8-bit
+// 11 bits down to 2^-21 of the largest weight. (The two operands of a product have one type, and FP16 does not hold what values in BF16 may be: there P has
+// 8 bits. Codes are FP16 whatever the rows are, queries brought to FP16.) O is multiplied in TMEM only when a row's maximum grew by more than 2^8. The keys' scales of an 8-bit
 // state multiply the scores, a block of 32 a factor; the values' scales join the exponent of P, and the running maximum is that of a weight times its
 // value's scale, so that P has its bits for what the row sees, however large the values are that it does not see or gives no weight. (The maximum of the
 // weights alone, with scales relative to the head's largest: a block of values 2^23 times the others, behind a row's window, left the row's FP16 P nothing.)
@@ -79,7 +80,9 @@ struct Args {
     const float* block_table;    // 8-bit states: [kv_heads][tiles of four blocks of 32 keys][12]: four key scales, log2 of four value scales (from a floor up), the rests below it
     uint32_t table_blocks;
     const uint16_t* queries;     // the query rows again, where they do not come through the map
+    const float* query_factors;  // 8-bit states under BF16 rows: [row][head] what a lifted query is to be multiplied by
     size_t query_stride;
+    uint32_t first_query;        // the row that queries, their map and their factors begin with
     const uint16_t* values;      // 16-bit rows: the values again, for the rows that see one that is not finite
     size_t value_stride;
     float scale_log2, cap, scale_over_cap;
@@ -282,10 +285,12 @@ template<int ROWS> struct Run {
     }
 };
 
-template<int D, bool BF16, bool RULE, bool KV8>   // KV8: keys and values are codes with scales beside (a path without them is 6 % faster than one that asks)
+// BF16: the type of the rows, queries and outputs. KV8: keys and values are codes with scales beside (a path without them is 6 % faster than one that asks).
+template<int D, bool BF16, bool RULE, bool KV8>
 __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __grid_constant__ Args a) {
     using S = Shape<D>;
     constexpr int T = S::kTiles, kGroups = T;   // a softmax thread's groups of 32 columns of S
+    constexpr bool kBf16 = BF16 && !KV8, kLifted = BF16 && KV8;   // the products' operands; codes are FP16, and BF16 queries are brought there
     extern __shared__ __align__(1024) uint8_t smem_raw[];
     if (!S::kSlack && smem_u32(smem_raw) % 1024) {   // (no operand layout without it: reported, not computed)
         if (threadIdx.x == 0) atomicExch(a.status, 1);
@@ -369,13 +374,13 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
             const KernelSequence& sequence = a.sequence[next.u.s];
             const uint32_t token = next.u.row + m / a.group, head = next.u.kv * a.group + m % a.group;
             const bool real = token < sequence.rows && uint32_t(m) < a.tokens * a.group;
-            const uint4* from = reinterpret_cast<const uint4*>(a.queries + (real ? (size_t(sequence.first_row) + token) * a.query_stride + size_t(head) * D + half * (D / 2) : 0));
+            const uint4* from = reinterpret_cast<const uint4*>(a.queries + (real ? (size_t(sequence.first_row - a.first_query) + token) * a.query_stride + size_t(head) * D + half * (D / 2) : 0));
             #pragma unroll 1
             for (int b = 0; b < D / 2 / 64; ++b) {
                 uint32_t w[32];
                 #pragma unroll
                 for (int n = 0; n < 8; ++n) {
-                    const uint4 v = real ? __ldg(from + 8 * b + n) : make_uint4(0, 0, 0, 0);
+                    const uint4 v = real ? from[8 * b + n] : make_uint4(0, 0, 0, 0);   // (plain: they may be the kernel's before)
                     w[4 * n] = v.x; w[4 * n + 1] = v.y; w[4 * n + 2] = v.z; w[4 * n + 3] = v.w;
                 }
                 tmem_store32(lane_base + S::kQ + half * (D / 4) + 32 * b, w);
@@ -397,6 +402,12 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
             const float slope = RULE && a.slopes && valid ? a.slopes[head] * 1.4426950408889634f : 0.0f;
             // 8-bit states: a tile's factors are 12 floats, [scores' | weights' log2 | rests] x [four groups of 32 keys]
             const float* table_at = KV8 ? a.block_table + (size_t(u.kv) * a.table_blocks + sequence.first_block) * 3 + half : nullptr;
+            float scale_log2 = a.scale_log2, scale_over_cap = a.scale_over_cap;
+            if (kLifted && tiles && valid) {
+                float factor[1];
+                load_factors(a.query_factors + (size_t(sequence.first_row - a.first_query) + token) * a.heads + head, factor);
+                scale_log2 *= factor[0]; scale_over_cap *= factor[0];
+            }
             float top_run = -INFINITY, sum_run = 0.0f;
             #pragma unroll 1
             for (uint32_t i = 0; i < tiles; ++i) {
@@ -452,7 +463,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
                             float d = shift[g] - under;
                             if (kBias) d = fmaf(-lean, float(position - int(key0) - half * 32 - 32 * g), d);
                             uint64_t d2 = kBias ? pair(d, d + lean) : both(d);
-                            const float c = a.scale_log2 * to_score[g], inner = kCap ? a.scale_over_cap * to_score[g] : 0.0f;
+                            const float c = scale_log2 * to_score[g], inner = kCap ? scale_over_cap * to_score[g] : 0.0f;
                             const uint64_t c1 = both(kCap ? c * kTanh1 : c), c3 = both(c * inner * inner * kTanh3), c5 = both(c * inner * inner * (inner * inner) * kTanh5);
                             const uint64_t step = both(2.0f * lean);
                             float farthest = 0.0f;
@@ -472,7 +483,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
                             auto weights = [&](int n, float x0, float x1) {
                                 x0 = fast_exp2(x0); x1 = fast_exp2(x1);
                                 sums = add2(sums, pair(x0, x1));
-                                packed[16 * g + n] = BF16 ? pack_bf16x2(x0, x1) : pack_half2(x0, x1);
+                                packed[16 * g + n] = kBf16 ? pack_bf16x2(x0, x1) : pack_half2(x0, x1);
                             };
                             // (exponents first and weights then, where the exponents are chains: 428 us against 495 with a bias; plain ones are 2 % faster in one go)
                             #pragma unroll
@@ -515,7 +526,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
                         return r;
                     };
                     // (a block of zero keys has a scale of 0, which a masked score of -inf must not be multiplied by)
-                    auto score_factor = [&](float key_scale) -> float { return fmaxf(a.scale_log2 * key_scale, FLT_TRUE_MIN); };
+                    auto score_factor = [&](float key_scale) -> float { return fmaxf(scale_log2 * key_scale, FLT_TRUE_MIN); };
                     const bool finish = !open || RULE;
                     float top = -INFINITY;
                     #pragma unroll 1
@@ -525,7 +536,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
                         tmem_load_wait(bits);
                         float c = of(to_score, g);
                         if (RULE && a.cap > 0.0f) {   // cap * tanh(s / cap): the cap (in the exp2 domain) stays outside
-                            c *= a.scale_over_cap;
+                            c *= scale_over_cap;
                             float most = 0.0f;
                             #pragma unroll
                             for (int n = 0; n < 32; n += 2) most = max3(most, fabsf(__uint_as_float(bits[n])), fabsf(__uint_as_float(bits[n + 1])));
@@ -602,7 +613,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
                         #pragma unroll
                         for (int n = 0; n < 16; ++n) {
                             const float p0 = fast_exp2(fmaf(__uint_as_float(bits[2 * n]), c, d)), p1 = fast_exp2(fmaf(__uint_as_float(bits[2 * n + 1]), c, d));
-                            bits[n] = BF16 ? pack_bf16x2(p0, p1) : pack_half2(p0, p1);
+                            bits[n] = kBf16 ? pack_bf16x2(p0, p1) : pack_half2(p0, p1);
                             sum0 += p0; sum1 += p1;
                         }
                         if (KV8 && rests) {   // (rare: once more, for the products alone)
@@ -612,7 +623,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
                             #pragma unroll
                             for (int n = 0; n < 16; ++n) {
                                 const float p0 = fast_exp2(fmaf(__uint_as_float(bits[2 * n]), c, d)) * down, p1 = fast_exp2(fmaf(__uint_as_float(bits[2 * n + 1]), c, d)) * down;
-                                bits[n] = BF16 ? pack_bf16x2(p0, p1) : pack_half2(p0, p1);
+                                bits[n] = kBf16 ? pack_bf16x2(p0, p1) : pack_half2(p0, p1);
                             }
                         }
                         sum_run = fmaf(sum0 + sum1, of(to_sum, g), sum_run);
@@ -734,11 +745,11 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
             // thread walking alone moved every operand there, 70 cycles a product, and was what bound the kernel.)
             const int tile = warp - kIssueWarp;
             const bool leader = elect_one();
-            const uint32_t idesc_o = instr_desc(kM, D, BF16, true);
+            const uint32_t idesc_o = instr_desc(kM, D, kBf16, true);
             const uint32_t tmem_base = __shfl_sync(0xffffffffu, tmem, 0), base = __shfl_sync(0xffffffffu, smem_u32(smem), 0);
             const uint32_t queries = desc_low(base + tile * S::kQueryBytes, 16);
             uint32_t looked = 0;
-            const uint32_t idesc_s = instr_desc(kM, kStep, BF16, false);
+            const uint32_t idesc_s = instr_desc(kM, kStep, kBf16, false);
             auto score = [&](uint32_t i, uint32_t tiles) -> bool {
                 const uint32_t at = done + i, slot = at % S::kKSlots;
                 if (!wait(kKFull + slot, (at / S::kKSlots) & 1)) return false;
@@ -804,7 +815,7 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
                         for (int tile = 0; tile < T; ++tile)
                             for (int x = 0; x < D / 64; ++x)
                                 tma_load(smem + tile * S::kQueryBytes + x * (kM * 128), &a.q_map, 64 * x, int(run.u.kv * a.group),
-                                         int(sequence.first_row + run.u.row + tile * a.tokens), &bars[kQFull]);
+                                         int(sequence.first_row - a.first_query + run.u.row + tile * a.tokens), &bars[kQFull]);
                     }
                     auto key_of = [&](uint32_t i) -> int { return int(sequence.first_key + run.u.key(run.begin + i)); };
                     auto load_k = [&](uint32_t i) {
@@ -955,27 +966,66 @@ struct UnpackArgs {
     uint32_t sequences, kv_heads, blocks;
     uint16_t* rows;       // [2 * kv_heads][blocks * 32][D]
     float* table;
+    const uint16_t* queries;   // BF16 rows to lift, or null
+    size_t query_stride;
+    uint64_t lifts;            // rows x heads
+    uint32_t heads;
+    uint16_t* lifted;          // [row][head][D]
+    float* factors;            // [row][head]
 };
 // Value scales count as 2^-88, or 2^-64 of their head's largest, where they are below: what is missing (`rest`) multiplies P then. So the sum of plain weights
 // (2^15 over the scale each, 2^24 of them) stays finite, and a weight beside a small scale, zero among them, stays in the sum: the exponential of weight times
 // scale is 2^-57 of the row's largest weight's or more.
 constexpr float kLowestScale = -88.0f, kScaleRange = 64.0f;
 
-template<int CODE, bool BF16> __device__ __forceinline__ void unpack4(uint32_t w, uint32_t (&out)[2]) {
+template<int CODE> __device__ __forceinline__ void unpack4(uint32_t w, uint32_t (&out)[2]) {
     float f[4];
     #pragma unroll
     for (int b = 0; b < 4; ++b) {
         if (CODE == kv8::kInt8) f[b] = __uint_as_float(prmt(w ^ 0x80808080u, 0x4b000000u, 0x7440u | b)) - 8388736.0f;   // 2^23 + 128 + c
         else f[b] = __uint_as_float(((w >> (8 * b)) & 0x80u) << 24 | ((w >> (8 * b)) & 0x7fu) << 20) * 1.329227995784916e36f;   // (at 2^-120 of its value)
     }
-    out[0] = BF16 ? pack_bf16x2(f[0], f[1]) : pack_half2(f[0], f[1]);
-    out[1] = BF16 ? pack_bf16x2(f[2], f[3]) : pack_half2(f[2], f[3]);
+    out[0] = pack_half2(f[0], f[1]);
+    out[1] = pack_half2(f[2], f[3]);
 }
 
-template<int D, int CODE, bool BF16>
+// BF16 queries in FP16: a warp a row and head. The whole of it is multiplied by the power of two that brings its largest value to 2^8 (exact, and what lies below
+// 2^-25 of that loses its last bits), undone on the scores. So the products of a chunk over 8-bit rows are FP16 ones, whose weights have eleven bits: in BF16
+// they had eight, and single tokens eleven. (To 2^14, as there, scores before their factor would leave the range the capped ones' polynomial is for.)
+template<int D> __device__ __forceinline__ void lift_queries(const UnpackArgs& a, uint64_t first, uint64_t step) {
+    constexpr int kWords = D / 64;
+    const int lane = threadIdx.x % 32;
+    for (uint64_t at = first; at < a.lifts; at += step) {
+        const uint32_t* from = reinterpret_cast<const uint32_t*>(a.queries + at / a.heads * a.query_stride + at % a.heads * D) + lane * kWords;
+        uint32_t w[kWords], top = 0;   // magnitudes of BF16 values compare as their bits do
+        if constexpr (kWords == 4) { const uint4 v = *reinterpret_cast<const uint4*>(from); w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w; }
+        else if constexpr (kWords == 2) { const uint2 v = *reinterpret_cast<const uint2*>(from); w[0] = v.x; w[1] = v.y; }
+        else w[0] = *from;
+        #pragma unroll
+        for (int i = 0; i < kWords; ++i) top = max(top, max(w[i] & 0x7fffu, (w[i] >> 16) & 0x7fffu));
+        top = __reduce_max_sync(0xffffffffu, top);
+        const int exponent = int(top >> 7);   // biased; 255: an infinity or a NaN among them, left as they are
+        const int lift = exponent == 255 || exponent == 0 ? 0 : min(100, 127 + 8 - exponent);
+        const float up = __uint_as_float(uint32_t(127 + lift) << 23);
+        #pragma unroll
+        for (int i = 0; i < kWords; ++i) w[i] = pack_half2(__uint_as_float(w[i] << 16) * up, __uint_as_float(w[i] & 0xffff0000u) * up);
+        uint32_t* to = reinterpret_cast<uint32_t*>(a.lifted + at * D) + lane * kWords;
+        if constexpr (kWords == 4) *reinterpret_cast<uint4*>(to) = make_uint4(w[0], w[1], w[2], w[3]);
+        else if constexpr (kWords == 2) *reinterpret_cast<uint2*>(to) = make_uint2(w[0], w[1]);
+        else *to = w[0];
+        if (lane == 0) a.factors[at] = __uint_as_float(uint32_t(127 - lift) << 23);
+    }
+}
+
+template<int D, int CODE>
 __global__ void __launch_bounds__(128) kv8_unpack_kernel(const __grid_constant__ UnpackArgs a) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const uint32_t planes = 2 * a.kv_heads;
+    if (blockIdx.y >= planes + a.kv_heads) {
+        const uint64_t block = uint64_t(blockIdx.y - planes - a.kv_heads) * gridDim.x + blockIdx.x, all = uint64_t(gridDim.y - planes - a.kv_heads) * gridDim.x;
+        lift_queries<D>(a, block * 4 + threadIdx.x / 32, all * 4);
+        return;
+    }
     if (blockIdx.y >= planes) {
         // the table of one (sequence, K/V head)
         if (blockIdx.x >= a.sequences) return;
@@ -1019,7 +1069,7 @@ __global__ void __launch_bounds__(128) kv8_unpack_kernel(const __grid_constant__
         const uint32_t w[4] = {v.x, v.y, v.z, v.w};
         uint32_t out[4][2];
         #pragma unroll
-        for (int i = 0; i < 4; ++i) unpack4<CODE, BF16>(w[i], out[i]);
+        for (int i = 0; i < 4; ++i) unpack4<CODE>(w[i], out[i]);
         uint4* at = reinterpret_cast<uint4*>(to + size_t(r) * D);
         at[0] = make_uint4(out[0][0], out[0][1], out[1][0], out[1][1]);
         at[1] = make_uint4(out[2][0], out[2][1], out[3][0], out[3][1]);
@@ -1176,6 +1226,16 @@ void attend_kv8(Device& d, const std::vector<Sequence>& sequences, uint64_t head
                 float cap, const float* slopes, uint64_t window, const void* q, uint64_t q_stride, void* out, uint64_t out_stride, int type) {
     const uint64_t total_rows = sequences.back().first_row + sequences.back().rows;
     Args args = rule_args(heads, kv_heads, dim, scale, cap, slopes, window, q, total_rows, q_stride, out, out_stride, type);
+    uint64_t lifts = 0;   // (row, head) pairs that the first unpacking launch has to lift
+    if (type == kv8::kBf16) {
+        args.first_query = uint32_t(sequences.front().first_row);
+        lifts = (total_rows - args.first_query) * heads;
+        const size_t bytes = checked_product({lifts, dim, 2});
+        auto* space = static_cast<uint8_t*>(workspace(d, d.kv8_queries, bytes + lifts * 4));
+        args.queries = reinterpret_cast<const uint16_t*>(space); args.query_stride = heads * dim;
+        args.query_factors = reinterpret_cast<const float*>(space + bytes);
+        args.q_map = tensor_map(space, false, dim, heads, total_rows - args.first_query, dim, heads * dim, args.group, args.tokens);
+    }
     constexpr uint64_t kMostBytes = uint64_t(1) << 31;   // unpacked rows a launch, unless one sequence alone has more
     for (size_t at = 0; at < sequences.size();) {
         UnpackArgs unpack{};
@@ -1199,16 +1259,24 @@ void attend_kv8(Device& d, const std::vector<Sequence>& sequences, uint64_t head
             auto* space = static_cast<uint8_t*>(workspace(d, d.kv8_rows, row_bytes + table_bytes));
             unpack.rows = reinterpret_cast<uint16_t*>(space);
             unpack.table = reinterpret_cast<float*>(space + row_bytes);
-            const dim3 grid{unsigned(std::max<uint64_t>(blocks, args.sequences)), unsigned(3 * kv_heads)};
-            const bool bf16 = type == kv8::kBf16, int8 = code == kv8::kInt8;
+            dim3 grid{unsigned(std::max<uint64_t>(blocks, args.sequences)), unsigned(3 * kv_heads)};
+            if (lifts) {
+                unpack.queries = static_cast<const uint16_t*>(q) + args.first_query * q_stride; unpack.query_stride = q_stride;
+                unpack.lifts = lifts; unpack.heads = uint32_t(heads);
+                unpack.lifted = const_cast<uint16_t*>(args.queries); unpack.factors = const_cast<float*>(args.query_factors);
+                const uint64_t lifting = (lifts + 15) / 16;   // blocks: four rows and heads a warp, more where the grid would not hold them
+                grid.y += unsigned(std::min<uint64_t>((lifting + grid.x - 1) / grid.x, 32768));
+                lifts = 0;
+            }
+            const bool int8 = code == kv8::kInt8;
             auto go = [&](auto* kernel) { kernel<<<grid, 128, 0, d.stream>>>(unpack); };
-            if (dim == 64) go(int8 ? (bf16 ? kv8_unpack_kernel<64, 0, true> : kv8_unpack_kernel<64, 0, false>) : (bf16 ? kv8_unpack_kernel<64, 1, true> : kv8_unpack_kernel<64, 1, false>));
-            else if (dim == 128) go(int8 ? (bf16 ? kv8_unpack_kernel<128, 0, true> : kv8_unpack_kernel<128, 0, false>) : (bf16 ? kv8_unpack_kernel<128, 1, true> : kv8_unpack_kernel<128, 1, false>));
-            else go(int8 ? (bf16 ? kv8_unpack_kernel<256, 0, true> : kv8_unpack_kernel<256, 0, false>) : (bf16 ? kv8_unpack_kernel<256, 1, true> : kv8_unpack_kernel<256, 1, false>));
+            if (dim == 64) go(int8 ? kv8_unpack_kernel<64, 0> : kv8_unpack_kernel<64, 1>);
+            else if (dim == 128) go(int8 ? kv8_unpack_kernel<128, 0> : kv8_unpack_kernel<128, 1>);
+            else go(int8 ? kv8_unpack_kernel<256, 0> : kv8_unpack_kernel<256, 1>);
             ++d.launches;
             const uint64_t keys = blocks * 32;
-            args.k_map = tensor_map(unpack.rows, bf16, dim, kv_heads, keys, keys * dim, dim, 1, kStep);
-            args.v_map = tensor_map(unpack.rows + kv_heads * keys * dim, bf16, dim, kv_heads, keys, keys * dim, dim, 1, kStep);
+            args.k_map = tensor_map(unpack.rows, false, dim, kv_heads, keys, keys * dim, dim, 1, kStep);
+            args.v_map = tensor_map(unpack.rows + kv_heads * keys * dim, false, dim, kv_heads, keys, keys * dim, dim, 1, kStep);
             args.block_table = unpack.table;
             args.table_blocks = uint32_t(blocks);
         } else {

@@ -19,8 +19,8 @@ void check_rule(uint64_t heads, uint64_t kv_heads, uint64_t dim, float scale, fl
 void check_rows(Device& d, const void* pointer, uint64_t rows, uint64_t stride, uint64_t width, const char* what);
 void check_slopes(Device& d, const float* slopes, uint64_t heads);
 
-// Sequences over 8-bit states whose query rows are too many for the decode kernel: their codes are unpacked to 16 bits (exactly), then the
-// prompt kernel runs over them with the blocks' scales beside.
+// Sequences over 8-bit states whose query rows are too many for the decode kernel: their codes are unpacked to FP16 (exactly) and BF16
+// queries brought to it by powers of two, then the prompt kernel runs over them with the scales beside.
 void attend_kv8(Device& d, const std::vector<Sequence>& sequences, uint64_t heads, uint64_t kv_heads, uint64_t dim, int code, float scale,
                 float cap, const float* slopes, uint64_t window, const void* q, uint64_t q_stride, void* out, uint64_t out_stride, int type);
 

@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from kv8_util import EPS, State, attention, evict, from_bits, rounded, state_bytes, to_bits
+from kv8_util import EPS, State, attention, evict, from_bits, random_state, rounded, state_bytes, to_bits
 from test_gpu_kv8_attention import attend, check
 
 pytestmark = pytest.mark.gpu
@@ -222,3 +222,51 @@ def test_a_score_far_under_a_large_cap_leaves_the_others_theirs(gpu, kind, dim, 
     want, _, size = attention(held, *state.values(n), dim ** -0.5, cap=cap)
     limit = EPS[kind] * np.abs(want) + (EPS[kind] + 2.0 ** -16) * size + 1e-7
     assert np.all(np.abs(got - want) <= limit), float((np.abs(got - want) / limit).max())
+
+
+# ---- the bits of a chunk's weights ----
+
+@pytest.mark.parametrize("code", [0, 1])
+@pytest.mark.parametrize("dim,heads,kv_heads,rows", [(64, 6, 2, 70), (128, 8, 2, 150), (256, 4, 1, 90), (128, 8, 1, 8), (64, 4, 4, 1)])
+def test_weights_under_bf16_rows_keep_eleven_bits(gpu, code, dim, heads, kv_heads, rows):
+    # few rows and chunks alike: all but the output's own rounding is FP16's (half a step of each weight, 2^-16 for the FP32 arithmetic, small products)
+    rng = np.random.default_rng(dim + rows + code)
+    lengths, chunk = [700, 300, 64], [rows, max(rows // 2, 1), rows]
+    states = [random_state(rng, rounded(n), kv_heads, dim, code, n) for n in lengths]
+    for size in (1.0, 1e-20):   # (rows of any size: a power of two brings them to FP16)
+        q = (rng.normal(size=(sum(chunk), heads, dim)) * size).astype(np.float32)
+        got, _, held = attend(gpu, states, lengths, chunk, heads, q, 30)
+        row = 0
+        for state, n, r in zip(states, lengths, chunk):
+            at = slice(row, row + r)
+            want, _, total = attention(held[at], *state.values(n), dim ** -0.5)
+            limit = bound(1, held[at], state, n, want, total, heads) + EPS[30] * np.abs(want)
+            assert np.all(np.abs(got[at] - want) <= limit), (size, n, float((np.abs(got[at] - want) / limit).max()))
+            row += r
+
+
+@pytest.mark.parametrize("dim,rows", [(64, 80), (128, 100), (256, 70)])
+def test_the_largest_queries_of_a_chunk(gpu, dim, rows):
+    # BF16 rows of up to 2^127 over keys of 1e-36, some rows small or zero
+    rng = np.random.default_rng(dim + rows)
+    n, heads, kv_heads = 300, 4, 2
+    x = rng.uniform(-1, 1, size=(2, n, kv_heads, dim)).astype(np.float32)
+    x[0] *= np.float32(1e-36)
+    state = State(320, kv_heads, dim, 0).write(0, x[0], x[1])
+    q = (rng.uniform(-1, 1, size=(rows, heads, dim)) * 2.0 ** 119).astype(np.float32)
+    q[0, 0] *= 2.0 ** -8
+    q[0, 1, 3] = 1.7e38
+    q[5], q[6] = 0.0, 1e-39
+    for rule in (dict(), dict(cap=3.0), dict(slopes=np.full(heads, 0.01, np.float32), window=150)):
+        got, _, held = attend(gpu, [state], [n], [rows], heads, q, 30, **rule)
+        want, _, total = attention(held, *state.values(n), dim ** -0.5, **rule)
+        limit = bound(30, held, state, n, want, total, heads, **rule)
+        assert np.all(np.abs(got - want) <= limit), float((np.abs(got - want) / limit).max())
+
+
+def test_chunks_of_bf16_rows_between_others(gpu):
+    # what is lifted begins with the first chunk's rows and has the others' between; more chunks than a launch takes
+    rng = np.random.default_rng(8)
+    lengths, rows = [90, 200, 40, 0, 300, 60] * 20, [2, 50, 3, 40, 64, 0] * 20
+    some = [random_state(rng, 320, 2, 128, 1, n) for n in lengths[:6]]
+    check(gpu, some * 20, lengths, rows, 6, 30, rng, q_pad=16, out_pad=8)
