@@ -1081,7 +1081,8 @@ __global__ void __launch_bounds__(128) kv8_unpack_kernel(const __grid_constant__
 void check_rule(uint64_t heads, uint64_t kv_heads, uint64_t dim, float scale, float cap, int type) {
     if (!heads || !kv_heads || heads % kv_heads || heads / kv_heads > kM || heads > 65535 || (dim != 64 && dim != 128 && dim != 256))
         throw std::runtime_error("invalid Straydog attention dimensions");
-    if (!(scale > 0.0f) || !(scale < 1e30f) || !(cap >= 0.0f) || !(cap < 1e30f)) throw std::runtime_error("invalid Straydog attention scale or cap");
+    // (scale / cap is what scores are multiplied by under a cap: an infinity would make a score of 0 a NaN)
+    if (!(scale > 0.0f) || !(scale < 1e30f) || !(cap >= 0.0f) || !(cap < 1e30f) || (cap > 0.0f && !(scale / cap < 1e30f))) throw std::runtime_error("invalid Straydog attention scale or cap");
     if (type != kv8::kF16 && type != kv8::kBf16) throw std::runtime_error("masked attention takes F16 (1) or BF16 (30) rows");
 }
 

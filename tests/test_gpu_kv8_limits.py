@@ -270,3 +270,17 @@ def test_chunks_of_bf16_rows_between_others(gpu):
     lengths, rows = [90, 200, 40, 0, 300, 60] * 20, [2, 50, 3, 40, 64, 0] * 20
     some = [random_state(rng, 320, 2, 128, 1, n) for n in lengths[:6]]
     check(gpu, some * 20, lengths, rows, 6, 30, rng, q_pad=16, out_pad=8)
+
+
+@pytest.mark.parametrize("scale,cap", [(1e20, 1e-20), (0.1, 1e-40), (1e29, 0.01)])
+def test_a_cap_far_below_the_scale_is_refused(gpu, scale, cap):
+    # scale / cap past 1e30: a score of 0 would be a NaN
+    from straydog_b200.backend import StraydogError
+    state, q, out = gpu.buffer(state_bytes(64, 1, 64)), gpu.buffer(128), gpu.upload(np.full(64, 0x5a5a, np.int16))
+    with pytest.raises(StraydogError, match="cap"):
+        gpu.kv8_attention([state], [64], [9], [1], 1, 1, 64, 0, scale, q, out, 1, cap=cap)
+    with pytest.raises(StraydogError, match="cap"):
+        gpu.masked_attention(q, state.pointer, state.pointer, out, [1], [4], 1, 1, 64, 1, scale, cap=cap)
+    assert np.all(gpu.read(out, np.int16, (64,)) == 0x5a5a)
+    for b in (state, q, out):
+        gpu.release(b)
