@@ -403,9 +403,9 @@ __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __g
             // 8-bit states: a tile's factors are 12 floats, [scores' | weights' log2 | rests] x [four groups of 32 keys]
             const float* table_at = KV8 ? a.block_table + (size_t(u.kv) * a.table_blocks + sequence.first_block) * 3 + half : nullptr;
             float scale_log2 = a.scale_log2, scale_over_cap = a.scale_over_cap;
-            if (kLifted && tiles && valid) {
-                float factor[1];
-                load_factors(a.query_factors + (size_t(sequence.first_row - a.first_query) + token) * a.heads + head, factor);
+            if (kLifted && tiles) {
+                float factor[1] = {0.0f};   // (M-rows without a query hold others' lifted ones: at a factor of 1 their scores made most steps take the slow pass)
+                if (valid) load_factors(a.query_factors + (size_t(sequence.first_row - a.first_query) + token) * a.heads + head, factor);
                 scale_log2 *= factor[0]; scale_over_cap *= factor[0];
             }
             float top_run = -INFINITY, sum_run = 0.0f;
