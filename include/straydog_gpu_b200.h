@@ -343,7 +343,8 @@ int sdx_attention_batch(void* handle, void* const* states, const uint64_t* conte
    for 256 columns, these carry one F32 scale for 32 rows of 64, 128 or 256 columns. A state is one allocation of sdx_kv8_bytes bytes,
    16-byte aligned: 2 * kv_heads planes (keys of head 0 .., then values) of `context` rows (a multiple of 32, at most 2^24) of `dim` one-byte
    codes, then the planes' scales, context / 32 F32 a plane. code 0: int8, value = code * scale, scale = max |x| / 127; code 1: E4M3, scale =
-   max |x| / 448. An infinity is held as its block's largest magnitude, a NaN as 0. Element types are 0 F32, 1 F16, 30 BF16. All arrays of
+   max |x| / 448. An infinity is held as its block's largest magnitude, a NaN as 0. A state's memory need not be cleared: what lies behind the
+   rows written so far is not counted on. Element types are 0 F32, 1 F16, 30 BF16. All arrays of
    per-sequence numbers and pointers are host arrays, read before the call returns; what they point to is device memory. The calls queue work
    on the handle's stream and read nothing back; they may be captured into a graph once a call of the same sizes has run (a call that would
    have to grow a workspace inside a capture is refused). Graphs of one handle share its workspaces: replays and other calls of the handle
@@ -367,7 +368,7 @@ int sdx_kv8_write(void* handle, void* const* states, const uint64_t* contexts, c
    most 64 query rows (rows * heads / kv_heads) a K/V head. Up to 64 such query rows a K/V head run on the decode kernel, more on the prompt
    kernel. A position's codes and scale must have been written. Weights enter the products
    with the values in FP16, relative to the largest product of weight and value scale that the row sees: values of blocks whose scale is below 2^-88, or
-   below 2^-64 of their K/V head's largest, may be off by 2^-113, or by 2^-96 of that head's largest value. */
+   below 2^-64 of their K/V head's largest, may be off by 2^-111, or by 2^-96 of that head's largest value. */
 int sdx_kv8_attention(void* handle, const void* const* states, const uint64_t* contexts, const uint64_t* lengths, const uint64_t* rows,
                       uint64_t sequences, uint64_t heads, uint64_t kv_heads, uint64_t dim, int code, float scale, float cap,
                       const float* slopes, uint64_t window, const uint64_t* prefixes, const void* q, uint64_t q_stride,
@@ -387,7 +388,8 @@ int sdx_masked_attention(void* handle, const void* q, uint64_t q_stride, const v
    positions 0 .. of targets[s] (another state, of target_contexts[s] positions), their weights to target_weights[s] ([kv_heads]
    [target_contexts[s]]), their positions to kept ([sequences][kv_heads][keep] int32, or null). A target block's scale is the largest among the blocks its
    rows come from; codes from a block with a smaller one are rounded again in it. Nothing written may overlap what is read or written
-   beside it. Positions behind the kept ones are not touched. The rows keep the rotation they were written with. */
+   beside it. Positions behind the kept ones are not touched. The rows keep the rotation they were written with. A kept row's position for later calls
+   is its place in the target: windows, prefixes and slopes over an evicted state count kept rows, not tokens, and other rows in every head. */
 int sdx_kv8_evict(void* handle, const void* const* states, const uint64_t* contexts, const uint64_t* lengths, const float* const* weights,
                   uint64_t sequences, uint64_t keep, uint64_t sinks, uint64_t recent, uint64_t kv_heads, uint64_t dim, int code,
                   void* const* targets, const uint64_t* target_contexts, float* const* target_weights, int32_t* kept);

@@ -2,7 +2,7 @@
 import numpy as np
 import pytest
 
-from kv8_util import EPS, State, attention, evict, from_bits, random_state, rounded, state_bytes, to_bits
+from kv8_util import EPS, TOP, State, attention, evict, from_bits, random_state, rounded, state_bytes, to_bits
 from test_gpu_kv8_attention import attend, check
 
 pytestmark = pytest.mark.gpu
@@ -64,12 +64,12 @@ def test_attention_over_an_eviction_into_memory_of_another_use(gpu, fill, code, 
 def bound(kind, held, state, length, want, size, heads, lowest=0.0, **rule):
     """What an output may be off, from what its own row sees: its rounding; the weights' (half a step of FP16 or BF16) and 2^-16 of the sum of |p v| for
     the FP32 arithmetic, as in kv8_util.tolerance; and, since a weight times its block's scale enters the products at 2^7 times its share of the row's largest
-    or more, half of 2^-24 a key of that (codes of up to 127): 127 * 2^-32 * n of the largest product, which is at most their sum. `lowest`: what a
-    value scale may be off at the low end, 127 times it a value. Outputs below the normal numbers of F16: half of 2^-24."""
+    or more, half of 2^-24 a key of that (codes of up to TOP): TOP * 2^-32 * n of the largest product, which is at most their sum. `lowest`: what a
+    value scale may be off at the low end, TOP times it a value. Outputs below the normal numbers of F16: half of 2^-24."""
     k, _ = state.values(length)
     scales = np.repeat(state.scales[state.kv_heads:], 32, 1)[:, :length].T[:, :, None].astype(np.float64)
     products, _, _ = attention(held, k, np.broadcast_to(scales, (length, state.kv_heads, held.shape[2])), held.shape[2] ** -0.5, **rule)
-    return (EPS[kind] * np.abs(want) + (EPS[kind] + 2.0 ** -16) * size + 127 * 2.0 ** -32 * length * products + 127 * lowest +
+    return (EPS[kind] * np.abs(want) + (EPS[kind] + 2.0 ** -16) * size + TOP[state.code] * 2.0 ** -32 * length * products + TOP[state.code] * lowest +
             (2.0 ** -25 if kind == 1 else 0.0))
 
 
