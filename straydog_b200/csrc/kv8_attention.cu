@@ -94,6 +94,12 @@ template<int CODE, bool KEYS> __device__ __forceinline__ void pairs_of(uint32_t 
     }
 }
 
+__device__ __forceinline__ float fast_log2(float x) {   // (-inf for subnormal numbers too: scales of values below 2^-117)
+    float y;
+    asm("lg2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 template<int D, int NT> struct Shape {
     static constexpr int kTile = D == 256 ? 16 : 32;                  // keys a tile: 8 KB of keys and values for D 128 and 256, 4 KB for 64
     static constexpr int kQueries = 8 * NT;
@@ -243,7 +249,7 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
         const int first_position = int(sequence.length) - int(sequence.rows);
         const int open_to = min(first_position, int(sequence.length) - 1), open_from = a.window ? int(sequence.length) - 1 - int(a.window) : -1;
         const int open_prefix = int(sequence.prefix);
-        float o[D / 16][NT][4], m[NT][2], l[NT][2], v_most = -INFINITY;
+        float o[D / 16][NT][4], m[NT][2], l[NT][2], v_floor = kLowestScale;
         #pragma unroll
         for (int n = 0; n < NT; ++n) {
             m[n][0] = m[n][1] = -INFINITY; l[n][0] = l[n][1] = 0.0f;
@@ -270,9 +276,8 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
             // Below 2^-88, or 2^-64 of the largest the piece has had, it counts as that, and what is missing comes off the weights' exponents on their way to FP16: the sum of
             // plain weights, at 2^10 over the scale each, stays finite with 2^24 keys, and blocks of almost nothing keep their weight in it. So do blocks of
             // zeros, whose maximum must not stand in the way of the others' weights (at a scale of 1 it took all bits of values of 1e-8).
-            const float v_true = __log2f(v_scale);
-            v_most = fmaxf(v_most, v_true);
-            const float v_log = fmaxf(v_true, fmaxf(v_most - kScaleRange, kLowestScale)), v_inverse = fast_exp2(-v_log);
+            const float v_true = fast_log2(v_scale), v_log = fmaxf(v_true, v_floor), v_inverse = fast_exp2(-v_log);
+            v_floor = fmaxf(v_floor, v_true - kScaleRange);
 
             // ---- scores ----
             float x[S::kTile / 16][NT][4];
