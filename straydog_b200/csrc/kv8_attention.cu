@@ -32,9 +32,9 @@ constexpr float kLift = 10.0f;   // log2 of what weights are multiplied by on th
 constexpr float kLowestScale = -88.0f, kScaleRange = 64.0f;   // log2 of the lowest value scale, and below the largest, that weights' exponents take
 
 // Query rows a K/V head up to which the decode kernel takes a sequence. It reads the codes again for every sixteen (eight) query rows, the prompt kernel
-// unpacks them once to 16 bits. Decode / prompt kernel, int8: 8 heads of 128, 8192 keys, 32 rows 16.6 / 34.0 us, 64 27.3 / 36.1, 128 36.9 / 37.7, 256 59.4 / 40.5;
-// 16 sequences of 4096 keys, 32 rows 65 / 156, 64 119 / 158, 96 166 / 159, 128 216 / 161; 4 heads of 64 alike (64 rows 48 / 67, 96 68 / 68), 2 of 256: 48 rows
-// 67 / 76, 64 86 / 79. One sequence of 1024 keys stays ahead to 256 rows (17.5 / 24.0 us), which a second rule would gain.
+// unpacks them once to 16 bits. Decode / prompt kernel, int8, BF16 rows: 8 heads of 128, 8192 keys, 32 rows 16.8 / 40.0 us, 64 27.9 / 42.2, 128 38.2 / 48.3, 256 61.3 / 49.2;
+// 16 sequences of 4096 keys, 32 rows 67 / 159, 64 123 / 161, 96 171 / 161, 128 224 / 161; 4 heads of 64 alike (64 rows 50 / 69, 96 70 / 69), 2 of 256: 48 rows
+// 68 / 78, 64 87 / 81. One sequence of 1024 keys stays ahead to 256 rows (18.0 / 23.0 us), which a second rule would gain.
 constexpr uint64_t kFewQueries = 64;
 
 struct AttentionSequence {
@@ -480,10 +480,10 @@ __global__ void __launch_bounds__(kThreads, 1) kv8_decode_kernel(const __grid_co
 }
 
 // Block = (unit, query): joins the partials of a unit that several warps worked on, and zeroes the rows of a sequence without keys.
-// Few partials (a batch of many sequences): 128 threads, so that all blocks run at once (4 verification rows of 16 sequences: 55.0 us against 65.2 with
-// 512; 64 sequences of up to 32768 keys: 197 against 203); many (one long sequence): 512. Where those are few blocks with long sums, four (two) of them share a row's columns: one
-// row of 8192 keys, 16/2 heads of 256 11.5 us against 17.5, 32768 keys 16.0 against 22.0; with 64 partials (1024 keys) 9.0 against 8.1, with 64 query rows
-// 22.8 against 20.8, so from more than 64 partials on, and up to two blocks an SM.
+// Few partials (a batch of many sequences): 128 threads, so that all blocks run at once (4 verification rows of 16 sequences: 55.3 us against 65.6 with
+// 512; 64 sequences of up to 32768 keys: 196 against 203); many (one long sequence): 512. Where those are few blocks with long sums, four (two) of them share a row's columns: one
+// row of 8192 keys, 16/2 heads of 256 11.8 us against 17.9, 32768 keys 17.2 against 23.2; with 64 partials (1024 keys) 8.3 against 7.6, with 64 query rows
+// 22.0 against 20.0, so from more than 64 partials on, and up to two blocks an SM.
 constexpr int kMostWarps = 2048, kFewPieces = 32;   // warps of a launch (eight an SM)
 template<int D, int kJoinThreads, int kColumns>   // kColumns: how many of a row's D / 4 pieces a block joins
 __global__ void __launch_bounds__(kJoinThreads) kv8_decode_join_kernel(const __grid_constant__ AttentionArgs a, uint32_t queries_a_unit) {

@@ -12,9 +12,10 @@
 // What bounds it: the softmax's issue slots and the tensor pipe, almost evenly. 128 columns: 64 keys of two tiles take 1780 cycles, of which the
 // products fill about 1000 (half the rate: a product of 64 keys reads Q from shared memory twice as often for its flops as one of 128) and
 // a softmax warp 1480 (64 scores a thread: load, maximum, exponential, sum, rounding, store), the rest is hand-over. Steps of 128 keys with
-// one buffer a tile left softmax and products in turn: 285 us for a chunk of 2048 rows over 8192 keys (32 / 8 heads of 128), 233 us now (1.03
-// PFLOP/s); 4096 rows over 16384 keys of 16 / 2 heads of 256 under a cap 830 us (1.16 PFLOP/s), 7 documents of up to 2100 rows 132 us. A distance
-// bias or a cap adds FMA work to the softmax: 4096 rows over 8192 keys of 32 / 8 heads of 128 take 385 us, 447 with a bias, 498 with a cap.
+// one buffer a tile left softmax and products in turn: 285 us for a chunk of 2048 rows over 8192 keys (32 / 8 heads of 128), 241 us now (1.0
+// PFLOP/s; 20 us of it unpacking codes and bringing queries to FP16); 4096 rows over 16384 keys of 16 / 2 heads of 256 under a cap 812 us (1.18 PFLOP/s), 7 documents of up to 2100 rows 131 us. A distance
+// bias or a cap adds FMA work to the softmax: 4096 rows over 8192 keys of 32 / 8 heads of 128 take 370 us, 404 with a bias, 451 to 467 with a cap of 50, 1265 with a cap
+// that most scores are past a quarter of (the slow pass).
 // Persistent blocks, one an SM: the units' steps laid end to end are cut into equal runs (a unit counts three steps more, for its first products, its masked
 // tiles and its output). A block walks its run without stopping: the next unit's first products are issued while the last one's output is written. A unit that
 // two or more blocks share leaves FP32 partials for a second kernel. (A block a unit left the last of 1.7 waves a third empty for a chunk of 2048
@@ -285,7 +286,8 @@ template<int ROWS> struct Run {
     }
 };
 
-// BF16: the type of the rows, queries and outputs. KV8: keys and values are codes with scales beside (a path without them is 6 % faster than one that asks).
+// BF16: the type of the rows, queries and outputs. KV8: keys and values are codes with scales beside (one kernel that asks took 1349 us for
+// 4096 rows over 8192 16-bit keys past a quarter of their cap, 1240 the one without).
 template<int D, bool BF16, bool RULE, bool KV8>
 __global__ void __launch_bounds__(kThreads, 1) masked_attention_kernel(const __grid_constant__ Args a) {
     using S = Shape<D>;
@@ -1137,7 +1139,8 @@ template<int D, bool BF16, bool KV8> static void launch(Device& d, Args& args, b
         units += q.blocks * args.kv_heads;
     }
     // The runs: a unit weighs its tiles and kUnitTiles more. The units of a block of rows, one a K/V head, are alike.
-    // (7 documents of up to 2100 rows: 2 steps 147.6 us, 3 132.9, 4 134.7, 6 139.0)
+    // (7 documents of up to 2100 rows, 32/8 heads of 128: 2 steps 141.8 us, 3 130.1, 4 133.1, 6 137.4; 12 of 1500, 16/16 heads of 64: 85.4, 81.3, 78.7, 78.6;
+    // 9 of 1800, 16/2 heads of 256: 207, 183, 170, 154; 30 of 400, 24/2 heads of 256: 100, 95.4, 95.4, 97.2. Wide heads, whose unit is one tile, would gain by more.)
     constexpr uint32_t kUnitTiles = 3;   // what a unit's first products, masked steps and output cost more, in steps
     uint64_t weight = 0;
     auto each_block = [&](auto&& act) {   // act(first unit, tiles of each of its kv_heads units); false ends
@@ -1149,7 +1152,10 @@ template<int D, bool BF16, bool KV8> static void launch(Device& d, Args& args, b
             }
     };
     each_block([&](uint32_t, uint32_t tiles) { weight += uint64_t(tiles + kUnitTiles) * args.kv_heads; return true; });
-    constexpr uint64_t kLeast = 8;   // what a run weighs at least, unless there are units enough
+    // What a run weighs at least, unless there are units enough: fewer and longer runs leave SMs idle, more and shorter ones join more. 4 / 8 / 16: one document
+    // of 300 rows, 16/2 heads of 256, 19.1 / 22.6 / 22.6 us; 4 of 100, 32/8 heads of 128, 9.8 / 12.8 / 12.7; one row over 8192 keys 29.4 / 29.7 / 30.8; 16 single rows
+    // over 2048 keys 33.7 each; long documents do not notice.
+    constexpr uint64_t kLeast = 8;
     const uint32_t blocks = uint32_t(std::max<uint64_t>(1, std::min<uint64_t>(std::min<uint64_t>(uint64_t(d.sms), kMostBlocks), std::max<uint64_t>(weight / kLeast, std::min<uint64_t>(units, weight / 2)))));
     uint64_t passed = 0;
     uint32_t next = 1;
