@@ -26,6 +26,7 @@ extern thread_local std::string last_error;
 
 inline void check_at(cudaError_t error, const char* file, int line) {
     if (error == cudaSuccess) return;
+    cudaGetLastError();   // (reported here: the next call must not find it again behind its own launches)
     const std::string path(file);
     const char* text = cudaGetErrorString(error);
     throw std::runtime_error(std::string(text ? text : "GPU error") + " (" + path.substr(path.find_last_of("/\\") + 1) + ":" +

@@ -284,3 +284,19 @@ def test_a_cap_far_below_the_scale_is_refused(gpu, scale, cap):
     assert np.all(gpu.read(out, np.int16, (64,)) == 0x5a5a)
     for b in (state, q, out):
         gpu.release(b)
+
+
+def test_memory_that_cannot_be_had_is_that_calls_error_alone(gpu):
+    # places for 8 x 1024 x 2^24 kept positions are 550 GB: refused. The calls behind it go on, and what they report is their own.
+    from straydog_b200.backend import StraydogError
+    rng = np.random.default_rng(3)
+    count, kv_heads, dim = 8, 1024, 64
+    states, targets = ([gpu.buffer(state_bytes(32, kv_heads, dim)) for _ in range(count)] for _ in range(2))
+    weights, moved = ([gpu.buffer(kv_heads * 32 * 4) for _ in range(count)] for _ in range(2))
+    with pytest.raises(StraydogError, match="memory"):
+        gpu.kv8_evict(states, [32] * count, [9] * count, weights, 1 << 24, 0, 0, kv_heads, dim, 0, targets, [32] * count, moved)
+    gpu.kv8_evict(states, [32] * count, [9] * count, weights, 8, 0, 0, kv_heads, dim, 0, targets, [32] * count, moved)
+    small = random_state(rng, 96, 2, dim, 1, 70)
+    check(gpu, [small], [70], [3], 4, 1, rng, weights=True)
+    for b in states + targets + weights + moved:
+        gpu.release(b)
