@@ -21,6 +21,11 @@ constexpr unsigned kSequences = 64;    // sequences a launch: their descriptors 
 constexpr int kInt8 = 0, kE4m3 = 1;
 constexpr int kF32 = 0, kF16 = 1, kBf16 = 30;   // element types by their GGML numbers, as sd_op_index_select_proj takes them
 
+// The attention kernels add the log2 of a value scale to the weights' exponents, from 2^-88, and from 2^-64 of the largest, up: so the sum of plain weights
+// (at most 2^15 over the scale each, 2^24 of them) stays finite, and a weight beside a small scale, or one of zero, stays in the sum, since the exponential of
+// weight times scale is 2^-57 of the row's largest or more.
+constexpr float kLowestScale = -88.0f, kScaleRange = 64.0f;
+
 inline size_t state_bytes(uint64_t context, uint64_t kv_heads, uint64_t dim) {
     const size_t raw = checked_product({2 * kv_heads, context, dim}) + checked_product({2 * kv_heads, context / kBlock, 4});
     return (raw + 15) / 16 * 16;

@@ -29,7 +29,6 @@ using attn::small_tanh;
 
 constexpr int kWarps = 8, kThreads = 32 * kWarps;
 constexpr float kLift = 10.0f;   // log2 of what weights are multiplied by on their way to FP16
-constexpr float kLowestScale = -88.0f, kScaleRange = 64.0f;   // log2 of the lowest value scale, and below the largest, that weights' exponents take
 
 // Query rows a K/V head up to which the decode kernel takes a sequence. It reads the codes again for every sixteen (eight) query rows, the prompt kernel
 // unpacks them once to 16 bits. Decode / prompt kernel, int8, BF16 rows: 8 heads of 128, 8192 keys, 32 rows 16.8 / 40.0 us, 64 27.9 / 42.2, 128 38.2 / 48.3, 256 61.3 / 49.2;

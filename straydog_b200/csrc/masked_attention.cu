@@ -975,10 +975,6 @@ struct UnpackArgs {
     uint16_t* lifted;          // [row][head][D]
     float* factors;            // [row][head]
 };
-// Value scales count as 2^-88, or 2^-64 of their head's largest, where they are below: what is missing (`rest`) multiplies P then. So the sum of plain weights
-// (2^15 over the scale each, 2^24 of them) stays finite, and a weight beside a small scale, zero among them, stays in the sum: the exponential of weight times
-// scale is 2^-57 of the row's largest weight's or more.
-constexpr float kLowestScale = -88.0f, kScaleRange = 64.0f;
 
 template<int CODE> __device__ __forceinline__ void unpack4(uint32_t w, uint32_t (&out)[2]) {
     float f[4];
@@ -1044,7 +1040,7 @@ __global__ void __launch_bounds__(128) kv8_unpack_kernel(const __grid_constant__
         if (threadIdx.x % 32 == 0) tops[threadIdx.x / 32] = top;
         __syncthreads();
         top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-        const float floor = fmaxf(log2f(top) - kScaleRange, kLowestScale);
+        const float floor = fmaxf(log2f(top) - kv8::kScaleRange, kv8::kLowestScale);   // (what is missing below it, `rest`, multiplies P)
         float* to = a.table + (size_t(kv) * a.blocks + q.first_block) * 3;
         for (uint32_t i = threadIdx.x; i < q.blocks; i += 128) {
             const float scale = i < real ? v[i] : 0.0f, exponent = log2f(scale);   // (-inf for a block of zeros: any rest serves)
